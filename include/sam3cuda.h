@@ -53,6 +53,9 @@ typedef enum {
 typedef enum { SAM3_SCORE_L2 = 0, SAM3_SCORE_L1 = 1 } sam3_score_norm_t;
 typedef enum { SAM3_ORDER_INDEX = 0, SAM3_ORDER_SCORE = 1 } sam3_keep_order_t;
 
+/* 16-bit element types of the operators that take both. */
+typedef enum { SAM3_F16 = 0, SAM3_BF16 = 1 } sam3_dtype_t;
+
 typedef struct sam3_ctx sam3_ctx_t;
 
 /* Encoder configuration. Reference: SAM3EncoderConfig.swift:6-64 and the
@@ -135,6 +138,22 @@ typedef struct {
   const sam3_block_weights_t* blocks;
   int32_t num_blocks;
 } sam3_windowed_encoder_weights_t;
+
+/* A paged cache of keys and values held in 8 bits (device pointers, caller-
+ * owned). k, v: e4m3 codes [num_pages, kv_heads, page_size, head_dim], 16-byte
+ * aligned; k_scale, v_scale: f32 [num_pages, kv_heads]. A code stands for its
+ * e4m3 value times its page's and head's scale, a power of two that
+ * sam3_kv_append keeps. page_size 16, 32, 64 or 128 tokens; head_dim 64 or 128.
+ * Which pages hold a sequence's tokens is told by a page table, int32
+ * [n_seqs, table_stride]: token t is in page table[seq][t / page_size]. Fresh
+ * pages need no initialisation. */
+typedef struct {
+  uint8_t* k;
+  uint8_t* v;
+  float* k_scale;
+  float* v_scale;
+  int32_t num_pages, page_size, kv_heads, head_dim;
+} sam3_kv_cache_t;
 
 /* ---- context ------------------------------------------------------------ */
 /* Fill *cfg with the benchmark defaults listed above. Reference: the
@@ -227,6 +246,78 @@ sam3_status_t sam3_rope_apply(sam3_ctx_t* ctx, uint16_t* qkv, int32_t m, int32_t
 sam3_status_t sam3_attention(sam3_ctx_t* ctx, const uint16_t* qkv, int32_t batch,
                              int32_t seq, int32_t heads, int32_t head_dim, float scale,
                              uint16_t* o);
+
+/* ---- packed prompts and the 8-bit cache ------------------------------------
+ * No counterpart in the reference, whose attention has one length per call and
+ * as many K/V heads as heads. These serve what consumes the encoder's tokens:
+ * prompts of image and text tokens of different lengths, then answers (or the
+ * tokens of later frames) one or a few at a time.
+ *
+ * Rows are tokens; a row's heads are contiguous (head h at h * head_dim), so
+ * q, k and v may be parts of one projection's rows. Row strides are in elements,
+ * multiples of 8; all pointers to rows are 16-byte aligned. dtype is one of
+ * sam3_dtype_t, the same for all rows of a call. heads is a multiple of
+ * kv_heads: heads [i * heads / kv_heads, ...) share K/V head i. scale > 0.
+ *
+ * Sequences: cu (int32 [n_seqs + 1], on the device) gives each sequence's first
+ * row and the end of the last; rows is the row count of the buffers, cu[n_seqs]
+ * <= rows. A sequence may have no rows. Rows that belong to no sequence are
+ * neither read for others nor written. Lengths, offsets and page numbers are
+ * read on the device and checked there: a sequence whose offsets or lengths do
+ * not fit the buffers is skipped, a page number outside the pool hides that
+ * page's tokens (sam3_attention_cached) or drops them (sam3_kv_append), and
+ * the next sam3_sync returns SAM3_ERR_INVALID_ARG. Keys that a row does not see
+ * take no part in it, whatever their rows hold, infinities and NaN included.
+ *
+ * All three can be captured into CUDA graphs and replayed with other lengths
+ * and page tables in the same buffers; the replays of one context are
+ * serialised by the caller, like its calls. */
+
+/* o [rows, heads, head_dim] = softmax attention of each row over its own
+ * sequence's rows: all of them, or with causal != 0 those up to itself.
+ * head_dim 64 or 128. Accumulation and softmax in fp32; the weights are rounded
+ * to dtype before they multiply v. o must not overlap q, k or v. */
+sam3_status_t sam3_attention_packed(sam3_ctx_t* ctx, int32_t dtype, const uint16_t* q,
+                                    int64_t q_stride, const uint16_t* k, int64_t k_stride,
+                                    const uint16_t* v, int64_t v_stride, const int32_t* cu,
+                                    int32_t n_seqs, int32_t rows, int32_t heads, int32_t kv_heads,
+                                    int32_t head_dim, float scale, int32_t causal, uint16_t* o,
+                                    int64_t o_stride);
+
+/* Write the new tokens' rows k, v [rows, kv_heads, head_dim] into the cache.
+ * seq_lens (int32 [n_seqs], on the device) counts each sequence's tokens with
+ * the new ones, which take its last positions; cu_new NULL means one new row
+ * per sequence (row i for sequence i, max_new 1). max_new: the most new tokens
+ * of one sequence. For each page and head that receives tokens the scale is 2^e,
+ * e the least integer in [-60, 60] with the largest finite |new value| <= 448 *
+ * 2^e; in a page that held tokens of the sequence it does not go below the
+ * page's scale, and where it rises, the held codes are re-rounded to it. Codes
+ * are value / scale rounded to the nearest e4m3, ties to even; infinities and
+ * values beyond 448 scales become +-448, NaN stays NaN. Calling again with the
+ * same arguments leaves the cache as it is. Pages that receive tokens must
+ * belong to one sequence each (shared pages: copy before writing). */
+sam3_status_t sam3_kv_append(sam3_ctx_t* ctx, const sam3_kv_cache_t* cache, int32_t dtype,
+                             const uint16_t* k, int64_t k_stride, const uint16_t* v,
+                             int64_t v_stride, const int32_t* cu_new, int32_t n_seqs,
+                             int32_t rows, int32_t max_new, const int32_t* page_table,
+                             int32_t table_stride, const int32_t* seq_lens);
+
+/* Sequences per sam3_attention_cached call. */
+#define SAM3_CACHED_MAX_SEQS 1024
+
+/* o [rows, heads, head_dim] = attention of each sequence's newest tokens over
+ * its tokens in the cache, the newest among them (sam3_kv_append comes first,
+ * with the same cu_new, max_new, page_table and seq_lens). With causal != 0 a
+ * new token sees the tokens up to itself, else all of its sequence. Made for
+ * one or a few new tokens per sequence: up to 64 query rows (new tokens times
+ * heads per K/V head) read the cache once, more read it again for each 64.
+ * Sequences may share pages. n_seqs <= SAM3_CACHED_MAX_SEQS. */
+sam3_status_t sam3_attention_cached(sam3_ctx_t* ctx, const sam3_kv_cache_t* cache, int32_t dtype,
+                                    const uint16_t* q, int64_t q_stride, const int32_t* cu_new,
+                                    int32_t n_seqs, int32_t rows, int32_t max_new,
+                                    const int32_t* page_table, int32_t table_stride,
+                                    const int32_t* seq_lens, int32_t heads, float scale,
+                                    int32_t causal, uint16_t* o, int64_t o_stride);
 
 /* Capacity of sam3_prune_noalloc's fixed score scratch (batch * seq rows). */
 #define SAM3_PRUNE_NOALLOC_MAX_ROWS 65536

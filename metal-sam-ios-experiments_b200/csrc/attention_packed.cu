@@ -1,0 +1,702 @@
+// attention_packed.cu - softmax attention over packed sequences of different
+// lengths, causal or not, with grouped K/V heads, on the sm_100a tensor cores.
+//
+// o[i, h] = sum_j p_ij v_j / sum_j p_ij, p_ij = 2^(c q_i . k_j - m_i), c =
+// scale log2(e), over the rows j of i's sequence (j <= i if causal); m_i is a
+// running maximum, so one pass over the keys suffices.
+//
+// A query tile is 128 rows of one sequence and head; keys come in tiles of 128.
+//   head_dim 64: one query tile per CTA, two CTAs per SM; S (fp32 scores, 128
+//     TMEM columns), P (64) and O (64) apart, so that the next S = Q K^T runs
+//     while this tile's exponentials are computed.
+//   head_dim 128: two query tiles per CTA sharing K and V, one CTA per SM. Two
+//     CTAs would each stream K and V: 64 KB per key tile and query tile, near
+//     what L2 delivers. The two tiles are two heads of one K/V head where the
+//     group is even (the same keys, the same causal length), else 256 rows of
+//     one head. P takes the first half of its S's columns (TMEM is full: two S,
+//     two O of 128); the next Q K^T of a tile is issued right behind the P V
+//     that reads P: the tensor pipe runs one thread's MMAs in order. While one
+//     tile's MMAs run, the other's softmax does.
+// Warps: 0 TMA producer, 1 TMEM allocator and MMA issuer (one thread), then
+// four softmax warps per query tile, one thread per row: the row's 128 scores
+// to registers, maximum, exponentials, P back to TMEM. O is rescaled in place,
+// and only when a row's maximum grew by more than 2^8.
+//
+// Masked places: scores are replaced before the maximum, whatever they are. V
+// needs more, because 0 * inf is NaN: in a sequence's last key tile and in the
+// causal diagonal ones, warp 0 zeroes the V rows behind the sequence's end and,
+// on the diagonal, the infinities and NaN of rows that only some queries see,
+// before the MMA reads the tile; those are added to the rows that see them at
+// the end (rare; read again from global memory).
+//
+// P is rounded to the inputs' type, as tcgen05 takes both operands in one: half
+// a step (fp16 2^-11, bf16 2^-8) of each weight.
+#include <algorithm>
+
+#include "common.cuh"
+#include "internal.h"
+
+#include <cuda_bf16.h>
+
+namespace sam3 {
+namespace {
+
+constexpr int BQ = 128, BKV = 128;
+constexpr int KST = 3, VST = 2;
+
+template <int D>
+struct PK {
+  static constexpr int T = D == 128 ? 2 : 1;     // query tiles per CTA
+  static constexpr bool OVERLAY = D == 128;      // P in its S's columns
+  static constexpr int HALVES = D / 64;          // 128-byte wide parts of a tile
+  static constexpr int THREADS = 64 + 128 * T;
+  static constexpr int TILE = BKV * D * 2;       // bytes of a Q, K or V tile
+  static constexpr int HALF = BKV * 128;
+  static constexpr int OFF_K = T * TILE;
+  static constexpr int OFF_V = OFF_K + KST * TILE;
+  static constexpr int OFF_BAR = OFF_V + VST * TILE;
+  // q_full[T], k_full/k_empty[KST], v_full/v_empty[VST], v_raw, s_full[T],
+  // s_free, p_full[T], o_full, o_done[T], drain
+  static constexpr int BARS = 4 * T + 2 * KST + 2 * VST + 4;
+  static constexpr int OFF_MISC = OFF_BAR + BARS * 8;
+  static constexpr int MISC = 80;
+  static constexpr int SMEM = OFF_MISC + MISC + 1024;
+  static constexpr uint32_t COLS = D == 128 ? 512 : 256;
+  static constexpr uint32_t S(int t) { return 128u * t; }
+  static constexpr uint32_t P(int t) { return OVERLAY ? 128u * t : 128u; }
+  static constexpr uint32_t O(int t) { return OVERLAY ? 256u + 128u * t : 192u; }
+};
+static_assert(2 * (PK<64>::SMEM + 1024) <= 228 * 1024 && 3 * PK<64>::SMEM > 228 * 1024,
+              "exactly two CTAs per SM: 256 TMEM columns each");
+static_assert(PK<128>::SMEM <= 227 * 1024 && 2 * PK<128>::SMEM > 228 * 1024, "one CTA per SM");
+
+struct PackedArgs {
+  uint16_t* o;
+  const uint16_t* v;
+  const int32_t* cu;
+  int* err;
+  int64_t o_stride, v_stride;
+  int n_seqs, rows, group;
+  int pair_heads;  // the CTA's two tiles are two heads (else 256 rows of one)
+  int units;       // heads, or pairs of heads
+  int causal;
+  float c;         // scale * log2(e)
+  int o32;         // o's rows are 32-byte aligned
+};
+
+struct Item {
+  int row0, len, tile;
+};
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if (BF) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return pack_half2(lo, hi);
+}
+// 0xFFFF in each half of w that is an infinity or NaN.
+template <bool BF>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  constexpr uint32_t E = BF ? 0x7F807F80u : 0x7C007C00u;
+  return __vcmpeq2(w & E, E);
+}
+
+// Which sequence and tile of `span` rows the CTA's tile number means, counted
+// from the last tile backwards (in a causal sequence the last tiles have the
+// most keys). By one warp; tile < 0: none.
+__device__ Item find_item(const PackedArgs& a, int span, int number) {
+  const int lane = threadIdx.x & 31;
+  auto tiles = [&](int i, int& r0, int& len) {
+    r0 = len = 0;
+    if (i >= a.n_seqs) return 0;
+    r0 = a.cu[i];
+    const int r1 = a.cu[i + 1];
+    if (!rows_fit(r0, r1, a.rows)) {
+      atomicExch(a.err, kDevErrBadLengths);
+      r0 = 0;
+      return 0;
+    }
+    len = r1 - r0;
+    return (len + span - 1) / span;
+  };
+  int seen = 0;
+  for (int i0 = (a.n_seqs - 1) / 32 * 32; i0 >= 0; i0 -= 32) {
+    int r0, len;
+    const int mine = tiles(i0 + 31 - lane, r0, len);  // lane 0 has the last sequence
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += u;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, seen + sum > number);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      Item it;
+      it.row0 = __shfl_sync(0xffffffffu, r0, l);
+      it.len = __shfl_sync(0xffffffffu, len, l);
+      const int end = seen + __shfl_sync(0xffffffffu, sum, l);
+      it.tile = end - 1 - number;
+      return it;
+    }
+    seen += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return {0, 0, -1};
+}
+
+template <int D, bool BF>
+__global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
+    packed_attn_kernel(const __grid_constant__ CUtensorMap map_q,
+                       const __grid_constant__ CUtensorMap map_k,
+                       const __grid_constant__ CUtensorMap map_v, const PackedArgs a) {
+  using C = PK<D>;
+  constexpr int T = C::T;
+  constexpr uint32_t FMT = BF ? (1u << 7) | (1u << 10) : 0u;  // bf16 operands
+  constexpr uint32_t IDESC_S = umma_idesc_f16(128, BKV, 0) | FMT;
+  constexpr uint32_t IDESC_O = umma_idesc_f16(128, D, 1) | FMT;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t sbase = smem_u32(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  const uint32_t bar_q = sbase + C::OFF_BAR;
+  const uint32_t bar_k_full = bar_q + 8 * T;
+  const uint32_t bar_k_empty = bar_k_full + 8 * KST;
+  const uint32_t bar_v_full = bar_k_empty + 8 * KST;
+  const uint32_t bar_v_empty = bar_v_full + 8 * VST;
+  const uint32_t bar_v_raw = bar_v_empty + 8 * VST;  // a V tile that warp 0 looks through
+  const uint32_t bar_s_full = bar_v_raw + 8;         // [T] Q K^T done (and the P V before it)
+  const uint32_t bar_s_free = bar_s_full + 8 * T;    // scores are in registers (P apart)
+  const uint32_t bar_p_full = bar_s_free + 8;        // [T] P written
+  const uint32_t bar_o_full = bar_p_full + 8 * T;    // P V done (P apart)
+  const uint32_t bar_o_done = bar_o_full + 8;        // [T] after the last P V
+  const uint32_t bar_drain = bar_o_done + 8 * T;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
+  volatile int* item_slot = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
+  int* fix_tile = reinterpret_cast<int*>(smem + C::OFF_MISC + 20);         // [2]
+  uint32_t* fix_rows = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC + 28);  // [2][4]
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < T; ++t) {
+      mbar_init(bar_q + 8 * t, 1);
+      mbar_init(bar_s_full + 8 * t, 1);
+      mbar_init(bar_p_full + 8 * t, 128);
+      mbar_init(bar_o_done + 8 * t, 1);
+    }
+    for (int s = 0; s < KST; ++s) {
+      mbar_init(bar_k_full + 8 * s, 1);
+      mbar_init(bar_k_empty + 8 * s, 1);
+    }
+    for (int s = 0; s < VST; ++s) {
+      mbar_init(bar_v_full + 8 * s, 1);
+      mbar_init(bar_v_empty + 8 * s, 1);
+    }
+    mbar_init(bar_v_raw, 1);
+    mbar_init(bar_s_free, 128);
+    mbar_init(bar_o_full, 1);
+    mbar_init(bar_drain, 1);
+    *abort_flag = 0;
+    for (int i = 0; i < 2; ++i) fix_tile[i] = 0;
+    for (int i = 0; i < 8; ++i) fix_rows[i] = 0;
+    fence_mbar_init();
+    prefetch_tmap(&map_q);
+    prefetch_tmap(&map_k);
+    prefetch_tmap(&map_v);
+  }
+  griddep_launch_dependents();
+  griddep_wait();  // offsets and rows may be earlier kernels' outputs
+  const int unit = blockIdx.x % a.units;
+  if (warp == 0) {
+    const Item it = find_item(a, T == 2 && !a.pair_heads ? 256 : 128, blockIdx.x / a.units);
+    if (lane == 0) {
+      item_slot[0] = it.row0;
+      item_slot[1] = it.len;
+      item_slot[2] = it.tile;
+    }
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), C::COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int row0 = item_slot[0], len = item_slot[1], tile = item_slot[2];
+
+  if (tile >= 0) {
+    // per query tile: head, first row in the sequence, key tiles
+    const bool ph = T == 2 && a.pair_heads;
+    const int head0 = ph ? 2 * unit : unit;
+    const int q0 = T == 2 && !ph ? tile * 256 : tile * 128;
+    const int qt[2] = {q0, ph ? q0 : q0 + 128};
+    int n[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int keys = a.causal ? min(len, qt[t] + BQ) : len;
+      n[t] = t < T && qt[t] < len ? (keys + BKV - 1) / BKV : 0;
+    }
+    const int nmax = max(n[0], n[1]);
+    const int kv_head = head0 / a.group;
+
+    if (warp == 0) {
+      // ----------------------------------------------------------- producer
+      uint32_t k_bits = 0, k_par = 0, v_bits = 0, v_par = 0;  // loads to drain on abort
+      uint32_t raw_uses = 0;
+      bool ok = true;
+      if (lane == 0) {
+        for (int t = 0; t < T; ++t)
+          if (n[t]) {
+            mbar_arrive_expect_tx(bar_q + 8 * t, C::TILE);
+            tma_load_3d(sbase + t * C::TILE, &map_q, bar_q + 8 * t, 0, row0 + qt[t],
+                        (ph ? head0 + t : head0) * C::HALVES);
+          }
+      }
+      for (int j = 0; j < nmax && ok; ++j) {
+        const int ks = j % KST, vs = j % VST;
+        const uint32_t kph = (uint32_t)(j / KST) & 1u, vph = (uint32_t)(j / VST) & 1u;
+        // does some query of the CTA see a part of this tile only?
+        const bool diag = a.causal && (j == n[0] - 1 || j == n[1] - 1);
+        const bool fix = diag || (j + 1) * BKV > len;
+        if (lane == 0) {
+          ok = mbar_wait(bar_k_empty + 8 * ks, kph ^ 1, abort_flag, a.err, kDevErrTimeoutPacked);
+          if (ok) {
+            mbar_arrive_expect_tx(bar_k_full + 8 * ks, C::TILE);
+            tma_load_3d(sbase + C::OFF_K + ks * C::TILE, &map_k, bar_k_full + 8 * ks, 0,
+                        row0 + j * BKV, kv_head * C::HALVES);
+            k_bits |= 1u << ks;
+            k_par = (k_par & ~(1u << ks)) | (kph << ks);
+            ok = mbar_wait(bar_v_empty + 8 * vs, vph ^ 1, abort_flag, a.err, kDevErrTimeoutPacked);
+          }
+          if (ok) {
+            const uint32_t bar = fix ? bar_v_raw : bar_v_full + 8 * vs;
+            mbar_arrive_expect_tx(bar, C::TILE);
+            tma_load_3d(sbase + C::OFF_V + vs * C::TILE, &map_v, bar, 0, row0 + j * BKV,
+                        kv_head * C::HALVES);
+            if (!fix) {
+              v_bits |= 1u << vs;
+              v_par = (v_par & ~(1u << vs)) | (vph << vs);
+            }
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        if (ok && fix) {
+          // drained here also on abort: the wait ignores the flag
+          ok = __all_sync(0xffffffffu, mbar_wait_drain(bar_v_raw, raw_uses & 1u));
+          if (!ok && lane == 0) {
+            *abort_flag = 1;
+            atomicExch(a.err, kDevErrTimeoutPacked);
+          }
+          const int nth = raw_uses ? 1 : 0;  // at most two such tiles per CTA
+          ++raw_uses;
+          if (lane == 0) fix_tile[nth] = j;
+          __syncwarp();
+          uint4* vt = reinterpret_cast<uint4*>(smem + C::OFF_V + vs * C::TILE);
+          const int held = len - j * BKV;  // rows of the sequence in this tile
+#pragma unroll 4
+          for (int i = lane; i < C::TILE / 16; i += 32) {
+            const int r = (i >> 3) & (BKV - 1);
+            if (r >= held) {
+              vt[i] = make_uint4(0, 0, 0, 0);
+            } else if (diag) {
+              const uint4 w = vt[i];
+              const uint4 b = make_uint4(not_finite<BF>(w.x), not_finite<BF>(w.y),
+                                         not_finite<BF>(w.z), not_finite<BF>(w.w));
+              if (b.x | b.y | b.z | b.w) {
+                vt[i] = make_uint4(w.x & ~b.x, w.y & ~b.y, w.z & ~b.z, w.w & ~b.w);
+                atomicOr(&fix_rows[nth * 4 + (r >> 5)], 1u << (r & 31));
+              }
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_v_full + 8 * vs);
+        }
+      }
+      if (lane == 0 && *abort_flag) {
+        for (int t = 0; t < T; ++t)
+          if (n[t]) mbar_wait_drain(bar_q + 8 * t, 0);
+        for (int s = 0; s < KST; ++s)
+          if (k_bits & (1u << s)) mbar_wait_drain(bar_k_full + 8 * s, (k_par >> s) & 1u);
+        for (int s = 0; s < VST; ++s)
+          if (v_bits & (1u << s)) mbar_wait_drain(bar_v_full + 8 * s, (v_par >> s) & 1u);
+      }
+    } else if (warp == 1) {
+      // ----------------------------------------------------------- MMA issuer
+      if (lane == 0) {
+        bool ok = true;
+        auto wait = [&](uint32_t bar, uint32_t par) {
+          return mbar_wait(bar, par, abort_flag, a.err, kDevErrTimeoutPacked);
+        };
+        auto wait_k = [&](int j) {
+          return wait(bar_k_full + 8 * (j % KST), (uint32_t)(j / KST) & 1u);
+        };
+        auto wait_v = [&](int j) {
+          return wait(bar_v_full + 8 * (j % VST), (uint32_t)(j / VST) & 1u);
+        };
+        auto last_of = [&](int j) { return T == 2 && j < n[1] ? 1 : 0; };
+        auto issue_qk = [&](int t, int j) {
+          const uint64_t dq = umma_desc_sw128(sbase + t * C::TILE);
+          const uint64_t dk = umma_desc_sw128(sbase + C::OFF_K + (j % KST) * C::TILE);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk / 4) * C::HALF + (kk % 4) * 32;
+            umma_f16_ss(tmem + C::S(t), desc_advance(dq, off), desc_advance(dk, off), IDESC_S,
+                        kk != 0);
+          }
+          umma_commit(bar_s_full + 8 * t);
+          if (t == last_of(j)) umma_commit(bar_k_empty + 8 * (j % KST));
+        };
+        auto issue_pv = [&](int t, int j) {
+          // V tile: keys along K, head_dim along N in 64-wide groups HALF apart
+          uint64_t dv = umma_desc_sw128_mn(sbase + C::OFF_V + (j % VST) * C::TILE);
+          dv = (dv & ~(0x3FFFull << 16)) | ((uint64_t)(C::HALF >> 4) << 16);
+#pragma unroll
+          for (int kk = 0; kk < BKV / 16; ++kk)
+            umma_f16_ts(tmem + C::O(t), tmem + C::P(t) + kk * 8, desc_advance(dv, kk * 2048),
+                        IDESC_O, (j | kk) != 0);
+          if (!C::OVERLAY) umma_commit(bar_o_full);
+          if (t == last_of(j)) umma_commit(bar_v_empty + 8 * (j % VST));
+        };
+        if (C::OVERLAY) {
+          ok = wait(bar_q, 0) && wait_k(0);
+          if (ok) {
+            tc_fence_after();
+            issue_qk(0, 0);
+          }
+          if (ok && n[1]) {
+            ok = wait(bar_q + 8 * (T - 1), 0);
+            if (ok) issue_qk(1, 0);
+          }
+          for (int j = 0; j < nmax && ok; ++j) {
+            bool v_here = false, k_here = false;
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+              if (j >= n[t] || !ok) continue;
+              ok = wait(bar_p_full + 8 * t, (uint32_t)j & 1u) && (v_here || wait_v(j));
+              if (!ok) continue;
+              v_here = true;
+              tc_fence_after();
+              issue_pv(t, j);
+              if (j + 1 < n[t]) {
+                ok = k_here || wait_k(j + 1);
+                if (!ok) continue;
+                k_here = true;
+                tc_fence_after();
+                issue_qk(t, j + 1);
+              } else {
+                umma_commit(bar_o_done + 8 * t);
+              }
+            }
+          }
+        } else {
+          ok = wait(bar_q, 0) && wait_k(0);
+          if (ok) {
+            tc_fence_after();
+            issue_qk(0, 0);
+          }
+          if (ok && nmax > 1) {
+            ok = wait_k(1) && wait(bar_s_free, 0);
+            if (ok) {
+              tc_fence_after();
+              issue_qk(0, 1);
+            }
+          }
+          for (int j = 0; j < nmax && ok; ++j) {
+            ok = wait(bar_p_full, (uint32_t)j & 1u) && wait_v(j);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(0, j);
+            if (j + 2 < nmax) {
+              ok = wait_k(j + 2) && wait(bar_s_free, (uint32_t)(j + 1) & 1u);
+              if (!ok) break;
+              tc_fence_after();
+              issue_qk(0, j + 2);
+            }
+          }
+          if (ok) umma_commit(bar_o_done);
+        }
+        if (*abort_flag) {
+          umma_commit(bar_drain);
+          mbar_wait_drain(bar_drain, 0);
+        }
+      }
+    } else {
+      // ----------------------------------------------------------- softmax rows
+      constexpr float kRescaleLog2 = 8.0f;
+      const int t = T == 2 ? (warp - 2) >> 2 : 0;
+      const int quad = warp & 3;  // this warp's TMEM lane quadrant
+      const int r = quad * 32 + lane;
+      const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
+      const uint32_t s_col = lane_base + C::S(t), p_col = lane_base + C::P(t),
+                     o_col = lane_base + C::O(t);
+      const int pos = qt[t] + r;                              // row in the sequence
+      const int lim = a.causal ? min(len, pos + 1) : len;     // keys it sees
+      const int lim_min = a.causal ? min(len, qt[t] + 1) : len;  // that all rows of the tile see
+      const float c = a.c;
+      float m_run = -INFINITY, l_run = 0.f;
+      bool ok = true;
+      for (int j = 0; j < n[t] && ok; ++j) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_s_full + 8 * t, (uint32_t)j & 1u, abort_flag,
+                                               a.err, kDevErrTimeoutPacked));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t v[BKV];
+        const bool edge = (j + 1) * BKV > lim_min;
+        const int valid = lim - j * BKV;
+        float mx[4];
+        auto half_max = [&](int h0) {
+          if (edge) {
+#pragma unroll
+            for (int e = 0; e < BKV / 2; ++e)
+              if (h0 * 32 + e >= valid) v[h0 * 32 + e] = __float_as_uint(-INFINITY);
+          }
+#pragma unroll
+          for (int q = h0; q < h0 + 2; ++q) {
+            float m = fmaxf(__uint_as_float(v[32 * q]), __uint_as_float(v[32 * q + 31]));
+#pragma unroll
+            for (int e = 1; e < 31; e += 2)
+              m = max3(m, __uint_as_float(v[32 * q + e]), __uint_as_float(v[32 * q + e + 1]));
+            mx[q] = m;
+          }
+        };
+        tmem_ld_32x32b_x32(s_col, *reinterpret_cast<uint32_t(*)[32]>(v));
+        tmem_ld_32x32b_x32(s_col + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+        tmem_wait_ld();
+        tmem_ld_32x32b_x32(s_col + 64, *reinterpret_cast<uint32_t(*)[32]>(v + 64));
+        tmem_ld_32x32b_x32(s_col + 96, *reinterpret_cast<uint32_t(*)[32]>(v + 96));
+        half_max(0);
+        tmem_wait_ld();
+        if (!C::OVERLAY) {
+          tc_fence_before();
+          mbar_arrive(bar_s_free);  // the next Q K^T may overwrite S now
+        }
+        half_max(2);
+        const float m_tile = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * c;
+        const bool grow = m_tile > m_run + kRescaleLog2;
+        const float m_use = grow ? m_tile : m_run;
+        const float alpha = grow ? ex2_approx(m_run - m_use) : 1.0f;  // 0 on the first tile
+        float ls[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t pk[BKV / 2];
+#pragma unroll
+        for (int e = 0; e < BKV / 2; ++e) {
+          const float p0 = ex2_approx(fmaf(__uint_as_float(v[2 * e]), c, -m_use));
+          const float p1 = ex2_approx(fmaf(__uint_as_float(v[2 * e + 1]), c, -m_use));
+          ls[e & 3] += p0 + p1;
+          pk[e] = pack2<BF>(p0, p1);
+        }
+        if (!C::OVERLAY && j > 0) {  // P V of the tile before still reads P
+          ok = __all_sync(0xffffffffu, mbar_wait(bar_o_full, (uint32_t)(j - 1) & 1u, abort_flag,
+                                                 a.err, kDevErrTimeoutPacked));
+          if (!ok) break;
+          tc_fence_after();
+        }
+#pragma unroll
+        for (int q = 0; q < BKV / 32; ++q)
+          tmem_st_32x32b_x16(p_col + q * 16, *reinterpret_cast<uint32_t(*)[16]>(pk + 16 * q));
+        l_run = fmaf(l_run, alpha, (ls[0] + ls[1]) + (ls[2] + ls[3]));
+        m_run = m_use;
+        // tcgen05.ld/st are warp-wide: the whole warp takes the branch when any
+        // of its rows grew (alpha is 1 for the others)
+        if (j > 0 && __any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int h = 0; h < C::HALVES; ++h) {
+            uint32_t o[64];
+            tmem_ld_32x32b_x32(o_col + 64 * h, *reinterpret_cast<uint32_t(*)[32]>(o));
+            tmem_ld_32x32b_x32(o_col + 64 * h + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
+            tmem_wait_ld();
+#pragma unroll
+            for (int d = 0; d < 64; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * alpha);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              tmem_st_32x32b_x16(o_col + 64 * h + q * 16,
+                                 *reinterpret_cast<uint32_t(*)[16]>(o + 16 * q));
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar_p_full + 8 * t);
+      }
+      if (ok && n[t])
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_o_done + 8 * t, 0u, abort_flag, a.err,
+                                               kDevErrTimeoutPacked));
+      if (ok && n[t]) {
+        tc_fence_after();
+        const float inv = 1.f / l_run;
+        const int head = ph ? head0 + t : head0;
+        uint16_t* drow = a.o + (int64_t)(row0 + pos) * a.o_stride + head * D;
+#pragma unroll
+        for (int h = 0; h < C::HALVES; ++h) {
+          uint32_t o[64];
+          tmem_ld_32x32b_x32(o_col + 64 * h, *reinterpret_cast<uint32_t(*)[32]>(o));
+          tmem_ld_32x32b_x32(o_col + 64 * h + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
+          tmem_wait_ld();
+          if (pos >= len) continue;
+#pragma unroll
+          for (int d = 0; d < 64; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * inv);
+          // infinities and NaN that warp 0 took out of the diagonal V tiles
+          for (int f = 0; f < 8; ++f) {
+            uint32_t bits = fix_rows[f];
+            while (bits) {
+              const int key = fix_tile[f >> 2] * BKV + (f & 3) * 32 + __ffs(bits) - 1;
+              bits &= bits - 1;
+              if (key >= lim) continue;
+              const uint16_t* vr = a.v + (int64_t)(row0 + key) * a.v_stride + kv_head * D + 64 * h;
+#pragma unroll
+              for (int d = 0; d < 64; ++d) {
+                const uint32_t w = vr[d];
+                const float x = BF ? __uint_as_float(w << 16) : unpack_half2(w).x;
+                if (not_finite<BF>(w) & 0xFFFFu)
+                  o[d] = __float_as_uint(__uint_as_float(o[d]) + x);
+              }
+            }
+          }
+          if (a.o32) {  // 32-byte stores: whole sectors
+#pragma unroll
+            for (int c16 = 0; c16 < 4; ++c16) {
+              uint32_t w[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                w[e] = pack2<BF>(__uint_as_float(o[16 * c16 + 2 * e]),
+                                 __uint_as_float(o[16 * c16 + 2 * e + 1]));
+              st_global_v8(drow + 64 * h + 16 * c16, w);
+            }
+          } else {
+#pragma unroll
+            for (int c8 = 0; c8 < 8; ++c8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = pack2<BF>(__uint_as_float(o[8 * c8 + 2 * e]),
+                                 __uint_as_float(o[8 * c8 + 2 * e + 1]));
+              *reinterpret_cast<uint4*>(drow + 64 * h + 8 * c8) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::COLS);
+  }
+}
+
+// Rows [rows, heads * D] as (64, rows, heads * D / 64): one box brings 128 rows
+// of one head, its 64-wide parts one after another.
+template <int D>
+bool rows_map(CUtensorMap* map, const uint16_t* x, int rows, int heads, int64_t stride, bool bf) {
+  cuuint64_t dims[3] = {64, (cuuint64_t)rows, (cuuint64_t)heads * (D / 64)};
+  cuuint64_t strides[2] = {(cuuint64_t)stride * 2, 128};
+  cuuint32_t box[3] = {64, BKV, D / 64};
+  cuuint32_t es[3] = {1, 1, 1};
+  return encode_tiled()(map,
+                        bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                        const_cast<uint16_t*>(x), dims, strides, box, es,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool BF>
+sam3_status_t launch_packed(sam3_ctx_t* ctx, const uint16_t* q, int64_t q_stride,
+                            const uint16_t* k, int64_t k_stride, PackedArgs& a, int heads,
+                            int kv_heads) {
+  using C = PK<D>;
+  CUtensorMap mq, mk, mv;
+  if (!rows_map<D>(&mq, q, a.rows, heads, q_stride, BF) ||
+      !rows_map<D>(&mk, k, a.rows, kv_heads, k_stride, BF) ||
+      !rows_map<D>(&mv, a.v, a.rows, kv_heads, a.v_stride, BF))
+    return set_error(ctx, SAM3_ERR_CUDA, "attention_packed: cuTensorMapEncodeTiled failed");
+  const uint32_t bit = (uint32_t)kSmemPacked << ((D == 128) * 2 + BF);
+  const sam3_status_t st = ensure_smem_attr(ctx, bit, packed_attn_kernel<D, BF>, C::SMEM,
+                                            "attention_packed smem attribute");
+  if (st != SAM3_OK) return st;
+  a.pair_heads = C::T == 2 && a.group % 2 == 0;
+  a.units = a.pair_heads ? heads / 2 : heads;
+  const int span = C::T == 2 && !a.pair_heads ? 256 : 128;
+  // at most rows / span full tiles, and one more for each sequence with rows
+  const long long tiles = a.rows / span + std::min(a.n_seqs, a.rows);
+  if (tiles * a.units > 0x7FFFFFFFll)
+    return set_error(ctx, SAM3_ERR_SHAPE, "attention_packed: too many rows for one call");
+  const cudaError_t e = launch_pdl(packed_attn_kernel<D, BF>, dim3((unsigned)(tiles * a.units)),
+                                   dim3(C::THREADS), C::SMEM, ctx->stream, mq, mk, mv, a);
+  return check_launch_ret(ctx, e, "packed_attn_kernel");
+}
+
+}  // namespace
+
+sam3_status_t attention_packed(sam3_ctx_t* ctx, int dtype, const uint16_t* q, int64_t q_stride,
+                               const uint16_t* k, int64_t k_stride, const uint16_t* v,
+                               int64_t v_stride, const int32_t* cu, int n_seqs, int rows, int heads,
+                               int kv_heads, int head_dim, float scale, int causal, uint16_t* o,
+                               int64_t o_stride) {
+  if (!q || !k || !v || !cu || !o)
+    return set_error(ctx, SAM3_ERR_INVALID_ARG, "attention_packed: null pointer");
+  if (dtype != SAM3_F16 && dtype != SAM3_BF16)
+    return set_error(ctx, SAM3_ERR_INVALID_ARG, "attention_packed: unknown dtype %d", dtype);
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o))
+    return set_error(ctx, SAM3_ERR_INVALID_ARG, "attention_packed: rows must be 16-byte aligned");
+  if (!(scale > 0.f) || scale > 3.402823466e38f)
+    return set_error(ctx, SAM3_ERR_INVALID_ARG, "attention_packed: scale must be positive");
+  if (head_dim != 64 && head_dim != 128)
+    return set_error(ctx, SAM3_ERR_SHAPE, "attention_packed: head_dim must be 64 or 128 (got %d)",
+                     head_dim);
+  if (heads <= 0 || kv_heads <= 0 || heads > 1024 || heads % kv_heads)
+    return set_error(ctx, SAM3_ERR_SHAPE, "attention_packed: %d heads over %d K/V heads", heads,
+                     kv_heads);
+  const int64_t wide = (int64_t)heads * head_dim, narrow = (int64_t)kv_heads * head_dim;
+  if (!stride_ok(q_stride, wide) || !stride_ok(o_stride, wide) || !stride_ok(k_stride, narrow) ||
+      !stride_ok(v_stride, narrow))
+    return set_error(ctx, SAM3_ERR_SHAPE,
+                     "attention_packed: row strides must be multiples of 8 that hold a row's heads");
+  if (n_seqs <= 0 || n_seqs > 65535 || rows <= 0 || rows > kMaxContext)
+    return set_error(ctx, SAM3_ERR_SHAPE, "attention_packed: bad shape");
+  PackedArgs a{};
+  a.o = o;
+  a.v = v;
+  a.cu = cu;
+  a.err = ctx->dev_err;
+  a.o_stride = o_stride;
+  a.v_stride = v_stride;
+  a.n_seqs = n_seqs;
+  a.rows = rows;
+  a.group = heads / kv_heads;
+  a.causal = causal != 0;
+  a.c = scale * 1.4426950408889634f;
+  a.o32 = (reinterpret_cast<uintptr_t>(o) & 31u) == 0 && o_stride % 16 == 0;
+  // lengths stay on the device: the work counted here is the rows read and written
+  ProfScope prof(ctx, SAM3_PROF_ATTENTION, 0.0, 4.0 * rows * (wide + narrow));
+  const bool bf = dtype == SAM3_BF16;
+  if (head_dim == 128)
+    return bf ? launch_packed<128, true>(ctx, q, q_stride, k, k_stride, a, heads, kv_heads)
+              : launch_packed<128, false>(ctx, q, q_stride, k, k_stride, a, heads, kv_heads);
+  return bf ? launch_packed<64, true>(ctx, q, q_stride, k, k_stride, a, heads, kv_heads)
+            : launch_packed<64, false>(ctx, q, q_stride, k, k_stride, a, heads, kv_heads);
+}
+
+}  // namespace sam3
+
+using namespace sam3;
+
+extern "C" sam3_status_t sam3_attention_packed(
+    sam3_ctx_t* ctx, int32_t dtype, const uint16_t* q, int64_t q_stride, const uint16_t* k,
+    int64_t k_stride, const uint16_t* v, int64_t v_stride, const int32_t* cu, int32_t n_seqs,
+    int32_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim, float scale, int32_t causal,
+    uint16_t* o, int64_t o_stride) {
+  SAM3_CHECK_CTX(ctx);
+  cudaSetDevice(ctx->device);
+  return attention_packed(ctx, dtype, q, q_stride, k, k_stride, v, v_stride, cu, n_seqs, rows,
+                          heads, kv_heads, head_dim, scale, causal, o, o_stride);
+}

@@ -26,7 +26,12 @@ enum DevErr : int {
   kDevErrTimeoutEpilogue = 0x104,
   kDevErrTimeoutDrain = 0x105,
   kDevErrTimeoutAttn = 0x106,
+  kDevErrTimeoutCached = 0x107,
+  kDevErrTimeoutPacked = 0x108,
   kDevErrTimeoutSelftest = 0x1FF,  // sam3_selftest_wait_timeout
+  // 0x2xx: an index in a kernel's input is out of range; what it names is skipped
+  kDevErrBadLengths = 0x202,  // offsets or lengths of a packed or cached sequence
+  kDevErrBadPage = 0x203,     // a page number of a page table
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

@@ -49,6 +49,10 @@ struct sam3_ctx {
   int32_t* idx = nullptr;       // [B*keep]
   uint16_t* image = nullptr;    // [B, H, W, 3] staging for the host API
   uint16_t* feats = nullptr;    // [B*keep, D] staging for the host API
+  // Pieces of sequences that attention_cached splits over CTAs, and which CTA
+  // left which (attention_cached.cu).
+  float* cached_part = nullptr;   // [num_sms, 2, kCachedPartFloats]
+  int32_t* cached_meta = nullptr; // [num_sms, 4]
   int rope_ready = 0;
   // Block-level scratch used by sam3_vit_block & co. outside the encoder.
   size_t block_rows = 0;        // rows the block scratch can hold (plain encoder)
@@ -101,8 +105,13 @@ sam3_status_t device_error_status(sam3_ctx_t* ctx, int err);
 // the attribute belongs to the device, and each context is bound to one.
 enum : uint32_t {
   kSmemAttn = 1u, kSmemWs = 2u, kSmemWsc = 4u, kSmemGemm = 8u /* << MODE */, kSmemPrune = 64u,
-  kSmemAttnPP = 128u
+  kSmemAttnPP = 128u, kSmemCached = 256u /* << variant, 4 of them */,
+  kSmemPacked = 4096u /* << variant, 4 of them */
 };
+// One piece: 64 rows of up to 128 unnormalised outputs, then their 64 running
+// maxima and 64 row sums.
+constexpr int kCachedPartRows = 64;
+constexpr int kCachedPartFloats = kCachedPartRows * 128 + 2 * kCachedPartRows;
 template <typename Kernel>
 sam3_status_t ensure_smem_attr(sam3_ctx_t* ctx, uint32_t bit, Kernel kernel, int bytes,
                                const char* what) {
@@ -154,6 +163,32 @@ sam3_status_t prune(sam3_ctx_t* ctx, const uint16_t* x, int batch, int seq, int 
 sam3_status_t patch_embed(sam3_ctx_t* ctx, const void* image, bool rgba, int batch, int h, int w,
                           const uint16_t* pw, const uint16_t* pb, int patch, int dim,
                           uint16_t* out, uint16_t* cols_scratch, uint16_t* wpad_scratch);
+
+// Most tokens that a row of a page table may name (positions are 32-bit).
+constexpr long long kMaxContext = 1ll << 30;
+// The checks that the kernels make of what they read on the device: lengths,
+// offsets and page numbers index memory only behind these.
+#ifdef __CUDACC__
+#define SAM3_HD __host__ __device__ __forceinline__
+#else
+#define SAM3_HD inline
+#endif
+// Rows [r0, r1) of a packed buffer of `rows` rows.
+SAM3_HD bool rows_fit(int r0, int r1, int rows) { return r0 >= 0 && r1 >= r0 && r1 <= rows; }
+// The same, as the newest of a sequence of `len` tokens whose page-table row
+// has `table_stride` pages of 2^page_shift tokens.
+SAM3_HD bool tokens_fit(int r0, int r1, int rows, int max_new, int len, int table_stride,
+                        int page_shift) {
+  return rows_fit(r0, r1, rows) && r1 - r0 <= max_new && len >= r1 - r0 &&
+         (long long)len <= (long long)table_stride << page_shift;
+}
+SAM3_HD bool page_fits(int page, int num_pages) { return page >= 0 && page < num_pages; }
+// The checks of a cache description that its writers and readers share.
+sam3_status_t check_kv_cache(sam3_ctx_t* ctx, const sam3_kv_cache_t* c, const char* what);
+// Row strides in elements: whole 16-byte groups, and wide enough for `width`.
+inline bool stride_ok(int64_t stride, int64_t width) {
+  return stride % 8 == 0 && stride >= width && stride <= (1ll << 31);
+}
 
 // Launch with programmatic stream serialization: the kernel may start while
 // the previous kernel in the stream finishes (its prologue overlapping that

@@ -24,13 +24,14 @@ OK, ERR_INVALID_ARG, ERR_SHAPE, ERR_OOM, ERR_CUDA, ERR_TIMEOUT, ERR_UNSUPPORTED 
 EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_RESIDUAL, EPI_BIAS_ROPE_QKV = range(4)
 FAULT_NONE, FAULT_ALLOC, FAULT_LAUNCH = 0, 1, 2
 SCORE_L2, SCORE_L1 = 0, 1
+F16, BF16 = 0, 1
 ORDER_INDEX, ORDER_SCORE = 0, 1
 
 STATUS_NAMES = {0: "SAM3_OK", 1: "SAM3_ERR_INVALID_ARG", 2: "SAM3_ERR_SHAPE", 3: "SAM3_ERR_OOM",
                 4: "SAM3_ERR_CUDA", 5: "SAM3_ERR_TIMEOUT", 6: "SAM3_ERR_UNSUPPORTED"}
 
 # Every symbol the header declares: (name, restype, argtypes).
-_P, _I, _F, _SZ = C.c_void_p, C.c_int32, C.c_float, C.c_size_t
+_P, _I, _F, _SZ, _L = C.c_void_p, C.c_int32, C.c_float, C.c_size_t, C.c_int64
 
 
 class EncoderConfig(C.Structure):
@@ -61,6 +62,12 @@ class EncoderWeights(C.Structure):
 class NeckWeights(C.Structure):
     _fields_ = [("conv1_w", C.c_void_p), ("conv1_b", C.c_void_p), ("conv2_w", C.c_void_p),
                 ("conv2_b", C.c_void_p), ("in_dim", C.c_int32), ("out_dim", C.c_int32)]
+
+
+class KVCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p),
+                ("v_scale", C.c_void_p), ("num_pages", C.c_int32), ("page_size", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32)]
 
 
 class WindowedEncoderWeights(C.Structure):
@@ -104,6 +111,12 @@ SIGNATURES = {
     "sam3_rope_table": (_S, [_P, _I, _I, _I, _F, _P]),
     "sam3_rope_apply": (_S, [_P, _P, _I, _I, _I, _P, _I]),
     "sam3_attention": (_S, [_P, _P, _I, _I, _I, _I, _F, _P]),
+    "sam3_attention_packed": (_S, [_P, _I, _P, _L, _P, _L, _P, _L, _P, _I, _I, _I, _I, _I, _F, _I,
+                                   _P, _L]),
+    "sam3_kv_append": (_S, [_P, C.POINTER(KVCache), _I, _P, _L, _P, _L, _P, _I, _I, _I, _P, _I,
+                            _P]),
+    "sam3_attention_cached": (_S, [_P, C.POINTER(KVCache), _I, _P, _L, _P, _I, _I, _I, _P, _I, _P,
+                                   _I, _F, _I, _P, _L]),
     "sam3_token_scores": (_S, [_P, _P, _I, _I, _I, _P]),
     "sam3_prune": (_S, [_P, _P, _I, _I, _I, _I, _I, _I, _P, _I, _I, _P, _P, _P]),
     "sam3_patch_embed": (_S, [_P, _P, _I, _I, _I, _P, _P, _I, _I, _P]),
@@ -133,6 +146,7 @@ SIGNATURES = {
 }
 
 PRUNE_NOALLOC_MAX_ROWS = 65536
+CACHED_MAX_SEQS = 1024
 
 
 def _load():
@@ -311,6 +325,26 @@ class Context:
         self._check(lib.sam3_attention(self.handle, ptr(qkv), batch, seq, heads, head_dim, scale,
                                        ptr(o)))
 
+    def attention_packed(self, dtype, q, q_stride, k, k_stride, v, v_stride, cu, n_seqs, rows,
+                         heads, kv_heads, head_dim, scale, causal, o, o_stride):
+        self._check(lib.sam3_attention_packed(self.handle, dtype, ptr(q), q_stride, ptr(k),
+                                              k_stride, ptr(v), v_stride, ptr(cu), n_seqs, rows,
+                                              heads, kv_heads, head_dim, scale, causal, ptr(o),
+                                              o_stride))
+
+    def kv_append(self, cache: KVCache, dtype, k, k_stride, v, v_stride, cu_new, n_seqs, rows,
+                  max_new, page_table, table_stride, seq_lens):
+        self._check(lib.sam3_kv_append(self.handle, C.byref(cache), dtype, ptr(k), k_stride,
+                                       ptr(v), v_stride, ptr(cu_new), n_seqs, rows, max_new,
+                                       ptr(page_table), table_stride, ptr(seq_lens)))
+
+    def attention_cached(self, cache: KVCache, dtype, q, q_stride, cu_new, n_seqs, rows, max_new,
+                         page_table, table_stride, seq_lens, heads, scale, causal, o, o_stride):
+        self._check(lib.sam3_attention_cached(self.handle, C.byref(cache), dtype, ptr(q), q_stride,
+                                              ptr(cu_new), n_seqs, rows, max_new, ptr(page_table),
+                                              table_stride, ptr(seq_lens), heads, scale, causal,
+                                              ptr(o), o_stride))
+
     def token_scores(self, x, rows, d, norm, scores):
         self._check(lib.sam3_token_scores(self.handle, ptr(x), rows, d, norm, ptr(scores)))
 
@@ -450,6 +484,13 @@ def block_weights(ln1_gamma, ln1_beta, qkv, proj, ln2_gamma, ln2_beta, fc1, fc2)
 
 def neck_weights(conv1_w, conv1_b, conv2_w, conv2_b, in_dim, out_dim) -> NeckWeights:
     return NeckWeights(ptr(conv1_w), ptr(conv1_b), ptr(conv2_w), ptr(conv2_b), in_dim, out_dim)
+
+
+def kv_cache(k, v, k_scale, v_scale, num_pages, page_size, kv_heads, head_dim) -> KVCache:
+    """k, v: e4m3 codes [num_pages, kv_heads, page_size, head_dim]; scales f32
+    [num_pages, kv_heads]."""
+    return KVCache(ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), num_pages, page_size, kv_heads,
+                   head_dim)
 
 
 def encoder_weights(patch_w, patch_b, blocks) -> EncoderWeights:
