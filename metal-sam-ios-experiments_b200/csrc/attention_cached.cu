@@ -1,35 +1,48 @@
 // attention_cached.cu - attention of each sequence's newest tokens over a paged
-// cache held in 8 bits (kv_cache.cu).
+// cache held in 8 bits (kv_cache.cu), on the sm_100a fp8 tensor cores.
 //
 // o[t, h] = sum_j p_j v_j / sum_j p_j, p_j = 2^(x_j), x_j = scale log2(e) *
 // q[t, h] . k_j, over the tokens j of t's sequence that t sees; k_j and v_j are
-// e4m3 codes times their page's scale. The K/V heads are shared by groups of
-// heads / kv_heads query heads.
+// e4m3 codes times their page's scale. Groups of heads / kv_heads query heads
+// share a K/V head; a K/V head's `rows` are its query heads times the new
+// tokens.
 //
-// HBM bound: every code is read once (2 * len * kv_heads * head_dim bytes) and
-// serves the `group * new` query rows of its K/V head, a handful, so the matrix
-// work is small: warp-level fp16 matrix instructions on 16-row tiles, not
-// tcgen05, whose smallest tile has 64 rows. Every e4m3 code is exact in fp16.
+// HBM bound: 2 * len * kv_heads * head_dim bytes of codes are read once. So the
+// codes go from global to shared memory by TMA and from there into tcgen05.mma
+// (kind::f8f6f4) as they are: no thread touches them.
+//   S^T[line, column] = K[line, 128 bytes] . Q[column, 128 bytes]
+//   O^T[byte, column] += V[line, byte] . P[column, line]
+// A line is 128 bytes of codes: one token of head_dim 128 or two of 64. The
+// large operand is the M = 128 side, the few rows are columns of the N side, and
+// each row takes three columns, the terms of an exact split of an 11-bit
+// number into e4m3 numbers: y = t0 + t1/16 + t2/256, each term the rounding
+// (4 bits, to nearest) of what is left. fp16 and bf16 queries (scaled by a
+// power of two to at most 448) are represented exactly down to 2^-6, smaller
+// elements to within 2^-18; the weights p are rounded to fp16 (half a step of
+// 2^-11) and split the same way. Products are exact and sums fp32. For
+// head_dim 64 a column serves one of the line's two tokens: Q's other half is
+// zero, and of O^T only the half of the column's token is used (the tensor
+// cores have room: an MMA is bound by its 128-row operand up to 64 columns).
+// 0 * NaN is NaN, so a line's other token must not be a NaN code that the row
+// does not see: warp 3 looks through the K lines where that can be, the odd
+// token behind a sequence's end and the newest tokens, before the MMA.
 //
-// Split: the context is cut into units of a few 64-token tiles (one for each
-// warp group of a CTA, below), the units of all (sequence, K/V head, row block)
-// are counted through, and each of the num_sms CTAs takes an equal run of them,
-// whatever the sequences' lengths. Where a run begins or ends inside an item,
-// the CTA leaves its unnormalised sum, maximum and row sum in the workspace, and
-// cached_join_kernel adds the pieces in the order of the CTAs (no atomics: the
-// result does not depend on timing).
+// A CTA, two per SM: warp 0 streams tiles of 128 lines (16 KB of K, 16 KB of V)
+// page by page through the table; warp 1 issues the MMAs; warp 2 loads and
+// splits the next item's queries; warps 4-7, one thread per line, turn scores
+// into weights: a handful of exponentials per thread and tile. The running
+// maximum moves only when a score exceeds it by 0.8, found by one barrier with
+// a vote; only then are maxima exchanged and O^T rescaled in tensor memory.
 //
-// A CTA: warp 8 streams tiles (64 tokens of K and V) through a shared-memory
-// ring by TMA, page by page through the table, 128-byte swizzled lines; warps
-// 0-7 are `rt` row tiles times 8 / rt groups, group g takes every (8 / rt)-th
-// tile of an item and keeps its own running maximum, sums and output in
-// registers. At the end of an item the groups meet in shared memory.
+// Split: the context is cut into units of tiles, the units of all (sequence,
+// K/V head, row block) are counted through, and each of the 2 * num_sms CTAs
+// takes an equal run of them, whatever the sequences' lengths. Where a run
+// begins or ends inside an item, the CTA leaves its unnormalised sum, maximum
+// and row sum in the workspace, and cached_join_kernel adds the pieces in the
+// order of the CTAs (no atomics: the result does not depend on timing).
 //
-// V's scale joins the exponent: P = 2^(x + log2(vs) - M) with M the running
-// maximum of x + log2(vs), so that P * code needs no second scale; the row sum
-// adds P / vs in fp32. P is rounded to fp16 at 2^12 times its value (its
-// largest entry is 2^12), which keeps weights down to 2^-26 of the largest in
-// fp16's normal range: half a step of 2^-11 of each weight.
+// V's scale joins the exponent: P = 2^(x + log2(vs) - M + 8) with M the running
+// maximum of x + log2(vs), at most 2^8.8 < 448; the row sum adds P / vs in fp32.
 #include <algorithm>
 
 #include "common.cuh"
@@ -40,27 +53,43 @@
 namespace sam3 {
 namespace {
 
-constexpr int KT = 64;                 // tokens per tile
-constexpr int CWARPS = 8;              // computing warps
-constexpr int THREADS = 32 * (CWARPS + 1);
+constexpr int THREADS = 256;
 constexpr int MAX_SEQS = SAM3_CACHED_MAX_SEQS;
-constexpr int RING_BYTES = 128 * 1024;
-constexpr float P_SHIFT = 12.f;
+constexpr int LINES = 128;             // lines per tile
+constexpr int TILE = LINES * 128;      // bytes of K or V per tile
+constexpr int UNIT_TILES = 4;          // tiles per unit of small jobs
+constexpr float P_EXP = 8.f;           // the largest weight at its maximum is 2^8
+constexpr float P_TOP = 8.8f;          // and may grow to 2^8.8 < 448 before M moves
+constexpr float T1 = 1.f / 16, T2 = 1.f / 256;  // weights of the second and third term
+enum : int { kFirst = 1, kLast = 2, kFinal = 4, kCheck = 8 };
+constexpr int kNever = 0x7FFFFFFF;
 
-template <int D>
+template <int D, int RB>
 struct Cfg {
-  static constexpr int TILE = KT * D;               // bytes of K or V in a tile
-  static constexpr int ST = RING_BYTES / (2 * TILE);
-  static constexpr int OFF_COMB = RING_BYTES;       // [CWARPS][16][D] f32
-  static constexpr int OFF_ML = OFF_COMB + CWARPS * 16 * D * 4;    // [CWARPS][16] (max, sum)
-  static constexpr int OFF_SCALE = OFF_ML + CWARPS * 16 * 8;       // [ST][4] float4
-  static constexpr int OFF_SEQ = OFF_SCALE + ST * 4 * 16;          // prefix, len, row, new
-  static constexpr int OFF_BAR = OFF_SEQ + (4 * MAX_SEQS + 4) * 4;
-  static constexpr int OFF_MISC = OFF_BAR + 2 * ST * 8;
-  static constexpr int SMEM = OFF_MISC + 16 + 1024;
+  static constexpr int TPL = 128 / D;             // tokens per line
+  static constexpr int TT = LINES * TPL;          // tokens per tile
+  static constexpr int NC = 3 * RB * TPL;         // columns used
+  static constexpr int N = (NC + 15) / 16 * 16;   // columns of the MMAs
+  static constexpr int ST = N <= 32 ? 3 : 2;      // ring stages (K and V tile each)
+  static constexpr uint32_t COLS = N <= 16 ? 32 : N <= 32 ? 64 : N <= 64 ? 128 : 256;
+  static constexpr int GRAN = TT / 16;            // scale entries per tile (16 tokens)
+  static constexpr int OFF_Q = ST * 2 * TILE;               // [2][N][128]
+  static constexpr int OFF_P = OFF_Q + 2 * N * 128;         // [N][128]
+  static constexpr int OFF_SCALE = OFF_P + N * 128;         // [ST][GRAN] float4
+  static constexpr int OFF_INFO = OFF_SCALE + ST * GRAN * 16;     // [ST] int4
+  static constexpr int OFF_ITEM = OFF_INFO + ST * 16;       // [2] ItemInfo
+  static constexpr int ITEM = 32 + RB * 8;
+  static constexpr int OFF_MAX = OFF_ITEM + 2 * ITEM;       // [RB] float4
+  static constexpr int OFF_POISON = OFF_MAX + RB * 16;      // [128] u32
+  static constexpr int OFF_BAR = OFF_POISON + 512;
+  static constexpr int BARS = 3 * ST + 4 + 7;
+  static constexpr int OFF_MISC = OFF_BAR + BARS * 8;
+  static constexpr int SMEM = OFF_MISC + 128 + 1024;
 };
-static_assert(Cfg<128>::SMEM <= 227 * 1024 && Cfg<64>::SMEM <= 227 * 1024, "shared memory");
-static_assert(Cfg<128>::ST >= CWARPS, "a unit's tiles fit the ring");
+static_assert(2 * (Cfg<128, 8>::SMEM + 1024) <= 228 * 1024, "two CTAs per SM");
+static_assert(2 * (Cfg<128, 32>::SMEM + 1024) <= 228 * 1024, "two CTAs per SM");
+static_assert(2 * (Cfg<64, 4>::SMEM + 1024) <= 228 * 1024, "two CTAs per SM");
+static_assert(2 * (Cfg<64, 16>::SMEM + 1024) <= 228 * 1024, "two CTAs per SM");
 
 struct CachedArgs {
   const uint16_t* q;
@@ -75,258 +104,295 @@ struct CachedArgs {
   int32_t* meta;
   int* err;
   int table_stride, num_pages, page_shift, kv_heads, group, n_seqs, rows, max_new;
-  int rt;  // row tiles of 16 in a row block: 1, 2 or 4
   int causal;
+  int whole;  // no sequence has more than one unit of UNIT_TILES tiles
   float scale_log2;
 };
 
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                         uint32_t b1) {
-  asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// What the query warp tells the others of an item (smem).
+struct ItemInfo {
+  int row0, head, block, n_rows, starts, ends, pad0, pad1;
+};
+
+__device__ __forceinline__ bool vote_any(bool p) {  // over warps 4-7
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 2, 128, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)p)
+      : "memory");
+  return r != 0;
 }
-// Four codes to two fp16 pairs.
-__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
-      "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-      : "=r"(lo), "=r"(hi)
-      : "r"(w));
+__device__ __forceinline__ void compute_barrier() {
+  asm volatile("barrier.cta.sync 2, 128;" ::: "memory");
 }
-__device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(0xffffffffu, v, 1);
-  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+__device__ __forceinline__ float warp_add(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
-// Whether any of the four codes is NaN (0x7F or 0xFF).
+
+// The three terms of a pair of fp16 numbers of at most 448, as code pairs:
+// every subtraction and product below is exact.
+__device__ __forceinline__ void split3(__half2 h, uint16_t (&t)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(&h);
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(t[i]) : "r"(w));
+    if (i == 2) break;
+    uint32_t b;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(b) : "h"(t[i]));
+    h = __hmul2(__hsub2(h, *reinterpret_cast<const __half2*>(&b)), __float2half2_rn(16.f));
+  }
+}
+
+// Bytes of w whose code is NaN (0x7F or 0xFF), as 0xFF.
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) {
   return __vcmpeq4(w & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
 }
-__device__ __forceinline__ void compute_barrier() {
-  asm volatile("bar.sync 1, %0;" ::"n"(32 * CWARPS) : "memory");
-}
 
-// Byte offset of 16-byte group `c` of a token's row in a tile. Lines of 128
-// bytes (one token of head_dim 128, two of 64) with TMA's 128-byte swizzle:
-// group index XOR line mod 8. The fragment loads below then hit every bank
-// once (V at head_dim 64: twice).
-template <int D>
-__device__ __forceinline__ uint32_t tile_off(int row, int c) {
-  const int line = D == 128 ? row : row >> 1;
-  const int grp = D == 128 ? c : (row & 1) * 4 + c;
-  return line * 128 + ((grp ^ (line & 7)) << 4);
-}
-
-// Row blocks of 16 * rt query rows per K/V head of a sequence.
-__device__ __forceinline__ int row_blocks(const CachedArgs& a, int fresh) {
-  return (fresh * a.group + 16 * a.rt - 1) / (16 * a.rt);
-}
-// The sequences' units times row blocks (prefix sums), lengths, first rows and
-// new tokens in shared memory. A sequence that does not fit its buffers counts
-// none.
-struct SeqTable {
-  int *prefix, *len, *row, *fresh;
+// A sequence as the kernels see it; one that does not fit its buffers counts
+// as having no new tokens.
+struct Seq {
+  int len, row0, fresh;
 };
-__device__ __forceinline__ SeqTable seq_table(uint8_t* base) {
-  int* p = reinterpret_cast<int*>(base);
-  return {p, p + MAX_SEQS + 1, p + 2 * MAX_SEQS + 1, p + 3 * MAX_SEQS + 1};
-}
-__device__ void load_seqs(const CachedArgs& a, const SeqTable& s, int kg, bool report) {
-  for (int i = threadIdx.x; i < a.n_seqs; i += blockDim.x) {
-    const int len = a.lens[i];
-    const int r0 = a.cu ? a.cu[i] : i;
-    const int r1 = a.cu ? a.cu[i + 1] : i + 1;
-    const bool ok = tokens_fit(r0, r1, a.rows, a.max_new, len, a.table_stride, a.page_shift);
-    if (!ok && report) atomicExch(a.err, kDevErrBadLengths);
-    const int fresh = ok ? r1 - r0 : 0;
-    s.prefix[i + 1] = fresh ? (len + KT * kg - 1) / (KT * kg) * row_blocks(a, fresh) : 0;
-    s.len[i] = len;
-    s.row[i] = r0;
-    s.fresh[i] = fresh;
-  }
-  if (threadIdx.x == 0) s.prefix[0] = 0;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    int sum = 0;
-    for (int i0 = 0; i0 < a.n_seqs; i0 += 32) {
-      const int i = i0 + threadIdx.x;
-      int v = i < a.n_seqs ? s.prefix[i + 1] : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, v, o);
-        if ((int)threadIdx.x >= o) v += u;
-      }
-      if (i < a.n_seqs) s.prefix[i + 1] = sum + v;
-      sum += __shfl_sync(0xffffffffu, v, 31);
-    }
-  }
-  __syncthreads();
+__device__ __forceinline__ Seq load_seq(const CachedArgs& a, int i, bool report) {
+  Seq s;
+  s.len = a.lens[i];
+  s.row0 = a.cu ? a.cu[i] : i;
+  const int r1 = a.cu ? a.cu[i + 1] : i + 1;
+  const bool ok = tokens_fit(s.row0, r1, a.rows, a.max_new, s.len, a.table_stride, a.page_shift);
+  if (!ok && report) atomicExch(a.err, kDevErrBadLengths);
+  s.fresh = ok ? r1 - s.row0 : 0;
+  return s;
 }
 
-// A run of units over the items (sequence, K/V head and row block).
+// A run of units over the items (sequence; K/V head and row block).
+template <int D, int RB>
 struct Run {
-  int seq, sub, unit;
-  int left;           // units to go
-  int units, blocks;  // of the sequence
+  int seq, sub, unit, left;  // where it is, and the units to go
+  int unit_tiles;
+  Seq s;
+  int units, blocks, tiles;  // of the sequence
+
+  __device__ __forceinline__ void enter(const CachedArgs& a) {
+    s = load_seq(a, seq, false);
+    blocks = (s.fresh * a.group + RB - 1) / RB;
+    tiles = s.fresh ? (s.len + Cfg<D, RB>::TT - 1) / Cfg<D, RB>::TT : 0;
+    units = (tiles + unit_tiles - 1) / unit_tiles;
+  }
+  // `at`: units of the sequence before the run's first
+  __device__ __forceinline__ void start(const CachedArgs& a, int seq_, int at, int left_, int ut) {
+    seq = seq_;
+    left = left_;
+    unit_tiles = ut;
+    enter(a);
+    sub = at / max(1, units);
+    unit = at - sub * units;
+  }
+  // tiles [tile0(), tile1()) of the item are next
+  __device__ __forceinline__ int n_units() const { return min(left, units - unit); }
+  __device__ __forceinline__ int tile0() const { return unit * unit_tiles; }
+  __device__ __forceinline__ int tile1() const { return min((unit + n_units()) * unit_tiles, tiles); }
+  __device__ __forceinline__ int head() const { return sub / blocks; }
+  __device__ __forceinline__ void next(const CachedArgs& a) {
+    left -= n_units();
+    unit = 0;
+    if (left <= 0 || ++sub < a.kv_heads * blocks) return;
+    sub = 0;
+    do {
+      if (++seq >= a.n_seqs) {
+        left = 0;
+        return;
+      }
+      enter(a);
+    } while (units == 0);
+  }
 };
-__device__ __forceinline__ void run_enter(const CachedArgs& a, const SeqTable& s, Run& r) {
-  r.blocks = row_blocks(a, s.fresh[r.seq]);
-  r.units = max(1, (s.prefix[r.seq + 1] - s.prefix[r.seq]) / max(1, r.blocks));
-}
-__device__ __forceinline__ Run run_start(const CachedArgs& a, const SeqTable& s, int x0, int x1) {
-  Run r;
-  r.left = x1 - x0;
-  int lo = 0, hi = a.n_seqs - 1;  // the first sequence that ends behind x0
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (s.prefix[mid + 1] * a.kv_heads > x0)
-      hi = mid;
-    else
-      lo = mid + 1;
-  }
-  r.seq = lo;
-  const int at = x0 - s.prefix[lo] * a.kv_heads;
-  run_enter(a, s, r);
-  r.sub = at / r.units;
-  r.unit = at - r.sub * r.units;
-  return r;
-}
-__device__ __forceinline__ void run_next(const CachedArgs& a, const SeqTable& s, Run& r, int taken) {
-  r.left -= taken;
-  r.unit = 0;
-  if (++r.sub < a.kv_heads * r.blocks) return;
-  r.sub = 0;
-  do {
-    ++r.seq;
-  } while (r.seq < a.n_seqs - 1 && s.prefix[r.seq + 1] == s.prefix[r.seq]);
-  if (r.seq < a.n_seqs) run_enter(a, s, r);
-}
 
 template <bool BF>
-__device__ __forceinline__ uint32_t pack_out(float lo, float hi) {
-  if (BF) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  return pack_half2(lo, hi);
-}
-// Four outputs of one (row, head): 8 bytes.
-template <bool BF>
-__device__ __forceinline__ void store_out4(uint16_t* p, float4 v) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(pack_out<BF>(v.x, v.y), pack_out<BF>(v.z, v.w));
+__device__ __forceinline__ uint16_t to_out(float v) {
+  if (BF) return __bfloat16_as_ushort(__float2bfloat16_rn(v));
+  return __half_as_ushort(__float2half_rn(v));
 }
 
-// Query fragments of one row in the K permutation (thread t of a quad holds
-// elements t*D/4 ... of the row), in fp16. A bf16 row is first multiplied by a
-// power of two that brings its largest element to [2^14, 2^15): exact for all
-// elements down to 2^-28 of the largest, and below that off by at most 2^-40
-// of it. Returns the power that undoes it.
-template <int D, bool BF>
-__device__ __forceinline__ float load_q_row(const uint16_t* row, int t, uint32_t (&f)[D / 8]) {
-  const uint4* src = reinterpret_cast<const uint4*>(row + t * (D / 4));
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    const uint4 u = row ? src[i] : make_uint4(0, 0, 0, 0);
-    f[4 * i] = u.x;
-    f[4 * i + 1] = u.y;
-    f[4 * i + 2] = u.z;
-    f[4 * i + 3] = u.w;
-  }
-  if (!BF) return 1.f;
-  float top = 0.f;
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i)
-    top = fmaxf(top, fmaxf(fabsf(__uint_as_float(f[i] << 16)),
-                           fabsf(__uint_as_float(f[i] & 0xFFFF0000u))));
-  top = quad_max(top);
-  // exponent of the largest, kept where both powers below are normal numbers
-  const int e = min(max(((__float_as_int(top) >> 23) & 255) - 127 - 14, -126), 113);
-  const float down = __int_as_float((127 - e) << 23);
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i)
-    f[i] = pack_half2(__uint_as_float(f[i] << 16) * down,
-                      __uint_as_float(f[i] & 0xFFFF0000u) * down);
-  return __int_as_float((127 + e) << 23);
-}
-
-template <int D, bool BF>
-__global__ void __launch_bounds__(THREADS, 1)
+template <int D, int RB, bool BF>
+__global__ void __launch_bounds__(THREADS, 2)
     cached_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const CachedArgs a) {
-  using C = Cfg<D>;
+  using C = Cfg<D, RB>;
+  constexpr int TPL = C::TPL, N = C::N, ST = C::ST;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t sbase = smem_u32(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rt = a.rt, kg = CWARPS / rt;
-  const uint32_t bar_full = sbase + C::OFF_BAR, bar_empty = bar_full + 8 * C::ST;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC);
-  const SeqTable seqs = seq_table(smem + C::OFF_SEQ);
+
+  const uint32_t bar_k = sbase + C::OFF_BAR;    // [ST] K tile, scales and info are there
+  const uint32_t bar_v = bar_k + 8 * ST;        // [ST] V tile is there
+  const uint32_t bar_empty = bar_v + 8 * ST;    // [ST] the tile's P V is done
+  const uint32_t bar_q = bar_empty + 8 * ST;    // [2] an item's queries are split
+  const uint32_t bar_q_empty = bar_q + 16;      // [2] the item is finished
+  const uint32_t bar_s = bar_q_empty + 16;      // scores are in tensor memory
+  const uint32_t bar_s_free = bar_s + 8;        // and have been read
+  const uint32_t bar_p = bar_s_free + 8;        // weights are in shared memory
+  const uint32_t bar_o = bar_p + 8;             // P V done: weights read, O^T current
+  const uint32_t bar_drain = bar_o + 8;
+  const uint32_t bar_raw = bar_drain + 8;       // a K tile for warp 3 is there (head_dim 64)
+  const uint32_t bar_raw_free = bar_raw + 8;    // and looked through
+  uint8_t* misc = smem + C::OFF_MISC;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 4);
+  volatile int* softmax_failed = reinterpret_cast<volatile int*>(misc + 8);
+  int* total_slot = reinterpret_cast<int*>(misc + 12);
+  volatile int* start_slot = reinterpret_cast<volatile int*>(misc + 16);  // seq, at
+  int* warp_sums = reinterpret_cast<int*>(misc + 32);                     // [8]
+  volatile int* raw_stage = reinterpret_cast<volatile int*>(misc + 64);
+  volatile int* k_nan = reinterpret_cast<volatile int*>(misc + 68);       // [ST]
   float4* scales = reinterpret_cast<float4*>(smem + C::OFF_SCALE);
+  int4* infos = reinterpret_cast<int4*>(smem + C::OFF_INFO);
+  uint32_t* poison = reinterpret_cast<uint32_t*>(smem + C::OFF_POISON);
+  auto item_info = [&](int b) { return reinterpret_cast<ItemInfo*>(smem + C::OFF_ITEM + b * C::ITEM); };
+  auto item_rs = [&](int b) { return reinterpret_cast<float*>(smem + C::OFF_ITEM + b * C::ITEM + 32); };
+  auto item_lim = [&](int b) { return reinterpret_cast<int*>(item_rs(b) + RB); };
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::ST; ++s) {
-      mbar_init(bar_full + 8 * s, 1);
-      mbar_init(bar_empty + 8 * s, rt);
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(bar_k + 8 * s, 1);
+      mbar_init(bar_v + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
     }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar_q + 8 * b, 1);
+      mbar_init(bar_q_empty + 8 * b, 128);
+    }
+    mbar_init(bar_s, 1);
+    mbar_init(bar_s_free, 128);
+    mbar_init(bar_p, 128);
+    mbar_init(bar_o, 1);
+    mbar_init(bar_drain, 1);
+    mbar_init(bar_raw, 1);
+    mbar_init(bar_raw_free, 1);
+    for (int s = 0; s < ST; ++s) k_nan[s] = kNever;
     *abort_flag = 0;
+    *softmax_failed = 0;
+    *total_slot = 0;
     fence_mbar_init();
     prefetch_tmap(&map_k);
     prefetch_tmap(&map_v);
   }
-  griddep_launch_dependents();
-  griddep_wait();  // lengths, pages, codes and queries may be earlier kernels' outputs
-  load_seqs(a, seqs, kg, blockIdx.x == 0);
-
-  const int total = seqs.prefix[a.n_seqs] * a.kv_heads;
-  const int chunk = (total + gridDim.x - 1) / gridDim.x;
-  const int x0 = min(total, (int)blockIdx.x * chunk), x1 = min(total, x0 + chunk);
-  if (threadIdx.x == 0) {
-    // bit 0: the run begins inside an item, 1: it ends inside an item that
-    // begins in it, 2: it lies inside one item and does not end it
-    int flags = 0, item_seq = 0, item_sub = 0;
-    if (x1 > x0) {
-      const Run f = run_start(a, seqs, x0, x1), l = run_start(a, seqs, x1 - 1, x1);
-      const bool open = l.unit + 1 < l.units;
-      const bool same = f.seq == l.seq && f.sub == l.sub;
-      if (f.unit > 0) flags |= 1;
-      if (open && (!same || f.unit == 0)) flags |= 2;
-      if (open && same && f.unit > 0) flags |= 4;
-      item_seq = l.seq;
-      item_sub = l.sub;
-    }
-    a.meta[blockIdx.x * 4] = flags;
-    a.meta[blockIdx.x * 4 + 1] = item_seq;
-    a.meta[blockIdx.x * 4 + 2] = item_sub;
+  if (threadIdx.x < 128) poison[threadIdx.x] = 0;
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), C::COLS);
+    tmem_relinquish();
   }
-  if (x1 <= x0) return;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_launch_dependents();  // behind the allocation: the next kernel allocates too
+  griddep_wait();  // lengths, pages, codes and queries may be earlier kernels' outputs
 
-  if (warp == CWARPS) {
+  // ------------------------------------------------- this CTA's run of units
+  int tiles_of[MAX_SEQS / THREADS], items_of[MAX_SEQS / THREADS];
+  long long mine = 0;
+#pragma unroll
+  for (int k = 0; k < MAX_SEQS / THREADS; ++k) {
+    const int i = k * THREADS + threadIdx.x;
+    tiles_of[k] = items_of[k] = 0;
+    if (i < a.n_seqs) {
+      const Seq s = load_seq(a, i, blockIdx.x == 0);
+      if (s.fresh) {
+        tiles_of[k] = (s.len + C::TT - 1) / C::TT;
+        items_of[k] = (s.fresh * a.group + RB - 1) / RB * a.kv_heads;
+      }
+      mine += (long long)tiles_of[k] * items_of[k];
+    }
+  }
+  {
+    int sum = (int)mine;  // the host has seen to it that all fit 31 bits
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0 && sum) atomicAdd(total_slot, sum);
+  }
+  if (threadIdx.x == 0) a.meta[blockIdx.x * 4] = 0;
+  __syncthreads();
+  // Few tiles: runs of whole units, so that short items are not cut (a piece
+  // costs a join, about as much as four tiles). Many: single tiles, for balance.
+  const int ut = a.whole || *total_slot < 8 * (int)gridDim.x ? UNIT_TILES : 1;
+  int units_before = 0, total = *total_slot;
+  if (ut > 1) {
+    __syncthreads();
+    if (threadIdx.x == 0) *total_slot = 0;
+    __syncthreads();
+    int sum = 0;
+#pragma unroll
+    for (int k = 0; k < MAX_SEQS / THREADS; ++k)
+      sum += (tiles_of[k] + ut - 1) / ut * items_of[k];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0 && sum) atomicAdd(total_slot, sum);
+    __syncthreads();
+    total = *total_slot;
+  }
+  // equal runs, without a gap between the CTAs that have one (the join's order)
+  const int busy_ctas = min((int)gridDim.x, total), cta = min((int)blockIdx.x, busy_ctas);
+  const int x0 = busy_ctas ? (int)((long long)cta * total / busy_ctas) : 0;
+  const int x1 = cta < busy_ctas ? (int)((long long)(cta + 1) * total / busy_ctas) : x0;
+#pragma unroll
+  for (int k = 0; k < MAX_SEQS / THREADS; ++k) {
+    if (k * THREADS >= a.n_seqs) break;
+    const int u = (tiles_of[k] + ut - 1) / ut * items_of[k];
+    int incl = u;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) warp_sums[warp] = incl;
+    __syncthreads();
+    int base = units_before, all = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) base += warp_sums[w];
+      all += warp_sums[w];
+    }
+    incl += base;
+    if (x0 < incl && x0 >= incl - u) {  // one thread at most
+      start_slot[0] = k * THREADS + threadIdx.x;
+      start_slot[1] = x0 - (incl - u);
+    }
+    units_before += all;
+    __syncthreads();
+  }
+  const bool busy = x1 > x0;
+
+  if (busy && warp == 0) {
     // ------------------------------------------------------------- producer
     const int page = 1 << a.page_shift;
-    const int per = KT >> min(a.page_shift, 6);  // pages per tile
-    const int box = min(page, KT);               // tokens per copy
-    const uint32_t copy_bytes = box * D;
+    const int per = C::TT >> a.page_shift;  // pages per tile: 1 ... 16
+    const uint32_t copy_bytes = (uint32_t)page * D;
     int stage = 0;
-    uint32_t phase = 0, used = 0;
-    Run r = run_start(a, seqs, x0, x1);
-    while (r.left > 0) {
-      const int n_units = min(r.left, r.units - r.unit);
-      const int len = seqs.len[r.seq];
-      const int head = r.sub / r.blocks;
-      const int tile1 = min((r.unit + n_units) * kg, (len + KT - 1) / KT);
+    uint32_t phase = 0, used = 0, raws = 0;
+    bool ok = true;
+    Run<D, RB> r;
+    r.start(a, start_slot[0], start_slot[1], x1 - x0, ut);
+    while (r.left > 0 && ok) {
+      const int len = r.s.len, head = r.head();
+      const int tile0 = r.tile0(), tile1 = r.tile1();
+      const int lim_min = a.causal ? len - r.s.fresh + 1 : len;
       const int pages = (len + page - 1) >> a.page_shift;
       const int32_t* row = a.table + (size_t)r.seq * a.table_stride;
-      int window = -32;
-      int slot = 0;
+      const bool final_item = r.left == r.n_units();
+      int window = -32, slot = -1;
       float ks = 0.f, lvs = 0.f, ivs = 0.f;
-      for (int tile = r.unit * kg; tile < tile1; ++tile) {
-        const int first = (tile * KT) >> a.page_shift;
+      for (int tile = tile0; tile < tile1 && ok; ++tile) {
+        const int first = tile * per;
         if (first >= window + 32) {
           // the next 32 pages of the sequence, one per lane, with their scales
           window = first & ~31;
@@ -345,364 +411,587 @@ __global__ void __launch_bounds__(THREADS, 1)
           lvs = __log2f(vs);
           ivs = 1.f / vs;
         }
-        mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, a.err, kDevErrTimeoutCached);
-        if (*abort_flag) break;
-        // lane l copies K (even) or V (odd) of page l / 2 of the tile
-        const int mine = first + (lane >> 1);
-        const int my_slot = __shfl_sync(0xffffffffu, slot, mine & 31);
-        const bool copies = lane < 2 * per && mine < pages && my_slot >= 0;
-        const uint32_t n_copies = __popc(__ballot_sync(0xffffffffu, copies));
-        // a missing page's codes are never used: its tokens count as masked
-        const int sp = first + ((lane & 3) * 16 >> min(a.page_shift, 6));
-        const float4 sc = make_float4(__shfl_sync(0xffffffffu, ks, sp & 31),
-                                      __shfl_sync(0xffffffffu, lvs, sp & 31),
-                                      __shfl_sync(0xffffffffu, ivs, sp & 31),
-                                      __shfl_sync(0xffffffffu, slot, sp & 31) >= 0 ? 1.f : 0.f);
-        if (lane < 4) scales[stage * 4 + lane] = sc;
+        ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, a.err, kDevErrTimeoutCached);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        // lane l copies K (l < 16) or V of page l % 16 of the tile
+        const int my_page = first + (lane & 15);
+        const int my_slot = __shfl_sync(0xffffffffu, slot, my_page & 31);
+        const bool copies = (lane & 15) < per && my_page < pages && my_slot >= 0;
+        const uint32_t n_copies = __popc(__ballot_sync(0xffffffffu, copies) & 0xFFFFu);
+        const bool hole = __any_sync(0xffffffffu, (lane & 15) < per && my_page < pages && my_slot < 0);
+        const int sp = (first + (((lane & 15) * 16) >> a.page_shift)) & 31;
+        // .w: the page is there; the tokens of one that is not count as masked
+        const float4 sc = make_float4(__shfl_sync(0xffffffffu, ks, sp),
+                                      __shfl_sync(0xffffffffu, lvs, sp),
+                                      __shfl_sync(0xffffffffu, ivs, sp),
+                                      __shfl_sync(0xffffffffu, slot, sp) >= 0 ? 1.f : 0.f);
+        // a line of this tile may hold a K code that not all rows see of it
+        const int tile_end = (tile + 1) * C::TT;
+        const bool raw = TPL == 2 && ((len & 1 && len < tile_end && len >= tile * C::TT) ||
+                                      (lim_min < len && tile_end > lim_min));
+        if (raw) {
+          ok = __all_sync(0xffffffffu, mbar_wait(bar_raw_free, (raws & 1u) ^ 1, abort_flag, a.err,
+                                                 kDevErrTimeoutCached));
+          if (!ok) break;
+          ++raws;
+        }
+        const uint32_t bar_k_tile = raw ? bar_raw : bar_k + 8 * stage;
+        if (lane < C::GRAN) scales[stage * C::GRAN + lane] = sc;
+        if (lane == 0) {
+          int flags = 0;
+          if (tile == tile0) flags |= kFirst;
+          if (tile == tile1 - 1) flags |= final_item ? kLast | kFinal : kLast;
+          if ((tile + 1) * C::TT > lim_min || hole) flags |= kCheck;
+          infos[stage] = make_int4(tile * C::TT, len, flags, lim_min);
+          if (raw)
+            *raw_stage = stage;
+          else if (TPL == 2)
+            k_nan[stage] = kNever;
+        }
         __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(bar_full + 8 * stage, n_copies * copy_bytes);
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar_k_tile, n_copies * copy_bytes);
+          mbar_arrive_expect_tx(bar_v + 8 * stage, n_copies * copy_bytes);
+        }
         __syncwarp();
         if (copies) {
-          const int which = lane & 1;
-          const uint32_t dst = sbase + (stage * 2 + which) * C::TILE + (lane >> 1) * copy_bytes;
-          const int tok = page > KT ? (tile * KT) & (page - 1) : 0;
+          const int which = lane >> 4;
+          const uint32_t dst =
+              sbase + (stage * 2 + which) * TILE + (uint32_t)(lane & 15) * copy_bytes;
           const long long at = ((long long)my_slot * a.kv_heads + head) << a.page_shift;
-          const int line = (int)((at + tok) / (128 / D));
-          tma_load_2d(dst, which ? &map_v : &map_k, bar_full + 8 * stage, 0, line);
+          tma_load_2d(dst, which ? &map_v : &map_k, which ? bar_v + 8 * stage : bar_k_tile, 0,
+                      (int)(at / TPL));
         }
-        used = min(used + 1, (uint32_t)C::ST);
-        if (++stage == C::ST) {
+        used = min(used + 1, (uint32_t)ST);
+        if (++stage == ST) {
           stage = 0;
           phase ^= 1;
         }
       }
-      if (*abort_flag) break;
-      run_next(a, seqs, r, n_units);
+      if (ok) r.next(a);
+    }
+    if (TPL == 2) {  // warp 3 may go
+      if (ok)
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_raw_free, (raws & 1u) ^ 1, abort_flag, a.err,
+                                               kDevErrTimeoutCached));
+      if (ok && lane == 0) {
+        *raw_stage = -1;
+        mbar_arrive(bar_raw);
+      }
     }
     if (*abort_flag) {
+      if (raws) mbar_wait_drain(bar_raw, (raws - 1) & 1u);
       // nothing may still be in flight into this CTA's shared memory
       for (uint32_t i = 0; i < used; ++i) {
         if (--stage < 0) {
-          stage = C::ST - 1;
+          stage = ST - 1;
           phase ^= 1;
         }
-        mbar_wait_drain(bar_full + 8 * stage, phase);
+        mbar_wait_drain(bar_k + 8 * stage, phase);
+        mbar_wait_drain(bar_v + 8 * stage, phase);
       }
     }
-    return;
-  }
-
-  // --------------------------------------------------------------- computing
-  const int g = lane >> 2, t = lane & 3;
-  const int my_rt = warp % rt, my_kg = warp / rt;
-  float* comb = reinterpret_cast<float*>(smem + C::OFF_COMB);
-  float2* ml = reinterpret_cast<float2*>(smem + C::OFF_ML);
-  int stage = 0;
-  uint32_t phase = 0;
-  Run r = run_start(a, seqs, x0, x1);
-  while (r.left > 0) {
-    const int n_units = min(r.left, r.units - r.unit);
-    const int len = seqs.len[r.seq], row0 = seqs.row[r.seq], fresh = seqs.fresh[r.seq];
-    const int head = r.sub / r.blocks, block = r.sub - head * r.blocks;
-    const int n_rows = min(16 * rt, fresh * a.group - block * 16 * rt);
-    const int tile0 = r.unit * kg;
-    const int tile1 = min((r.unit + n_units) * kg, (len + KT - 1) / KT);
-    // this thread's two rows: query token and head, tokens it sees
-    uint32_t qf[D / 16][4];
-    float rs[2];
-    int lim[2];
+  } else if (busy && warp == 1) {
+    // ------------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t IDESC_S = umma_idesc_e4m3(128, N, 0);
+      constexpr uint32_t IDESC_O = umma_idesc_e4m3(128, N, 1);
+      const uint32_t s_col = tmem, o_col = tmem + C::COLS / 2;
+      auto wait = [&](uint32_t bar, uint32_t par) {
+        return mbar_wait(bar, par, abort_flag, a.err, kDevErrTimeoutCached);
+      };
+      int items = 0;  // begun
+      auto issue_qk = [&](int st, int flags) {
+        if (flags & kFirst) {
+          if (!wait(bar_q + 8 * (items & 1), (uint32_t)(items >> 1) & 1u)) return false;
+          ++items;
+        }
+        const uint64_t dk = umma_desc_sw128(sbase + st * 2 * TILE);
+        const uint64_t dq = umma_desc_sw128(sbase + C::OFF_Q + ((items - 1) & 1) * N * 128);
+        tc_fence_after();
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int lr = my_rt * 16 + g + 8 * h;
-      const int gr = block * 16 * rt + lr;
-      const int tok = gr / a.group, gq = gr - tok * a.group;
-      const uint16_t* src =
-          lr < n_rows ? a.q + (int64_t)(row0 + tok) * a.q_stride + (head * a.group + gq) * D
-                      : nullptr;
-      uint32_t f[D / 8];
-      rs[h] = load_q_row<D, BF>(src, t, f);
-#pragma unroll
-      for (int s = 0; s < D / 16; ++s) {
-        qf[s][h] = f[2 * s];
-        qf[s][2 + h] = f[2 * s + 1];
+        for (int k = 0; k < 4; ++k)
+          umma_f8_ss(s_col, desc_advance(dk, k * 32), desc_advance(dq, k * 32), IDESC_S, k != 0);
+        umma_commit(bar_s);
+        return true;
+      };
+      int st = 0, st_next = 0;
+      uint32_t ph = 0, ph_next = 0;
+      auto step = [&](int& s, uint32_t& p) {
+        if (++s == ST) {
+          s = 0;
+          p ^= 1;
+        }
+      };
+      bool ok = wait(bar_k, 0);
+      int flags = 0;
+      if (ok) {
+        flags = infos[0].z;
+        ok = issue_qk(0, flags);
+        step(st_next, ph_next);
       }
-      lim[h] = a.causal && lr < n_rows ? len - fresh + tok + 1 : len;
+      for (uint32_t i = 0; ok; ++i) {
+        int flags_next = 0;
+        if (!(flags & kFinal)) {  // the next tile's scores, as soon as these are read
+          ok = wait(bar_k + 8 * st_next, ph_next) && wait(bar_s_free, i & 1u);
+          if (!ok) break;
+          flags_next = infos[st_next].z;
+          ok = issue_qk(st_next, flags_next);
+          if (!ok) break;
+          step(st_next, ph_next);
+        }
+        ok = wait(bar_p, i & 1u) && wait(bar_v + 8 * st, ph);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t dv = umma_desc_sw128_mn(sbase + (st * 2 + 1) * TILE);
+        const uint64_t dp = umma_desc_sw128(sbase + C::OFF_P);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          umma_f8_ss(o_col, desc_advance(dv, k * 4096), desc_advance(dp, k * 32), IDESC_O,
+                     !(flags & kFirst) || k != 0);
+        umma_commit(bar_o);
+        umma_commit(bar_empty + 8 * st);
+        step(st, ph);
+        if (flags & kFinal) break;
+        flags = flags_next;
+      }
+      if (*abort_flag) {
+        umma_commit(bar_drain);
+        mbar_wait_drain(bar_drain, 0);
+      }
     }
-    const int lim_min = a.causal ? len - fresh + 1 : len;
-    float o[D / 8][4];
+  } else if (busy && warp == 2) {
+    // ------------------------------------------------------------- queries
+    bool ok = true;
+    Run<D, RB> r;
+    r.start(a, start_slot[0], start_slot[1], x1 - x0, ut);
+    for (uint32_t item = 0; r.left > 0 && ok; ++item) {
+      const int b = item & 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(bar_q_empty + 8 * b, (item >> 1 & 1) ^ 1, abort_flag,
+                                             a.err, kDevErrTimeoutCached));
+      if (!ok) break;
+      const int head = r.head(), block = r.sub - head * r.blocks;
+      const int n_rows = min(RB, r.s.fresh * a.group - block * RB);
+      uint8_t* qb = smem + C::OFF_Q + b * N * 128;
+      constexpr int EPL = D / 32;  // elements per lane
+#pragma unroll 4
+      for (int i = 0; i < RB; ++i) {
+        const int gr = block * RB + i;
+        const int tok = gr / a.group, gq = gr - tok * a.group;
+        uint32_t w[EPL / 2];
+        if (i < n_rows) {
+          const uint32_t* src = reinterpret_cast<const uint32_t*>(
+              a.q + (int64_t)(r.s.row0 + tok) * a.q_stride + (head * a.group + gq) * D + lane * EPL);
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i)
+          for (int e = 0; e < EPL / 2; ++e) w[e] = src[e];
+        } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+          for (int e = 0; e < EPL / 2; ++e) w[e] = 0;
+        }
+        float x[EPL];
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < EPL / 2; ++e) {
+          const float2 f = BF ? make_float2(__uint_as_float(w[e] << 16),
+                                            __uint_as_float(w[e] & 0xFFFF0000u))
+                              : unpack_half2(w[e]);
+          x[2 * e] = f.x;
+          x[2 * e + 1] = f.y;
+          top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+        top = warp_max(top);
+        // the power of two that brings the largest to [128, 256)
+        const int e2 = min(max(((__float_as_int(top) >> 23) & 255) - 127 - 7, -120), 120);
+        const float down = __int_as_float((127 - e2) << 23);
+        uint16_t t[EPL / 2][3];
+#pragma unroll
+        for (int e = 0; e < EPL / 2; ++e)
+          split3(__floats2half2_rn(x[2 * e] * down, x[2 * e + 1] * down), t[e]);
+#pragma unroll
+        for (int p = 0; p < TPL; ++p)
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            const int n = (p * 3 + k) * RB + i;
+            if (D == 128) {
+              const uint32_t at = (uint32_t)(lane * 4) ^ ((n & 7) << 4);
+              *reinterpret_cast<uint32_t*>(qb + n * 128 + at) =
+                  t[0][k] | (uint32_t)t[EPL / 2 - 1][k] << 16;
+            } else {
+              const uint32_t at = (uint32_t)(p * 64 + lane * 2) ^ ((n & 7) << 4);
+              const uint32_t not_at = (uint32_t)((p ^ 1) * 64 + lane * 2) ^ ((n & 7) << 4);
+              *reinterpret_cast<uint16_t*>(qb + n * 128 + at) = t[0][k];
+              *reinterpret_cast<uint16_t*>(qb + n * 128 + not_at) = 0;
+            }
+          }
+        if (lane == 0) {
+          item_rs(b)[i] = __int_as_float((127 + e2) << 23);
+          item_lim(b)[i] = a.causal && i < n_rows ? r.s.len - r.s.fresh + tok + 1 : r.s.len;
+        }
+      }
+      const bool starts = r.unit == 0, ends = r.unit + r.n_units() == r.units;
+      if (lane == 0) {
+        ItemInfo* it = item_info(b);
+        it->row0 = r.s.row0;
+        it->head = head;
+        it->block = block;
+        it->n_rows = n_rows;
+        it->starts = starts;
+        it->ends = ends;
+        if (r.left == r.n_units() && !ends) {
+          // for the join: 2: an item that begins here ends in a later CTA, 4:
+          // the run lies inside one item
+          a.meta[blockIdx.x * 4 + 1] = r.seq;
+          a.meta[blockIdx.x * 4 + 2] = r.sub;
+          a.meta[blockIdx.x * 4] = starts ? 2 : 4;
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_q + 8 * b);
+      r.next(a);
+    }
+  } else if (TPL == 2 && busy && warp == 3) {
+    // ------------------------------------------- K lines shared by two tokens
+    for (uint32_t i = 0;; ++i) {
+      if (!__all_sync(0xffffffffu,
+                      mbar_wait(bar_raw, i & 1u, abort_flag, a.err, kDevErrTimeoutCached)))
+        break;
+      const int st = *raw_stage;
+      if (st < 0) break;
+      const int4 info = infos[st];
+      uint8_t* kt = smem + st * 2 * TILE;
+      auto group = [&](int tok, int c) {  // 16 bytes of a token's row
+        const int line = (tok - info.x) / TPL, p = (tok - info.x) % TPL;
+        return reinterpret_cast<uint4*>(kt + line * 128 + (((p * (D / 16) + c) ^ (line & 7)) << 4));
+      };
+      // the token behind the end, if its line has the last one
+      if ((info.y & 1) && info.y < info.x + C::TT && lane < D / 16)
+        *group(info.y, lane) = make_uint4(0, 0, 0, 0);
+      // the newest tokens: NaN codes become 0, and the first token with one is told
+      const int from = max(info.x, info.w), to = min(info.y, info.x + C::TT);
+      int bad_tok = kNever;
+      for (int j = lane; j < (to - from) * (D / 16); j += 32) {
+        const int tok = from + j / (D / 16);
+        uint4* at = group(tok, j % (D / 16));
+        const uint4 v = *at;
+        const uint4 n = make_uint4(nan_codes(v.x), nan_codes(v.y), nan_codes(v.z), nan_codes(v.w));
+        if (n.x | n.y | n.z | n.w) {
+          *at = make_uint4(v.x & ~n.x, v.y & ~n.y, v.z & ~n.z, v.w & ~n.w);
+          bad_tok = min(bad_tok, tok);
+        }
+      }
+      bad_tok = __reduce_min_sync(0xffffffffu, bad_tok);
+      if (lane == 0) k_nan[st] = bad_tok;
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(bar_k + 8 * st);
+        mbar_arrive(bar_raw_free);
+      }
+    }
+  } else if (busy && warp >= 4) {
+    // ------------------------------------------------------------- weights
+    const int line = (warp - 4) * 32 + lane;
+    const uint32_t lane_base = tmem + ((uint32_t)((warp - 4) * 32) << 16);
+    const uint32_t s_col = lane_base, o_col = lane_base + C::COLS / 2;
+    constexpr int CH = RB < 16 ? RB : 16;
+    float4* wmax = reinterpret_cast<float4*>(smem + C::OFF_MAX);
+    uint8_t* pb = smem + C::OFF_P;
+    float off[RB], l[RB];
+    int stage = 0;
+    uint32_t phase = 0, items = 0;
+    bool ok = true;
+    for (uint32_t i = 0;; ++i) {
+      // an expired wait is remembered, and all threads leave together below
+      ok = ok && mbar_wait(bar_k + 8 * stage, phase, abort_flag, a.err, kDevErrTimeoutCached);
+      ok = ok && mbar_wait(bar_s, i & 1u, abort_flag, a.err, kDevErrTimeoutCached);
+      ok = __all_sync(0xffffffffu, ok);
+      const int4 info = infos[stage];
+      const int b = items & 1;
+      if (ok && (info.z & kFirst))
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_q + 8 * b, (items >> 1) & 1u, abort_flag, a.err,
+                                               kDevErrTimeoutCached));
+      tc_fence_after();
+      float x[TPL][RB];
+#pragma unroll
+      for (int p = 0; p < TPL; ++p)
+#pragma unroll
+        for (int c = 0; c < RB / CH; ++c) {
+          uint32_t s[3][CH];
+#pragma unroll
+          for (int t = 0; t < 3; ++t) tmem_ld_32x32b(s_col + (p * 3 + t) * RB + c * CH, s[t]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int r = 0; r < CH; ++r)
+            x[p][c * CH + r] = fmaf(__uint_as_float(s[2][r]), T2,
+                                    fmaf(__uint_as_float(s[1][r]), T1, __uint_as_float(s[0][r])));
+        }
+      tc_fence_before();
+      mbar_arrive(bar_s_free);
+      const float4 sc = scales[stage * C::GRAN + line * TPL / 16];
+      const float* rs = item_rs(b);
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        const float f = sc.x * rs[r];
+#pragma unroll
+        for (int p = 0; p < TPL; ++p) x[p][r] = fmaf(x[p][r], f, sc.y);
+      }
+      const int tok0 = info.x + line * TPL;
+      const bool check = info.z & kCheck;
+      if (check) {
+        const int* lim = item_lim(b);
+        const int bad_tok = k_nan[stage];
+#pragma unroll
+        for (int r = 0; r < RB; ++r)
+#pragma unroll
+          for (int p = 0; p < TPL; ++p)
+            if (tok0 + p >= lim[r] || sc.w == 0.f)
+              x[p][r] = -INFINITY;
+            else if (TPL == 2 && tok0 + p == bad_tok)
+              x[p][r] = NAN;
+      }
+      bool grow = !ok || (info.z & kFirst);
+      if (!grow) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < RB; ++r)
+#pragma unroll
+          for (int p = 0; p < TPL; ++p) top = fmaxf(top, x[p][r] + off[r]);
+        grow = top > P_TOP;
+      }
+      bool o_waited = false;
+      if (vote_any(grow)) {
+        // the rows' maxima over the tile; M moves where they exceed it by 0.8
+        if (!ok) *softmax_failed = 1;
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+          float m = x[0][r];
+          if (TPL == 2) m = fmaxf(m, x[TPL - 1][r]);
+          m = warp_max(m);
+          if (lane == (r & 31)) reinterpret_cast<float*>(wmax + r)[warp - 4] = m;
+        }
+        compute_barrier();
+        const bool failed = *softmax_failed;
+        float alpha[RB];
+        const bool first = info.z & kFirst;
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+          const float4 w = wmax[r];
+          const float m = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w));
+          if (first) {
+            // a row that sees nothing in its first tile sees nothing after it
+            off[r] = P_EXP - (m == -INFINITY ? 0.f : m);
+            l[r] = 0.f;
+            alpha[r] = 1.f;
+          } else {
+            const float to = m + off[r] > P_TOP ? P_EXP - m : off[r];
+            alpha[r] = ex2_approx(to - off[r]);
+            off[r] = to;
+            l[r] *= alpha[r];
+          }
+        }
+        compute_barrier();  // wmax and the flag may be written again
+        if (failed) break;
+        if (!first) {
+          ok = __all_sync(0xffffffffu, mbar_wait(bar_o, (i - 1) & 1u, abort_flag, a.err,
+                                                 kDevErrTimeoutCached));
+          o_waited = true;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < N / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld_32x32b(o_col + 16 * c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha[(16 * c + e) % RB]);
+            tmem_st_32x32b_x16(o_col + 16 * c, o);
+          }
+          tmem_wait_st();
+        }
+      }
+      if (i > 0 && !o_waited) {  // P V of the tile before has read the weights
+        const bool w = mbar_wait(bar_o, (i - 1) & 1u, abort_flag, a.err, kDevErrTimeoutCached);
+        ok = __all_sync(0xffffffffu, w) && ok;
+      }
+#pragma unroll
+      for (int p = 0; p < TPL; ++p)
+#pragma unroll
+        for (int r = 0; r < RB; r += 2) {
+          const float p0 = ex2_approx(x[p][r] + off[r]), p1 = ex2_approx(x[p][r + 1] + off[r + 1]);
+          l[r] = fmaf(p0, sc.z, l[r]);
+          l[r + 1] = fmaf(p1, sc.z, l[r + 1]);
+          uint16_t t[3];
+          split3(__floats2half2_rn(p0, p1), t);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            const int n = (p * 3 + k) * RB + r;
+            pb[n * 128 + (line ^ ((n & 7) << 4))] = (uint8_t)t[k];
+            pb[(n + 1) * 128 + (line ^ (((n + 1) & 7) << 4))] = (uint8_t)(t[k] >> 8);
+          }
+        }
+      if (check) {
+        // Codes of tokens that no row sees become 0 (their weight is 0, but 0 *
+        // NaN is not); NaN codes of new tokens that only later rows see become 0
+        // and are put into those rows' results at the end.
+        const bool w = mbar_wait(bar_v + 8 * stage, phase, abort_flag, a.err, kDevErrTimeoutCached);
+        ok = __all_sync(0xffffffffu, w) && ok;
+        uint8_t* vl = smem + (stage * 2 + 1) * TILE + line * 128;
+#pragma unroll
+        for (int p = 0; p < TPL; ++p) {
+          const int tok = tok0 + p;
+          const bool gone = tok >= info.y || sc.w == 0.f;
+          const bool look = a.causal && tok >= info.w;
+          if (!gone && !look) continue;
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) {
+            uint4* at = reinterpret_cast<uint4*>(vl + (((p * (D / 16) + c) ^ (line & 7)) << 4));
+            if (gone) {
+              *at = make_uint4(0, 0, 0, 0);
+              continue;
+            }
+            const uint4 v = *at;
+            const uint32_t bad[4] = {nan_codes(v.x), nan_codes(v.y), nan_codes(v.z), nan_codes(v.w)};
+            if (bad[0] | bad[1] | bad[2] | bad[3]) {
+              *at = make_uint4(v.x & ~bad[0], v.y & ~bad[1], v.z & ~bad[2], v.w & ~bad[3]);
+              uint32_t rows = 0;
+#pragma unroll
+              for (int r = 0; r < RB; ++r)
+                if (tok < item_lim(b)[r]) rows |= 1u << r;
+              for (int e = 0; e < 16; ++e)
+                if (bad[e >> 2] >> (8 * (e & 3)) & 1u)
+                  atomicOr(&poison[p * D + c * 16 + e], rows);
+            }
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      mbar_arrive(bar_p);
 
-    for (int tile = tile0; tile < tile1; ++tile) {
-      const int st = stage;
-      const uint32_t ph = phase;
-      if (++stage == C::ST) {
+      if (info.z & kLast) {
+        // ---------------------------------------------------- the item's end
+        const bool w = mbar_wait(bar_o, i & 1u, abort_flag, a.err, kDevErrTimeoutCached);
+        ok = __all_sync(0xffffffffu, w) && ok;
+        compute_barrier();  // all of `poison` is there
+        tc_fence_after();
+        // O^T: this thread's byte is column d of token half `half` of the lines
+        const int half = TPL == 2 ? line >> 6 : 0, d = TPL == 2 ? line & 63 : line;
+        float v[RB];
+#pragma unroll
+        for (int c = 0; c < RB / CH; ++c) {
+          uint32_t o[3][CH];
+#pragma unroll
+          for (int t = 0; t < 3; ++t)
+            tmem_ld_32x32b(o_col + (half * 3 + t) * RB + c * CH, o[t]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int r = 0; r < CH; ++r)
+            v[c * CH + r] =
+                fmaf(__uint_as_float(o[2][r]), T2,
+                     fmaf(__uint_as_float(o[1][r]), T1, __uint_as_float(o[0][r])));
+        }
+        const uint32_t bits = poison[line];
+        if (bits) {
+#pragma unroll
+          for (int r = 0; r < RB; ++r)
+            if (bits >> r & 1u) v[r] = NAN;
+        }
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+          const float s = warp_add(l[r]);
+          if (lane == (r & 31)) reinterpret_cast<float*>(wmax + r)[warp - 4] = s;
+        }
+        float* other = reinterpret_cast<float*>(pb);  // the weights have been read
+        if (TPL == 2 && half) {
+#pragma unroll
+          for (int r = 0; r < RB; ++r) other[r * 64 + d] = v[r];
+        }
+        compute_barrier();
+        poison[line] = 0;
+        const ItemInfo it = *item_info(b);
+        if (TPL == 1 || !half) {
+          // a piece that continues an earlier CTA's item goes to slot 0, one
+          // that begins here and ends elsewhere to slot 1
+          float* part = a.part + ((size_t)blockIdx.x * 2 + (it.starts ? 1 : 0)) * kCachedPartFloats;
+#pragma unroll
+          for (int r = 0; r < RB; ++r) {
+            if (r >= it.n_rows) break;
+            if (TPL == 2) v[r] += other[r * 64 + d];
+            const float4 w4 = wmax[r];
+            const float sum = (w4.x + w4.y) + (w4.z + w4.w);
+            if (it.starts && it.ends) {
+              const int gr = it.block * RB + r;
+              const int tok = gr / a.group, gq = gr - tok * a.group;
+              a.o[(int64_t)(it.row0 + tok) * a.o_stride + (it.head * a.group + gq) * D + d] =
+                  to_out<BF>(sum == 0.f ? 0.f : v[r] / sum);
+            } else {
+              part[r * D + d] = v[r];
+              if (line == 0) {
+                // a row that saw nothing has no maximum
+                part[kCachedPartRows * 128 + r] = sum == 0.f ? -INFINITY : P_EXP - off[r];
+                part[kCachedPartRows * 129 + r] = sum;
+              }
+            }
+          }
+        }
+        tc_fence_before();
+        mbar_arrive(bar_q_empty + 8 * b);
+        compute_barrier();  // `other`, wmax and poison may be written again
+        ++items;
+        if (info.z & kFinal) break;
+      }
+      if (++stage == ST) {
         stage = 0;
         phase ^= 1;
       }
-      if ((tile & (kg - 1)) != my_kg) continue;
-      // on an expired wait the loop runs on over stale data: the barriers below
-      // are met by every warp, and the host learns of the error
-      mbar_wait(bar_full + 8 * st, ph, abort_flag, a.err, kDevErrTimeoutCached);
-      __syncwarp();
-      const uint8_t *sk = smem + st * 2 * C::TILE, *sv = sk + C::TILE;
-      const int kbase = tile * KT;
-      float s[KT / 8][4];
-#pragma unroll
-      for (int j = 0; j < KT / 8; ++j) {
-        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-        const int row = 8 * j + g;
-        uint4 w[D / 64];
-#pragma unroll
-        for (int i = 0; i < D / 64; ++i) 
-          w[i] = *reinterpret_cast<const uint4*>(sk + tile_off<D>(row, t * (D / 64) + i));
-#pragma unroll
-        for (int i = 0; i < D / 64; ++i) {
-          const uint32_t ww[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t b0, b1;
-            codes_to_half(ww[q], b0, b1);
-            mma16816(s[j], qf[4 * i + q], b0, b1);
-          }
-        }
-      }
-      float ivs[4];
-      const bool edge = kbase + KT > lim_min;
-      float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        const float4 sc = scales[st * 4 + kk];
-        ivs[kk] = sc.z;
-        const float c0 = sc.x * rs[0], c1 = sc.x * rs[1];
-#pragma unroll
-        for (int j = 2 * kk; j < 2 * kk + 2; ++j) {
-          s[j][0] = fmaf(s[j][0], c0, sc.y);
-          s[j][1] = fmaf(s[j][1], c0, sc.y);
-          s[j][2] = fmaf(s[j][2], c1, sc.y);
-          s[j][3] = fmaf(s[j][3], c1, sc.y);
-          if (edge || sc.w == 0.f) {
-            const int key = kbase + 8 * j + 2 * t;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (key + (e & 1) >= lim[e >> 1] || sc.w == 0.f) s[j][e] = -INFINITY;
-          }
-          top[0] = fmaxf(top[0], fmaxf(s[j][0], s[j][1]));
-          top[1] = fmaxf(top[1], fmaxf(s[j][2], s[j][3]));
-        }
-      }
-      float off[2], alpha[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float mn = fmaxf(m[h], quad_max(top[h]));
-        const float mu = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: weights of 0
-        alpha[h] = ex2_approx(m[h] - mu);
-        off[h] = P_SHIFT - mu;
-        m[h] = mn;
-        l[h] *= alpha[h];
-      }
-      uint32_t p[4][4];
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        float sum[2] = {0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float* x = s[2 * kk + j];
-          x[0] = ex2_approx(x[0] + off[0]);
-          x[1] = ex2_approx(x[1] + off[0]);
-          x[2] = ex2_approx(x[2] + off[1]);
-          x[3] = ex2_approx(x[3] + off[1]);
-          sum[0] += x[0] + x[1];
-          sum[1] += x[2] + x[3];
-          p[kk][2 * j] = pack_half2(x[0], x[1]);
-          p[kk][2 * j + 1] = pack_half2(x[2], x[3]);
-        }
-        l[0] = fmaf(sum[0], ivs[kk], l[0]);
-        l[1] = fmaf(sum[1], ivs[kk], l[1]);
-      }
-      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          o[i][0] *= alpha[0];
-          o[i][1] *= alpha[0];
-          o[i][2] *= alpha[1];
-          o[i][3] *= alpha[1];
-        }
-      }
-      // Codes of tokens that no row sees are taken as 0 (their weight is 0, but
-      // 0 * NaN is not); a NaN code of a new token that only later rows see is
-      // taken as 0 here and set in those rows below.
-      const bool tail = kbase + KT > len;
-      const bool look = a.causal && fresh > 1 && edge;
-      uint32_t found = 0;
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        uint32_t v[4][D / 32];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = 16 * kk + 2 * t + (i & 1) + (i >> 1) * 8;
-          if (D == 128) {
-            const uint4 w = *reinterpret_cast<const uint4*>(sv + tile_off<D>(row, g));
-            v[i][0] = w.x;
-            v[i][1] = w.y;
-            v[i][D / 32 - 2] = w.z;
-            v[i][D / 32 - 1] = w.w;
-          } else {
-            const uint2 w =
-                *reinterpret_cast<const uint2*>(sv + tile_off<D>(row, g >> 1) + (g & 1) * 8);
-            v[i][0] = w.x;
-            v[i][1] = w.y;
-          }
-          if (tail && kbase + row >= len)
-#pragma unroll
-            for (int q = 0; q < D / 32; ++q) v[i][q] = 0;
-          if (look && kbase + row >= lim_min)
-#pragma unroll
-            for (int q = 0; q < D / 32; ++q) {
-              const uint32_t bad = nan_codes(v[i][q]);
-              found |= bad;
-              v[i][q] &= ~bad;
-            }
-        }
-        if (scales[st * 4 + kk].w == 0.f)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int q = 0; q < D / 32; ++q) v[i][q] = 0;
-#pragma unroll
-        for (int q = 0; q < D / 32; ++q) {
-          uint32_t b0[4], b1[4];
-          codes_to_half(__byte_perm(v[0][q], v[1][q], 0x5140), b0[0], b0[1]);
-          codes_to_half(__byte_perm(v[0][q], v[1][q], 0x7362), b0[2], b0[3]);
-          codes_to_half(__byte_perm(v[2][q], v[3][q], 0x5140), b1[0], b1[1]);
-          codes_to_half(__byte_perm(v[2][q], v[3][q], 0x7362), b1[2], b1[3]);
-#pragma unroll
-          for (int n = 0; n < 4; ++n) mma16816(o[4 * q + n], p[kk], b0[n], b1[n]);
-        }
-      }
-      if (look && __any_sync(0xffffffffu, found != 0)) {
-        for (int key = max(kbase, lim_min); key < min(len, kbase + KT); ++key)
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int d = (2 * t + e) * (D / 8) + i;  // the output's column
-              const uint32_t code = sv[tile_off<D>(key - kbase, d >> 4) + (d & 15)];
-              if ((code & 0x7F) == 0x7F) {
-                if (key < lim[0]) o[i][e] = NAN;
-                if (key < lim[1]) o[i][2 + e] = NAN;
-              }
-            }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_empty + 8 * st);
     }
+  }
 
-    // The groups' sums meet: outputs [row][D] (16-byte groups permuted so that
-    // the stores hit every bank once), maxima and row sums.
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float ls = quad_sum(l[h]);
-      if (t == 0) ml[warp * 16 + g + 8 * h] = make_float2(m[h], ls);
-      float4* dst = reinterpret_cast<float4*>(comb + (warp * 16 + g + 8 * h) * D);
-      // thread t holds columns [2t * D/8, (2t + 2) * D/8): first o[.][0], then o[.][1]
-#pragma unroll
-      for (int u = 0; u < D / 16; ++u) {
-        const int e = u / (D / 32), i = 4 * (u % (D / 32));
-        const int perm = D == 128 ? (2 * t + g) & 7 : (g & 1) | (t >> 1) << 1;
-        dst[t * (D / 16) + (u ^ perm)] = make_float4(o[i][2 * h + e], o[i + 1][2 * h + e],
-                                                     o[i + 2][2 * h + e], o[i + 3][2 * h + e]);
-      }
-    }
-    compute_barrier();
-    const bool starts = r.unit == 0, ends = r.unit + n_units == r.units;
-    // a piece that continues an earlier CTA's item goes to slot 0, one that
-    // this CTA begins and does not end to slot 1
-    float* part = a.part + ((size_t)blockIdx.x * 2 + (starts ? 1 : 0)) * kCachedPartFloats;
-    for (int i = threadIdx.x; i < n_rows * (D / 4); i += 32 * CWARPS) {
-      const int lr = i / (D / 4), c = i % (D / 4);
-      const int rr = lr & 15, w0 = lr >> 4;
-      const int tt = c / (D / 16), u = c % (D / 16);
-      const int perm = D == 128 ? (2 * tt + rr) & 7 : (rr & 1) | (tt >> 1) << 1;
-      const int pos = tt * (D / 16) + (u ^ perm);
-      float top = -INFINITY;
-      for (int k = 0; k < kg; ++k) top = fmaxf(top, ml[(w0 + rt * k) * 16 + rr].x);
-      const float mu = top == -INFINITY ? 0.f : top;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      float sum = 0.f;
-      for (int k = 0; k < kg; ++k) {
-        const float2 x = ml[(w0 + rt * k) * 16 + rr];
-        const float f = ex2_approx(x.x - mu);
-        const float4 y =
-            reinterpret_cast<const float4*>(comb + ((w0 + rt * k) * 16 + rr) * D)[pos];
-        sum = fmaf(x.y, f, sum);
-        acc.x = fmaf(y.x, f, acc.x);
-        acc.y = fmaf(y.y, f, acc.y);
-        acc.z = fmaf(y.z, f, acc.z);
-        acc.w = fmaf(y.w, f, acc.w);
-      }
-      if (starts && ends) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const int gr = block * 16 * rt + lr;
-        const int tok = gr / a.group, gq = gr - tok * a.group;
-        store_out4<BF>(a.o + (int64_t)(row0 + tok) * a.o_stride + (head * a.group + gq) * D + 4 * c,
-                       make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-      } else {
-        reinterpret_cast<float4*>(part + lr * D)[c] = acc;
-        if (c == 0) {
-          part[kCachedPartRows * 128 + lr] = top;
-          part[kCachedPartRows * 129 + lr] = sum;
-        }
-      }
-    }
-    compute_barrier();
-    run_next(a, seqs, r, n_units);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::COLS);
   }
 }
 
 // Adds the pieces of the items that attention left in parts. Block c looks
 // after the item that CTA c began and did not end: its slot 1, then slot 0 of
 // the CTAs that follow, in order.
-template <int D, bool BF>
+template <int D, int RB, bool BF>
 __global__ void __launch_bounds__(256) cached_join_kernel(const CachedArgs a, int ctas) {
   griddep_launch_dependents();
   griddep_wait();  // the pieces are the previous kernel's output
   const int c0 = blockIdx.x;
-  if (!(a.meta[c0 * 4] & 2)) return;
+  if (a.meta[c0 * 4] != 2) return;
   const int seq = a.meta[c0 * 4 + 1], sub = a.meta[c0 * 4 + 2];
   const int row0 = a.cu ? a.cu[seq] : seq;
   const int fresh = a.cu ? a.cu[seq + 1] - row0 : 1;
-  const int blocks = row_blocks(a, fresh);
+  const int blocks = (fresh * a.group + RB - 1) / RB;
   const int head = sub / blocks, block = sub - head * blocks;
-  const int n_rows = min(16 * a.rt, fresh * a.group - block * 16 * a.rt);
+  const int n_rows = min(RB, fresh * a.group - block * RB);
   int last = c0 + 1;  // the CTA that ends the item
-  while (last < ctas - 1 && (a.meta[last * 4] & 4)) ++last;
-  for (int i = blockIdx.y * 256 + threadIdx.x; i < n_rows * (D / 4); i += 256 * gridDim.y) {
-    const int lr = i / (D / 4), c = i % (D / 4);
-    float top = -INFINITY, sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = c0; k <= last; ++k) {
+  while (last < ctas - 1 && a.meta[last * 4] == 4) ++last;
+  for (int i = threadIdx.x; i < n_rows * D; i += 256) {
+    const int r = i / D, d = i % D;
+    float top = -INFINITY, sum = 0.f, acc = 0.f;
+    for (int k = c0; k <= last && k < ctas; ++k) {
       const float* part = a.part + ((size_t)k * 2 + (k == c0 ? 1 : 0)) * kCachedPartFloats;
-      const float pm = part[kCachedPartRows * 128 + lr], pl = part[kCachedPartRows * 129 + lr];
-      const float4 y = reinterpret_cast<const float4*>(part + lr * D)[c];
+      const float pm = part[kCachedPartRows * 128 + r], pl = part[kCachedPartRows * 129 + r];
+      const float y = part[r * D + d];
       const float mn = fmaxf(top, pm);
       const float mu = mn == -INFINITY ? 0.f : mn;
       const float f0 = ex2_approx(top - mu), f1 = ex2_approx(pm - mu);
       top = mn;
       sum = fmaf(sum, f0, pl * f1);
-      acc.x = fmaf(acc.x, f0, y.x * f1);
-      acc.y = fmaf(acc.y, f0, y.y * f1);
-      acc.z = fmaf(acc.z, f0, y.z * f1);
-      acc.w = fmaf(acc.w, f0, y.w * f1);
+      acc = fmaf(acc, f0, y * f1);
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int gr = block * 16 * a.rt + lr;
+    const int gr = block * RB + r;
     const int tok = gr / a.group, gq = gr - tok * a.group;
-    store_out4<BF>(a.o + (int64_t)(row0 + tok) * a.o_stride + (head * a.group + gq) * D + 4 * c,
-                   make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+    a.o[(int64_t)(row0 + tok) * a.o_stride + (head * a.group + gq) * D + d] =
+        to_out<BF>(sum == 0.f ? 0.f : acc / sum);
   }
 }
 
@@ -717,19 +1006,37 @@ bool pool_map(CUtensorMap* map, const uint8_t* codes, long long lines, int box_l
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, bool BF>
+template <int D, int RB, bool BF>
 sam3_status_t launch_cached(sam3_ctx_t* ctx, const CUtensorMap& mk, const CUtensorMap& mv,
-                            const CachedArgs& a) {
-  const uint32_t bit = (uint32_t)kSmemCached << ((D == 128) * 2 + BF);
-  sam3_status_t st = ensure_smem_attr(ctx, bit, cached_attn_kernel<D, BF>, Cfg<D>::SMEM,
+                            CachedArgs& a, long long capacity) {
+  using C = Cfg<D, RB>;
+  constexpr int variant = (RB == 4 ? 0 : RB == 8 ? 1 : RB == 16 ? 2 : 3) * 4 + (D == 128) * 2 + BF;
+  sam3_status_t st = ensure_smem_attr(ctx, (uint32_t)kSmemCached << variant,
+                                      cached_attn_kernel<D, RB, BF>, C::SMEM,
                                       "attention_cached smem attribute");
   if (st != SAM3_OK) return st;
-  const int ctas = ctx->num_sms;
-  cudaError_t e = launch_pdl(cached_attn_kernel<D, BF>, dim3(ctas), dim3(THREADS), Cfg<D>::SMEM,
+  const long long blocks = ((long long)a.max_new * a.group + RB - 1) / RB;
+  const long long tiles = (capacity + C::TT - 1) / C::TT;
+  if (blocks * a.kv_heads * a.n_seqs * tiles > 0x7FFFFFFFll)
+    return set_error(ctx, SAM3_ERR_SHAPE, "attention_cached: too much work for one call");
+  a.whole = tiles <= UNIT_TILES;
+  const int ctas = 2 * ctx->num_sms;
+  cudaError_t e = launch_pdl(cached_attn_kernel<D, RB, BF>, dim3(ctas), dim3(THREADS), C::SMEM,
                              ctx->stream, mk, mv, a);
-  if ((st = check_launch_ret(ctx, e, "cached_attn_kernel")) != SAM3_OK) return st;
-  e = launch_pdl(cached_join_kernel<D, BF>, dim3(ctas), dim3(256), 0, ctx->stream, a, ctas);
+  st = check_launch_ret(ctx, e, "cached_attn_kernel");
+  if (st != SAM3_OK || a.whole) return st;  // whole items: nothing to join
+  e = launch_pdl(cached_join_kernel<D, RB, BF>, dim3(ctas), dim3(256), 0, ctx->stream, a, ctas);
   return check_launch_ret(ctx, e, "cached_join_kernel");
+}
+
+template <int D, bool BF>
+sam3_status_t pick_rows(sam3_ctx_t* ctx, const CUtensorMap& mk, const CUtensorMap& mv,
+                        CachedArgs& a, long long capacity, long long rows) {
+  if (rows <= 4) return launch_cached<D, 4, BF>(ctx, mk, mv, a, capacity);
+  if (rows <= 8) return launch_cached<D, 8, BF>(ctx, mk, mv, a, capacity);
+  // 16 rows of head_dim 64 take 96 columns, as 32 rows of 128 do
+  if (D == 64 || rows <= 16) return launch_cached<D, 16, BF>(ctx, mk, mv, a, capacity);
+  return launch_cached<128, 32, BF>(ctx, mk, mv, a, capacity);
 }
 
 }  // namespace
@@ -757,19 +1064,17 @@ sam3_status_t attention_cached(sam3_ctx_t* ctx, const sam3_kv_cache_t* c, int dt
     return set_error(ctx, SAM3_ERR_SHAPE,
                      "attention_cached: row strides must be multiples of 8 of at least heads * "
                      "head_dim");
+  const long long capacity = (long long)table_stride * c->page_size;
+  const long long most = (long long)max_new * (heads / c->kv_heads);  // rows per K/V head
   if (n_seqs <= 0 || n_seqs > MAX_SEQS || rows <= 0 || max_new <= 0 || max_new > rows ||
-      table_stride <= 0 || (long long)table_stride * c->page_size > kMaxContext ||
+      table_stride <= 0 || capacity > kMaxContext || most > kMaxContext ||
       (!cu_new && (max_new != 1 || rows < n_seqs)))
     return set_error(ctx, SAM3_ERR_SHAPE, "attention_cached: bad shape (at most %d sequences)",
                      MAX_SEQS);
-  CachedArgs a;
-  a.group = heads / c->kv_heads;
-  const long long most = (long long)max_new * a.group;  // query rows per K/V head
-  a.rt = most <= 16 ? 1 : most <= 32 ? 2 : 4;
-  const long long blocks = (most + 16 * a.rt - 1) / (16 * a.rt);
-  const long long tiles = ((long long)table_stride * c->page_size + KT - 1) / KT;
-  if (most > 0x7FFFFF00ll || blocks * c->kv_heads * n_seqs * tiles > 0x7FFFFFFFll)
+  if ((most + 31) / 32 * c->kv_heads * n_seqs * ((capacity + 127) / 128) > 0x7FFFFFFFll)
     return set_error(ctx, SAM3_ERR_SHAPE, "attention_cached: too much work for one call");
+  CachedArgs a{};
+  a.group = heads / c->kv_heads;
   a.q = q;
   a.o = o;
   a.q_stride = q_stride;
@@ -793,7 +1098,7 @@ sam3_status_t attention_cached(sam3_ctx_t* ctx, const sam3_kv_cache_t* c, int dt
   a.scale_log2 = scale * 1.4426950408889634f;
   const long long lines =
       (long long)c->num_pages * c->kv_heads * c->page_size * c->head_dim / 128;
-  const int box = std::min(c->page_size, KT) * c->head_dim / 128;
+  const int box = c->page_size * c->head_dim / 128;
   CUtensorMap mk, mv;
   if (!pool_map(&mk, c->k, lines, box) || !pool_map(&mv, c->v, lines, box))
     return set_error(ctx, SAM3_ERR_CUDA, "attention_cached: cuTensorMapEncodeTiled failed");
@@ -801,8 +1106,10 @@ sam3_status_t attention_cached(sam3_ctx_t* ctx, const sam3_kv_cache_t* c, int dt
   ProfScope prof(ctx, SAM3_PROF_ATTENTION, 0.0, 4.0 * rows * width);
   const bool bf = dtype == SAM3_BF16;
   if (c->head_dim == 128)
-    return bf ? launch_cached<128, true>(ctx, mk, mv, a) : launch_cached<128, false>(ctx, mk, mv, a);
-  return bf ? launch_cached<64, true>(ctx, mk, mv, a) : launch_cached<64, false>(ctx, mk, mv, a);
+    return bf ? pick_rows<128, true>(ctx, mk, mv, a, capacity, most)
+              : pick_rows<128, false>(ctx, mk, mv, a, capacity, most);
+  return bf ? pick_rows<64, true>(ctx, mk, mv, a, capacity, most)
+            : pick_rows<64, false>(ctx, mk, mv, a, capacity, most);
 }
 
 }  // namespace sam3

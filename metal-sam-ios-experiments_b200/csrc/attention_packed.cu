@@ -211,7 +211,15 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
     prefetch_tmap(&map_k);
     prefetch_tmap(&map_v);
   }
-  griddep_launch_dependents();
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), C::COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_launch_dependents();  // behind the allocation: the next kernel allocates too
   griddep_wait();  // offsets and rows may be earlier kernels' outputs
   const int unit = blockIdx.x % a.units;
   if (warp == 0) {
@@ -222,14 +230,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
       item_slot[2] = it.tile;
     }
   }
-  if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), C::COLS);
-    tmem_relinquish();
-  }
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
   const int row0 = item_slot[0], len = item_slot[1], tile = item_slot[2];
 
   if (tile >= 0) {

@@ -186,8 +186,8 @@ size_t carve(sam3_ctx_t* ctx, char* base) {
   ctx->rope_pos_pruned = cv.take<int32_t>(B * keep);
   ctx->rope_pruned = cv.take<float>(B * keep * hd);
   ctx->idx = cv.take<int32_t>(B * S);
-  ctx->cached_part = cv.take<float>((size_t)ctx->num_sms * 2 * kCachedPartFloats);
-  ctx->cached_meta = cv.take<int32_t>((size_t)ctx->num_sms * 4);
+  ctx->cached_part = cv.take<float>((size_t)ctx->num_sms * 4 * kCachedPartFloats);
+  ctx->cached_meta = cv.take<int32_t>((size_t)ctx->num_sms * 8);
   ctx->image = cv.take<uint16_t>(B * (size_t)c.image_size * c.image_size * 3);
   ctx->block_rows = B * S;
   ctx->token_rows = B * R;

@@ -51,8 +51,8 @@ struct sam3_ctx {
   uint16_t* feats = nullptr;    // [B*keep, D] staging for the host API
   // Pieces of sequences that attention_cached splits over CTAs, and which CTA
   // left which (attention_cached.cu).
-  float* cached_part = nullptr;   // [num_sms, 2, kCachedPartFloats]
-  int32_t* cached_meta = nullptr; // [num_sms, 4]
+  float* cached_part = nullptr;   // [2 * num_sms, 2, kCachedPartFloats]
+  int32_t* cached_meta = nullptr; // [2 * num_sms, 4]
   int rope_ready = 0;
   // Block-level scratch used by sam3_vit_block & co. outside the encoder.
   size_t block_rows = 0;        // rows the block scratch can hold (plain encoder)
@@ -105,12 +105,12 @@ sam3_status_t device_error_status(sam3_ctx_t* ctx, int err);
 // the attribute belongs to the device, and each context is bound to one.
 enum : uint32_t {
   kSmemAttn = 1u, kSmemWs = 2u, kSmemWsc = 4u, kSmemGemm = 8u /* << MODE */, kSmemPrune = 64u,
-  kSmemAttnPP = 128u, kSmemCached = 256u /* << variant, 4 of them */,
-  kSmemPacked = 4096u /* << variant, 4 of them */
+  kSmemAttnPP = 128u, kSmemPacked = 256u /* << variant, 4 of them */,
+  kSmemCached = 4096u /* << variant, 16 of them */
 };
-// One piece: 64 rows of up to 128 unnormalised outputs, then their 64 running
-// maxima and 64 row sums.
-constexpr int kCachedPartRows = 64;
+// One piece: 32 rows of up to 128 unnormalised outputs, then their 32 running
+// maxima and 32 row sums.
+constexpr int kCachedPartRows = 32;
 constexpr int kCachedPartFloats = kCachedPartRows * 128 + 2 * kCachedPartRows;
 template <typename Kernel>
 sam3_status_t ensure_smem_attr(sam3_ctx_t* ctx, uint32_t bit, Kernel kernel, int bytes,
