@@ -11,7 +11,7 @@
 // codes go from global to shared memory by TMA and from there into tcgen05.mma
 // (kind::f8f6f4) as they are: no thread touches them.
 //   S^T[line, column] = K[line, 128 bytes] . Q[column, 128 bytes]
-//   O^T[byte, column] += V[line, byte] . P[column, line]
+//   O^T[byte, column] += V[line, byte] . P[line, column]
 // A line is 128 bytes of codes: one token of head_dim 128 or two of 64. The
 // large operand is the M = 128 side, the few rows are columns of the N side, and
 // each row takes three columns, the terms of an exact split of an 11-bit
@@ -31,17 +31,18 @@
 // page by page through the table; warp 1 issues the MMAs; warp 2 loads and
 // splits the next item's queries; warps 4-7, one thread per line, turn scores
 // into weights: a handful of exponentials per thread and tile. The running
-// maximum moves only when a score exceeds it by 0.8, found by one barrier with
+// maximum moves only when a score exceeds it by 2.8, found by one barrier with
 // a vote; only then are maxima exchanged and O^T rescaled in tensor memory.
 //
-// Split: the context is cut into units of tiles, the units of all (sequence,
-// K/V head, row block) are counted through, and each of the 2 * num_sms CTAs
-// takes an equal run of them, whatever the sequences' lengths. Where a run
+// Split: the context is cut into units of tiles, the units of all items
+// (sequence, K/V head, row block) are counted through, an item's begin and end
+// as two more, and each of the 2 * num_sms CTAs takes an equal run of them,
+// whatever the sequences' lengths. Where a run
 // begins or ends inside an item, the CTA leaves its unnormalised sum, maximum
 // and row sum in the workspace, and cached_join_kernel adds the pieces in the
 // order of the CTAs (no atomics: the result does not depend on timing).
 //
-// V's scale joins the exponent: P = 2^(x + log2(vs) - M + 8) with M the running
+// V's scale joins the exponent: P = 2^(x + log2(vs) - M + 6) with M the running
 // maximum of x + log2(vs), at most 2^8.8 < 448; the row sum adds P / vs in fp32.
 #include <algorithm>
 
@@ -58,7 +59,8 @@ constexpr int MAX_SEQS = SAM3_CACHED_MAX_SEQS;
 constexpr int LINES = 128;             // lines per tile
 constexpr int TILE = LINES * 128;      // bytes of K or V per tile
 constexpr int UNIT_TILES = 4;          // tiles per unit of small jobs
-constexpr float P_EXP = 8.f;           // the largest weight at its maximum is 2^8
+constexpr int ITEM_COST = 2;           // what an item costs besides its tiles, in tiles
+constexpr float P_EXP = 6.f;           // the weight at the running maximum is 2^6
 constexpr float P_TOP = 8.8f;          // and may grow to 2^8.8 < 448 before M moves
 constexpr float T1 = 1.f / 16, T2 = 1.f / 256;  // weights of the second and third term
 enum : int { kFirst = 1, kLast = 2, kFinal = 4, kCheck = 8 };
@@ -70,21 +72,29 @@ struct Cfg {
   static constexpr int TT = LINES * TPL;          // tokens per tile
   static constexpr int NC = 3 * RB * TPL;         // columns used
   static constexpr int N = (NC + 15) / 16 * 16;   // columns of the MMAs
+  static constexpr int PW = N <= 32 ? 32 : N <= 64 ? 64 : 128;  // bytes of a line of P
   static constexpr int ST = N <= 32 ? 3 : 2;      // ring stages (K and V tile each)
   static constexpr uint32_t COLS = N <= 16 ? 32 : N <= 32 ? 64 : N <= 64 ? 128 : 256;
   static constexpr int GRAN = TT / 16;            // scale entries per tile (16 tokens)
   static constexpr int OFF_Q = ST * 2 * TILE;               // [2][N][128]
-  static constexpr int OFF_P = OFF_Q + 2 * N * 128;         // [N][128]
-  static constexpr int OFF_SCALE = OFF_P + N * 128;         // [ST][GRAN] float4
+  static constexpr int OFF_P = OFF_Q + 2 * N * 128;         // [LINES][PW]
+  static constexpr int OFF_SCALE = OFF_P + LINES * PW;      // [ST][GRAN] float4
   static constexpr int OFF_INFO = OFF_SCALE + ST * GRAN * 16;     // [ST] int4
   static constexpr int OFF_ITEM = OFF_INFO + ST * 16;       // [2] ItemInfo
-  static constexpr int ITEM = 32 + RB * 8;
+  static constexpr int ITEM = 16 + RB * 16;
   static constexpr int OFF_MAX = OFF_ITEM + 2 * ITEM;       // [RB] float4
   static constexpr int OFF_POISON = OFF_MAX + RB * 16;      // [128] u32
   static constexpr int OFF_BAR = OFF_POISON + 512;
   static constexpr int BARS = 3 * ST + 4 + 7;
   static constexpr int OFF_MISC = OFF_BAR + BARS * 8;
   static constexpr int SMEM = OFF_MISC + 128 + 1024;
+  // column of term t of row r for token p of a line: a pair of rows takes six
+  // neighbours, as split3 gives them
+  static constexpr __host__ __device__ int col(int p, int r, int t) {
+    return (p * RB + r) / 2 * 6 + 2 * t + (r & 1);
+  }
+  // row of a column (any row for those not used)
+  static constexpr __host__ __device__ int row_of(int n) { return (n / 6 * 2 + (n & 1)) % RB; }
 };
 static_assert(2 * (Cfg<128, 8>::SMEM + 1024) <= 228 * 1024, "two CTAs per SM");
 static_assert(2 * (Cfg<128, 32>::SMEM + 1024) <= 228 * 1024, "two CTAs per SM");
@@ -111,7 +121,7 @@ struct CachedArgs {
 
 // What the query warp tells the others of an item (smem).
 struct ItemInfo {
-  int row0, head, block, n_rows, starts, ends, pad0, pad1;
+  int n_rows, starts, ends, pad;
 };
 
 __device__ __forceinline__ bool vote_any(bool p) {  // over warps 4-7
@@ -132,10 +142,22 @@ __device__ __forceinline__ float warp_max(float v) {
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
-__device__ __forceinline__ float warp_add(float v) {
+// Sums of RB values over the warp: lane i returns that of value i * RB / 32.
+template <int RB>
+__device__ __forceinline__ float warp_add(float (&v)[RB]) {
+  const int lane = threadIdx.x & 31;
+  int o = 16;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+  for (int n = RB / 2; n > 0; n /= 2, o /= 2)
+#pragma unroll
+    for (int k = 0; k < n; ++k) {
+      const bool up = lane & o;
+      const float keep = up ? v[k + n] : v[k], send = up ? v[k] : v[k + n];
+      v[k] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+#pragma unroll
+  for (int k = 16 / RB; k > 0; k /= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], k);
+  return v[0];
 }
 
 // The three terms of a pair of fp16 numbers of at most 448, as code pairs:
@@ -173,11 +195,15 @@ __device__ __forceinline__ Seq load_seq(const CachedArgs& a, int i, bool report)
   return s;
 }
 
-// A run of units over the items (sequence; K/V head and row block).
+// A run of cost over the items (sequence; K/V head and row block): an item costs
+// `extra` and then one for each of its units. A run that ends inside the extra
+// part leaves the item to the next CTA, one that begins there takes it from its
+// first unit.
 template <int D, int RB>
 struct Run {
-  int seq, sub, unit, left;  // where it is, and the units to go
-  int unit_tiles;
+  int seq, sub, unit;        // where it is
+  int left;                  // cost to go, with the extra part of this item behind it
+  int unit_tiles, extra;
   Seq s;
   int units, blocks, tiles;  // of the sequence
 
@@ -187,14 +213,17 @@ struct Run {
     tiles = s.fresh ? (s.len + Cfg<D, RB>::TT - 1) / Cfg<D, RB>::TT : 0;
     units = (tiles + unit_tiles - 1) / unit_tiles;
   }
-  // `at`: units of the sequence before the run's first
-  __device__ __forceinline__ void start(const CachedArgs& a, int seq_, int at, int left_, int ut) {
+  // `at`: cost of the sequence before the run's begin
+  __device__ __forceinline__ void start(const CachedArgs& a, int seq_, int at, int cost, int ut,
+                                        int ex) {
     seq = seq_;
-    left = left_;
     unit_tiles = ut;
+    extra = ex;
     enter(a);
-    sub = at / max(1, units);
-    unit = at - sub * units;
+    sub = at / (units + extra);
+    const int f = at - sub * (units + extra);
+    unit = max(0, f - extra);
+    left = cost - max(0, extra - f);
   }
   // tiles [tile0(), tile1()) of the item are next
   __device__ __forceinline__ int n_units() const { return min(left, units - unit); }
@@ -202,7 +231,7 @@ struct Run {
   __device__ __forceinline__ int tile1() const { return min((unit + n_units()) * unit_tiles, tiles); }
   __device__ __forceinline__ int head() const { return sub / blocks; }
   __device__ __forceinline__ void next(const CachedArgs& a) {
-    left -= n_units();
+    left -= n_units() + extra;
     unit = 0;
     if (left <= 0 || ++sub < a.kv_heads * blocks) return;
     sub = 0;
@@ -258,7 +287,10 @@ __global__ void __launch_bounds__(THREADS, 2)
   int4* infos = reinterpret_cast<int4*>(smem + C::OFF_INFO);
   uint32_t* poison = reinterpret_cast<uint32_t*>(smem + C::OFF_POISON);
   auto item_info = [&](int b) { return reinterpret_cast<ItemInfo*>(smem + C::OFF_ITEM + b * C::ITEM); };
-  auto item_rs = [&](int b) { return reinterpret_cast<float*>(smem + C::OFF_ITEM + b * C::ITEM + 32); };
+  // of each row: where its output goes, the power of two its queries were
+  // divided by, how many tokens it sees
+  auto item_out = [&](int b) { return reinterpret_cast<int64_t*>(smem + C::OFF_ITEM + b * C::ITEM + 16); };
+  auto item_rs = [&](int b) { return reinterpret_cast<float*>(item_out(b) + RB); };
   auto item_lim = [&](int b) { return reinterpret_cast<int*>(item_rs(b) + RB); };
 
   if (threadIdx.x == 0) {
@@ -300,7 +332,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 
   // ------------------------------------------------- this CTA's run of units
   int tiles_of[MAX_SEQS / THREADS], items_of[MAX_SEQS / THREADS];
-  long long mine = 0;
+  int mine = 0;
 #pragma unroll
   for (int k = 0; k < MAX_SEQS / THREADS; ++k) {
     const int i = k * THREADS + threadIdx.x;
@@ -311,29 +343,32 @@ __global__ void __launch_bounds__(THREADS, 2)
         tiles_of[k] = (s.len + C::TT - 1) / C::TT;
         items_of[k] = (s.fresh * a.group + RB - 1) / RB * a.kv_heads;
       }
-      mine += (long long)tiles_of[k] * items_of[k];
+      mine += (tiles_of[k] + UNIT_TILES - 1) / UNIT_TILES * items_of[k];
     }
   }
   {
-    int sum = (int)mine;  // the host has seen to it that all fit 31 bits
+    int sum = mine;  // the host has seen to it that all costs fit 31 bits
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0 && sum) atomicAdd(total_slot, sum);
   }
   if (threadIdx.x == 0) a.meta[blockIdx.x * 4] = 0;
   __syncthreads();
-  // Few tiles: runs of whole units, so that short items are not cut (a piece
-  // costs a join, about as much as four tiles). Many: single tiles, for balance.
-  const int ut = a.whole || *total_slot < 8 * (int)gridDim.x ? UNIT_TILES : 1;
-  int units_before = 0, total = *total_slot;
-  if (ut > 1) {
+  // Few tiles: runs of whole units of UNIT_TILES, so that short items are not cut
+  // (a piece costs a join, about as much as four tiles), as long as no CTA gets
+  // more than one. Else single tiles, for balance.
+  const int big = *total_slot;
+  const bool few = a.whole || big <= (int)gridDim.x;
+  const int ut = few ? UNIT_TILES : 1, extra = few ? 0 : ITEM_COST;
+  int before = 0, total = big;
+  if (!few) {
     __syncthreads();
     if (threadIdx.x == 0) *total_slot = 0;
     __syncthreads();
     int sum = 0;
 #pragma unroll
     for (int k = 0; k < MAX_SEQS / THREADS; ++k)
-      sum += (tiles_of[k] + ut - 1) / ut * items_of[k];
+      sum += tiles_of[k] ? (tiles_of[k] + extra) * items_of[k] : 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0 && sum) atomicAdd(total_slot, sum);
@@ -347,7 +382,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll
   for (int k = 0; k < MAX_SEQS / THREADS; ++k) {
     if (k * THREADS >= a.n_seqs) break;
-    const int u = (tiles_of[k] + ut - 1) / ut * items_of[k];
+    const int u = tiles_of[k] ? ((tiles_of[k] + ut - 1) / ut + extra) * items_of[k] : 0;
     int incl = u;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -356,7 +391,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
     if (lane == 31) warp_sums[warp] = incl;
     __syncthreads();
-    int base = units_before, all = 0;
+    int base = before, all = 0;
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) {
       if (w < warp) base += warp_sums[w];
@@ -367,10 +402,15 @@ __global__ void __launch_bounds__(THREADS, 2)
       start_slot[0] = k * THREADS + threadIdx.x;
       start_slot[1] = x0 - (incl - u);
     }
-    units_before += all;
+    before += all;
     __syncthreads();
   }
-  const bool busy = x1 > x0;
+  bool busy = x1 > x0;
+  if (busy) {  // a run may lie inside one item's extra part
+    Run<D, RB> r;
+    r.start(a, start_slot[0], start_slot[1], x1 - x0, ut, extra);
+    busy = r.left > 0;
+  }
 
   if (busy && warp == 0) {
     // ------------------------------------------------------------- producer
@@ -381,35 +421,67 @@ __global__ void __launch_bounds__(THREADS, 2)
     uint32_t phase = 0, used = 0, raws = 0;
     bool ok = true;
     Run<D, RB> r;
-    r.start(a, start_slot[0], start_slot[1], x1 - x0, ut);
+    r.start(a, start_slot[0], start_slot[1], x1 - x0, ut, extra);
+    // Pages come in windows of 32, one per lane, with their scales. Loads run
+    // ahead of their use: page numbers two windows, scales one; and where a
+    // sequence fits one window, the next head's scales while this one's tiles
+    // are streamed.
+    struct Scales {
+      float k = 0.f, v = 1.f;
+    };
+    auto load_slot = [&](const int32_t* row, int window, int pages) {
+      const int p = window + lane;
+      int s = p < pages ? row[p] : -1;
+      if (p < pages && !page_fits(s, a.num_pages)) {
+        atomicExch(a.err, kDevErrBadPage);
+        s = -1;
+      }
+      return s;
+    };
+    auto load_scales = [&](int s, int head) {
+      Scales v;
+      if (s >= 0) {
+        v.k = a.k_scale[(size_t)s * a.kv_heads + head];
+        v.v = a.v_scale[(size_t)s * a.kv_heads + head];
+      }
+      return v;
+    };
+    int seq = -1, slot = -1, slot1 = -1, slot2 = -1, window = 0;
+    Scales sc0, sc1;  // of slot, and of slot1 or the next head
+    bool one_window = false;
     while (r.left > 0 && ok) {
       const int len = r.s.len, head = r.head();
       const int tile0 = r.tile0(), tile1 = r.tile1();
       const int lim_min = a.causal ? len - r.s.fresh + 1 : len;
       const int pages = (len + page - 1) >> a.page_shift;
       const int32_t* row = a.table + (size_t)r.seq * a.table_stride;
-      const bool final_item = r.left == r.n_units();
-      int window = -32, slot = -1;
-      float ks = 0.f, lvs = 0.f, ivs = 0.f;
+      const bool final_item = r.left <= r.n_units() + r.extra;
+      if (one_window && seq == r.seq) {
+        sc0 = sc1;
+      } else {
+        seq = r.seq;
+        one_window = pages <= 32 && r.blocks == 1;
+        window = (tile0 * per) & ~31;
+        slot = load_slot(row, window, pages);
+        slot1 = load_slot(row, window + 32, pages);
+        slot2 = load_slot(row, window + 64, pages);
+        sc0 = load_scales(slot, head);
+        if (!one_window) sc1 = load_scales(slot1, head);
+      }
+      if (one_window && head + 1 < a.kv_heads) sc1 = load_scales(slot, head + 1);
+      float ks = sc0.k * a.scale_log2, lvs = __log2f(sc0.v), ivs = 1.f / sc0.v;
       for (int tile = tile0; tile < tile1 && ok; ++tile) {
         const int first = tile * per;
         if (first >= window + 32) {
-          // the next 32 pages of the sequence, one per lane, with their scales
-          window = first & ~31;
-          const int p = window + lane;
-          slot = p < pages ? row[p] : -1;
-          if (p < pages && !page_fits(slot, a.num_pages)) {
-            atomicExch(a.err, kDevErrBadPage);
-            slot = -1;
-          }
-          ks = 0.f;
-          float vs = 1.f;
-          if (slot >= 0) {
-            ks = a.k_scale[(size_t)slot * a.kv_heads + head] * a.scale_log2;
-            vs = a.v_scale[(size_t)slot * a.kv_heads + head];
-          }
-          lvs = __log2f(vs);
-          ivs = 1.f / vs;
+          window += 32;
+          slot = slot1;
+          slot1 = slot2;
+          slot2 = load_slot(row, window + 64, pages);
+          sc0 = sc1;
+          sc1 = load_scales(slot1, head);
+          ks = sc0.k * a.scale_log2;
+          lvs = __log2f(sc0.v);
+          ivs = 1.f / sc0.v;
         }
         ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, a.err, kDevErrTimeoutCached);
         ok = __all_sync(0xffffffffu, ok);
@@ -498,63 +570,78 @@ __global__ void __launch_bounds__(THREADS, 2)
       constexpr uint32_t IDESC_S = umma_idesc_e4m3(128, N, 0);
       constexpr uint32_t IDESC_O = umma_idesc_e4m3(128, N, 1);
       const uint32_t s_col = tmem, o_col = tmem + C::COLS / 2;
-      auto wait = [&](uint32_t bar, uint32_t par) {
-        return mbar_wait(bar, par, abort_flag, a.err, kDevErrTimeoutCached);
-      };
-      int items = 0;  // begun
-      auto issue_qk = [&](int st, int flags) {
-        if (flags & kFirst) {
-          if (!wait(bar_q + 8 * (items & 1), (uint32_t)(items >> 1) & 1u)) return false;
-          ++items;
+      struct Slot {
+        int st = 0;
+        uint32_t ph = 0;
+        __device__ void step() {
+          if (++st == ST) {
+            st = 0;
+            ph ^= 1;
+          }
         }
-        const uint64_t dk = umma_desc_sw128(sbase + st * 2 * TILE);
-        const uint64_t dq = umma_desc_sw128(sbase + C::OFF_Q + ((items - 1) & 1) * N * 128);
-        tc_fence_after();
+      } qk, pv;                     // stages of the next Q K^T and P V
+      uint32_t n_qk = 0, n_pv = 0;  // issued
+      uint32_t items = 0;           // begun by Q K^T
+      bool all_qk = false, ok = true;
+      // what the next of each waits for, as far as it has been seen to be there
+      bool have_k = false, have_s = true, have_p = false;
+      uint64_t since = global_timer_ns();
+      // Whichever is ready goes first: the next tile's scores (its K may be late,
+      // its item's queries too) or this tile's P V.
+      while (ok) {
+        bool did = false;
+        if (!all_qk) {
+          have_s = have_s || mbar_test(bar_s_free, (n_qk - 1) & 1u);
+          have_k = have_k || mbar_test(bar_k + 8 * qk.st, qk.ph);
+          if (have_s && have_k) {
+            const int flags = infos[qk.st].z;
+            if (!(flags & kFirst) || mbar_test(bar_q + 8 * (items & 1), (items >> 1) & 1u)) {
+              if (flags & kFirst) ++items;
+              const uint64_t dk = umma_desc_sw128(sbase + qk.st * 2 * TILE);
+              const uint64_t dq = umma_desc_sw128(sbase + C::OFF_Q + ((items - 1) & 1) * N * 128);
+              tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          umma_f8_ss(s_col, desc_advance(dk, k * 32), desc_advance(dq, k * 32), IDESC_S, k != 0);
-        umma_commit(bar_s);
-        return true;
-      };
-      int st = 0, st_next = 0;
-      uint32_t ph = 0, ph_next = 0;
-      auto step = [&](int& s, uint32_t& p) {
-        if (++s == ST) {
-          s = 0;
-          p ^= 1;
+              for (int k = 0; k < 4; ++k)
+                umma_f8_ss(s_col, desc_advance(dk, k * 32), desc_advance(dq, k * 32), IDESC_S,
+                           k != 0);
+              umma_commit(bar_s);
+              all_qk = flags & kFinal;
+              qk.step();
+              ++n_qk;
+              have_s = have_k = false;
+              did = true;
+            }
+          }
         }
-      };
-      bool ok = wait(bar_k, 0);
-      int flags = 0;
-      if (ok) {
-        flags = infos[0].z;
-        ok = issue_qk(0, flags);
-        step(st_next, ph_next);
-      }
-      for (uint32_t i = 0; ok; ++i) {
-        int flags_next = 0;
-        if (!(flags & kFinal)) {  // the next tile's scores, as soon as these are read
-          ok = wait(bar_k + 8 * st_next, ph_next) && wait(bar_s_free, i & 1u);
-          if (!ok) break;
-          flags_next = infos[st_next].z;
-          ok = issue_qk(st_next, flags_next);
-          if (!ok) break;
-          step(st_next, ph_next);
-        }
-        ok = wait(bar_p, i & 1u) && wait(bar_v + 8 * st, ph);
-        if (!ok) break;
-        tc_fence_after();
-        const uint64_t dv = umma_desc_sw128_mn(sbase + (st * 2 + 1) * TILE);
-        const uint64_t dp = umma_desc_sw128(sbase + C::OFF_P);
+        if (n_pv < n_qk) {
+          have_p = have_p || mbar_test(bar_p, n_pv & 1u);
+          if (have_p && mbar_test(bar_v + 8 * pv.st, pv.ph)) {
+            const int flags = infos[pv.st].z;
+            tc_fence_after();
+            const uint64_t dv = umma_desc_mn<128>(sbase + (pv.st * 2 + 1) * TILE);
+            const uint64_t dp = umma_desc_mn<C::PW>(sbase + C::OFF_P);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          umma_f8_ss(o_col, desc_advance(dv, k * 4096), desc_advance(dp, k * 32), IDESC_O,
-                     !(flags & kFirst) || k != 0);
-        umma_commit(bar_o);
-        umma_commit(bar_empty + 8 * st);
-        step(st, ph);
-        if (flags & kFinal) break;
-        flags = flags_next;
+            for (int k = 0; k < 4; ++k)
+              umma_f8_ss(o_col, desc_advance(dv, k * 4096), desc_advance(dp, k * 32 * C::PW),
+                         IDESC_O, !(flags & kFirst) || k != 0);
+            umma_commit(bar_o);
+            umma_commit(bar_empty + 8 * pv.st);
+            pv.step();
+            ++n_pv;
+            have_p = false;
+            did = true;
+            if (flags & kFinal) break;
+          }
+        }
+        if (did) {
+          since = global_timer_ns();
+        } else if (*abort_flag) {
+          ok = false;
+        } else if (global_timer_ns() - since > kWaitTimeoutNs) {
+          *abort_flag = 1;
+          atomicExch(a.err, kDevErrTimeoutCached);
+          ok = false;
+        }
       }
       if (*abort_flag) {
         umma_commit(bar_drain);
@@ -563,39 +650,46 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
   } else if (busy && warp == 2) {
     // ------------------------------------------------------------- queries
-    bool ok = true;
+    constexpr int EPL = D / 32;  // elements per lane
     Run<D, RB> r;
-    r.start(a, start_slot[0], start_slot[1], x1 - x0, ut);
-    for (uint32_t item = 0; r.left > 0 && ok; ++item) {
-      const int b = item & 1;
-      ok = __all_sync(0xffffffffu, mbar_wait(bar_q_empty + 8 * b, (item >> 1 & 1) ^ 1, abort_flag,
-                                             a.err, kDevErrTimeoutCached));
-      if (!ok) break;
+    r.start(a, start_slot[0], start_slot[1], x1 - x0, ut, extra);
+    uint32_t w[RB][EPL / 2];  // this lane's elements of an item's rows
+    int n_rows = 0, lim = 0;  // lane i: of row i
+    int64_t out = 0;
+    auto load_rows = [&]() {
       const int head = r.head(), block = r.sub - head * r.blocks;
-      const int n_rows = min(RB, r.s.fresh * a.group - block * RB);
-      uint8_t* qb = smem + C::OFF_Q + b * N * 128;
-      constexpr int EPL = D / 32;  // elements per lane
-#pragma unroll 4
+      n_rows = min(RB, r.s.fresh * a.group - block * RB);
+      const int gr = block * RB + lane;
+      const int tok = gr / a.group, col = (head * a.group + gr - tok * a.group) * D;
+      out = (int64_t)(r.s.row0 + tok) * a.o_stride + col;
+      lim = a.causal && lane < n_rows ? r.s.len - r.s.fresh + tok + 1 : r.s.len;
+      const int64_t from = (int64_t)(r.s.row0 + tok) * a.q_stride + col;
+#pragma unroll
       for (int i = 0; i < RB; ++i) {
-        const int gr = block * RB + i;
-        const int tok = gr / a.group, gq = gr - tok * a.group;
-        uint32_t w[EPL / 2];
-        if (i < n_rows) {
-          const uint32_t* src = reinterpret_cast<const uint32_t*>(
-              a.q + (int64_t)(r.s.row0 + tok) * a.q_stride + (head * a.group + gq) * D + lane * EPL);
+        const uint32_t* src =
+            reinterpret_cast<const uint32_t*>(a.q + __shfl_sync(0xffffffffu, from, i)) +
+            lane * (EPL / 2);
 #pragma unroll
-          for (int e = 0; e < EPL / 2; ++e) w[e] = src[e];
-        } else {
+        for (int e = 0; e < EPL / 2; ++e) w[i][e] = i < n_rows ? src[e] : 0u;
+      }
+    };
+    load_rows();
+    for (uint32_t item = 0;; ++item) {
+      const int b = item & 1;
+      if (!__all_sync(0xffffffffu, mbar_wait(bar_q_empty + 8 * b, (item >> 1 & 1) ^ 1, abort_flag,
+                                             a.err, kDevErrTimeoutCached)))
+        break;
+      uint8_t* qb = smem + C::OFF_Q + b * N * 128;
+      float rs = 0.f;
 #pragma unroll
-          for (int e = 0; e < EPL / 2; ++e) w[e] = 0;
-        }
+      for (int i = 0; i < RB; ++i) {
         float x[EPL];
         float top = 0.f;
 #pragma unroll
         for (int e = 0; e < EPL / 2; ++e) {
-          const float2 f = BF ? make_float2(__uint_as_float(w[e] << 16),
-                                            __uint_as_float(w[e] & 0xFFFF0000u))
-                              : unpack_half2(w[e]);
+          const float2 f = BF ? make_float2(__uint_as_float(w[i][e] << 16),
+                                            __uint_as_float(w[i][e] & 0xFFFF0000u))
+                              : unpack_half2(w[i][e]);
           x[2 * e] = f.x;
           x[2 * e + 1] = f.y;
           top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
@@ -604,6 +698,7 @@ __global__ void __launch_bounds__(THREADS, 2)
         // the power of two that brings the largest to [128, 256)
         const int e2 = min(max(((__float_as_int(top) >> 23) & 255) - 127 - 7, -120), 120);
         const float down = __int_as_float((127 - e2) << 23);
+        if (lane == (i & 31)) rs = __int_as_float((127 + e2) << 23);
         uint16_t t[EPL / 2][3];
 #pragma unroll
         for (int e = 0; e < EPL / 2; ++e)
@@ -612,7 +707,7 @@ __global__ void __launch_bounds__(THREADS, 2)
         for (int p = 0; p < TPL; ++p)
 #pragma unroll
           for (int k = 0; k < 3; ++k) {
-            const int n = (p * 3 + k) * RB + i;
+            const int n = C::col(p, i, k);
             if (D == 128) {
               const uint32_t at = (uint32_t)(lane * 4) ^ ((n & 7) << 4);
               *reinterpret_cast<uint32_t*>(qb + n * 128 + at) =
@@ -624,21 +719,16 @@ __global__ void __launch_bounds__(THREADS, 2)
               *reinterpret_cast<uint16_t*>(qb + n * 128 + not_at) = 0;
             }
           }
-        if (lane == 0) {
-          item_rs(b)[i] = __int_as_float((127 + e2) << 23);
-          item_lim(b)[i] = a.causal && i < n_rows ? r.s.len - r.s.fresh + tok + 1 : r.s.len;
-        }
+      }
+      if (lane < RB) {
+        item_out(b)[lane] = out;
+        item_rs(b)[lane] = rs;
+        item_lim(b)[lane] = lim;
       }
       const bool starts = r.unit == 0, ends = r.unit + r.n_units() == r.units;
       if (lane == 0) {
-        ItemInfo* it = item_info(b);
-        it->row0 = r.s.row0;
-        it->head = head;
-        it->block = block;
-        it->n_rows = n_rows;
-        it->starts = starts;
-        it->ends = ends;
-        if (r.left == r.n_units() && !ends) {
+        *item_info(b) = {n_rows, starts, ends, 0};
+        if (r.left <= r.n_units() + r.extra && !ends) {
           // for the join: 2: an item that begins here ends in a later CTA, 4:
           // the run lies inside one item
           a.meta[blockIdx.x * 4 + 1] = r.seq;
@@ -650,6 +740,8 @@ __global__ void __launch_bounds__(THREADS, 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_q + 8 * b);
       r.next(a);
+      if (r.left <= 0) break;
+      load_rows();  // on their way while the item before is worked on
     }
   } else if (TPL == 2 && busy && warp == 3) {
     // ------------------------------------------- K lines shared by two tokens
@@ -695,7 +787,19 @@ __global__ void __launch_bounds__(THREADS, 2)
     const int line = (warp - 4) * 32 + lane;
     const uint32_t lane_base = tmem + ((uint32_t)((warp - 4) * 32) << 16);
     const uint32_t s_col = lane_base, o_col = lane_base + C::COLS / 2;
-    constexpr int CH = RB < 16 ? RB : 16;
+    constexpr int CH = RB < 16 ? RB : 16;  // rows that tensor memory is read for at a time
+    // columns col(p, r0, 0) ... of CH rows, their three terms added
+    auto read_rows = [&](uint32_t col, float (&v)[CH]) {
+      constexpr int W = CH == 4 ? 4 : CH == 8 ? 8 : 16;
+      uint32_t s[3 * CH / W][W];
+#pragma unroll
+      for (int i = 0; i < 3 * CH / W; ++i) tmem_ld_32x32b(col + W * i, s[i]);
+      tmem_wait_ld();
+      auto at = [&](int n) { return __uint_as_float(s[n / W][n % W]); };
+#pragma unroll
+      for (int r = 0; r < CH; ++r)
+        v[r] = fmaf(at(C::col(0, r, 2)), T2, fmaf(at(C::col(0, r, 1)), T1, at(C::col(0, r, 0))));
+    };
     float4* wmax = reinterpret_cast<float4*>(smem + C::OFF_MAX);
     uint8_t* pb = smem + C::OFF_P;
     float off[RB], l[RB];
@@ -718,14 +822,10 @@ __global__ void __launch_bounds__(THREADS, 2)
       for (int p = 0; p < TPL; ++p)
 #pragma unroll
         for (int c = 0; c < RB / CH; ++c) {
-          uint32_t s[3][CH];
+          float v[CH];
+          read_rows(s_col + C::col(p, c * CH, 0), v);
 #pragma unroll
-          for (int t = 0; t < 3; ++t) tmem_ld_32x32b(s_col + (p * 3 + t) * RB + c * CH, s[t]);
-          tmem_wait_ld();
-#pragma unroll
-          for (int r = 0; r < CH; ++r)
-            x[p][c * CH + r] = fmaf(__uint_as_float(s[2][r]), T2,
-                                    fmaf(__uint_as_float(s[1][r]), T1, __uint_as_float(s[0][r])));
+          for (int r = 0; r < CH; ++r) x[p][c * CH + r] = v[r];
         }
       tc_fence_before();
       mbar_arrive(bar_s_free);
@@ -800,12 +900,16 @@ __global__ void __launch_bounds__(THREADS, 2)
           tc_fence_after();
 #pragma unroll
           for (int c = 0; c < N / 16; ++c) {
+            bool any = false;  // the same for all threads
+#pragma unroll
+            for (int e = 0; e < 16; ++e) any |= alpha[C::row_of(16 * c + e)] != 1.f;
+            if (!any) continue;
             uint32_t o[16];
             tmem_ld_32x32b(o_col + 16 * c, o);
             tmem_wait_ld();
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha[(16 * c + e) % RB]);
+              o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha[C::row_of(16 * c + e)]);
             tmem_st_32x32b_x16(o_col + 16 * c, o);
           }
           tmem_wait_st();
@@ -815,6 +919,8 @@ __global__ void __launch_bounds__(THREADS, 2)
         const bool w = mbar_wait(bar_o, (i - 1) & 1u, abort_flag, a.err, kDevErrTimeoutCached);
         ok = __all_sync(0xffffffffu, w) && ok;
       }
+      // the weights' terms: a line of P in the order of the columns
+      uint16_t terms[N / 2];
 #pragma unroll
       for (int p = 0; p < TPL; ++p)
 #pragma unroll
@@ -825,12 +931,24 @@ __global__ void __launch_bounds__(THREADS, 2)
           uint16_t t[3];
           split3(__floats2half2_rn(p0, p1), t);
 #pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            const int n = (p * 3 + k) * RB + r;
-            pb[n * 128 + (line ^ ((n & 7) << 4))] = (uint8_t)t[k];
-            pb[(n + 1) * 128 + (line ^ (((n + 1) & 7) << 4))] = (uint8_t)(t[k] >> 8);
-          }
+          for (int k = 0; k < 3; ++k) terms[C::col(p, r, k) / 2] = t[k];
         }
+#pragma unroll
+      for (int n = C::NC / 2; n < N / 2; ++n) terms[n] = 0;
+      {
+        // 16-byte groups swizzled like the tensor cores' PW-byte pattern
+        constexpr int G = C::PW / 16;
+        const int sw = (line * C::PW >> 7) & (G - 1);
+#pragma unroll
+        for (int c = 0; c < N / 16; ++c) {
+          uint32_t w[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            w[q] = terms[8 * c + 2 * q] | (uint32_t)terms[8 * c + 2 * q + 1] << 16;
+          *reinterpret_cast<uint4*>(pb + line * C::PW + ((c ^ sw) << 4)) =
+              make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
       if (check) {
         // Codes of tokens that no row sees become 0 (their weight is 0, but 0 *
         // NaN is not); NaN codes of new tokens that only later rows see become 0
@@ -881,16 +999,10 @@ __global__ void __launch_bounds__(THREADS, 2)
         float v[RB];
 #pragma unroll
         for (int c = 0; c < RB / CH; ++c) {
-          uint32_t o[3][CH];
+          float o[CH];
+          read_rows(o_col + C::col(half, c * CH, 0), o);
 #pragma unroll
-          for (int t = 0; t < 3; ++t)
-            tmem_ld_32x32b(o_col + (half * 3 + t) * RB + c * CH, o[t]);
-          tmem_wait_ld();
-#pragma unroll
-          for (int r = 0; r < CH; ++r)
-            v[c * CH + r] =
-                fmaf(__uint_as_float(o[2][r]), T2,
-                     fmaf(__uint_as_float(o[1][r]), T1, __uint_as_float(o[0][r])));
+          for (int r = 0; r < CH; ++r) v[c * CH + r] = o[r];
         }
         const uint32_t bits = poison[line];
         if (bits) {
@@ -898,11 +1010,9 @@ __global__ void __launch_bounds__(THREADS, 2)
           for (int r = 0; r < RB; ++r)
             if (bits >> r & 1u) v[r] = NAN;
         }
-#pragma unroll
-        for (int r = 0; r < RB; ++r) {
-          const float s = warp_add(l[r]);
-          if (lane == (r & 31)) reinterpret_cast<float*>(wmax + r)[warp - 4] = s;
-        }
+        const float sums = warp_add<RB>(l);
+        if (lane % (32 / RB) == 0)
+          reinterpret_cast<float*>(wmax + lane / (32 / RB))[warp - 4] = sums;
         float* other = reinterpret_cast<float*>(pb);  // the weights have been read
         if (TPL == 2 && half) {
 #pragma unroll
@@ -915,25 +1025,30 @@ __global__ void __launch_bounds__(THREADS, 2)
           // a piece that continues an earlier CTA's item goes to slot 0, one
           // that begins here and ends elsewhere to slot 1
           float* part = a.part + ((size_t)blockIdx.x * 2 + (it.starts ? 1 : 0)) * kCachedPartFloats;
+          const bool whole = it.starts && it.ends;
+          // lane r of each warp: row r's sum
+          const float4 w4 = wmax[lane & (RB - 1)];
+          const float sum = (w4.x + w4.y) + (w4.z + w4.w);
+          const float inv = sum == 0.f ? 0.f : whole ? __fdividef(1.f, sum) : 1.f;
+          uint16_t* o = a.o + d;
 #pragma unroll
           for (int r = 0; r < RB; ++r) {
-            if (r >= it.n_rows) break;
             if (TPL == 2) v[r] += other[r * 64 + d];
-            const float4 w4 = wmax[r];
-            const float sum = (w4.x + w4.y) + (w4.z + w4.w);
-            if (it.starts && it.ends) {
-              const int gr = it.block * RB + r;
-              const int tok = gr / a.group, gq = gr - tok * a.group;
-              a.o[(int64_t)(it.row0 + tok) * a.o_stride + (it.head * a.group + gq) * D + d] =
-                  to_out<BF>(sum == 0.f ? 0.f : v[r] / sum);
-            } else {
-              part[r * D + d] = v[r];
-              if (line == 0) {
-                // a row that saw nothing has no maximum
-                part[kCachedPartRows * 128 + r] = sum == 0.f ? -INFINITY : P_EXP - off[r];
-                part[kCachedPartRows * 129 + r] = sum;
-              }
+            v[r] *= __shfl_sync(0xffffffffu, inv, r);
+            if (r < it.n_rows) {
+              if (whole)
+                o[item_out(b)[r]] = to_out<BF>(v[r]);
+              else
+                part[r * D + d] = v[r];
             }
+          }
+          if (!whole && line < it.n_rows) {
+            // a row that saw nothing has no maximum
+            float top = 0.f;
+#pragma unroll
+            for (int r = 0; r < RB; ++r) top = lane == r ? P_EXP - off[r] : top;
+            part[kCachedPartRows * 128 + line] = sum == 0.f ? -INFINITY : top;
+            part[kCachedPartRows * 129 + line] = sum;
           }
         }
         tc_fence_before();
@@ -957,11 +1072,20 @@ __global__ void __launch_bounds__(THREADS, 2)
   }
 }
 
-// Adds the pieces of the items that attention left in parts. Block c looks
+// Adds the pieces of the items that attention left in parts. Blocks (c, *) look
 // after the item that CTA c began and did not end: its slot 1, then slot 0 of
-// the CTAs that follow, in order.
+// the CTAs that follow, in order. Block (c, y) has RB / 4 of its rows: first
+// the pieces' weights 2^(M_k - M) and the row sum, one warp per row, then the
+// weighted sums, the warps of a row taking every G-th piece.
 template <int D, int RB, bool BF>
 __global__ void __launch_bounds__(256) cached_join_kernel(const CachedArgs a, int ctas) {
+  constexpr int NR = RB / 4;              // rows per block
+  constexpr int L = D / 4;                // lanes for a row's float4
+  constexpr int G = 8 / NR * (32 / L);    // piece groups
+  constexpr int CHUNK = 64;               // pieces at a time
+  __shared__ float weight[NR][CHUNK];
+  __shared__ float4 sums[G][NR][L];
+  __shared__ float inv_sum[NR];
   griddep_launch_dependents();
   griddep_wait();  // the pieces are the previous kernel's output
   const int c0 = blockIdx.x;
@@ -972,26 +1096,84 @@ __global__ void __launch_bounds__(256) cached_join_kernel(const CachedArgs a, in
   const int blocks = (fresh * a.group + RB - 1) / RB;
   const int head = sub / blocks, block = sub - head * blocks;
   const int n_rows = min(RB, fresh * a.group - block * RB);
-  int last = c0 + 1;  // the CTA that ends the item
-  while (last < ctas - 1 && a.meta[last * 4] == 4) ++last;
-  for (int i = threadIdx.x; i < n_rows * D; i += 256) {
-    const int r = i / D, d = i % D;
-    float top = -INFINITY, sum = 0.f, acc = 0.f;
-    for (int k = c0; k <= last && k < ctas; ++k) {
-      const float* part = a.part + ((size_t)k * 2 + (k == c0 ? 1 : 0)) * kCachedPartFloats;
-      const float pm = part[kCachedPartRows * 128 + r], pl = part[kCachedPartRows * 129 + r];
-      const float y = part[r * D + d];
-      const float mn = fmaxf(top, pm);
-      const float mu = mn == -INFINITY ? 0.f : mn;
-      const float f0 = ex2_approx(top - mu), f1 = ex2_approx(pm - mu);
-      top = mn;
-      sum = fmaf(sum, f0, pl * f1);
-      acc = fmaf(acc, f0, y * f1);
+  const int first_row = blockIdx.y * NR;
+  if (first_row >= n_rows) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the CTA that ends the item: the first behind c0 that does not pass it on
+  int pieces = 2;
+  for (int c = c0 + 1;; c += 32) {
+    const uint32_t pass = __ballot_sync(0xffffffffu, c + lane < ctas && a.meta[(c + lane) * 4] == 4);
+    if (pass != 0xffffffffu) {
+      pieces = c - c0 + __ffs(~pass);
+      break;
     }
+  }
+  pieces = min(pieces, ctas - c0);
+  auto piece = [&](int k) {
+    return a.part + ((size_t)(c0 + k) * 2 + (k == 0 ? 1 : 0)) * kCachedPartFloats;
+  };
+  // this warp's row (of the block) for the weights, the largest maximum
+  const int wr = warp % NR;
+  float top = -INFINITY;
+  for (int k = lane; k < pieces; k += 32)
+    top = fmaxf(top, piece(k)[kCachedPartRows * 128 + first_row + wr]);
+  top = warp_max(top);
+  const float mu = top == -INFINITY ? 0.f : top;
+  const int sr = warp % NR;  // and for the sums
+  const int grp = warp / NR * (32 / L) + lane / L, col = lane % L;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  for (int k0 = 0; k0 < pieces; k0 += CHUNK) {
+    if (warp < NR) {
+      for (int k = lane; k < CHUNK; k += 32) {
+        float w = 0.f;
+        if (k0 + k < pieces) {
+          const float* p = piece(k0 + k) + kCachedPartRows * 128 + first_row + wr;
+          w = ex2_approx(p[0] - mu);
+          sum = fmaf(p[kCachedPartRows], w, sum);
+        }
+        weight[wr][k] = w;
+      }
+    }
+    __syncthreads();
+    const int n = min(CHUNK, pieces - k0);
+#pragma unroll 8
+    for (int k = grp; k < n; k += G) {
+      const float w = weight[sr][k];
+      const float4 y = reinterpret_cast<const float4*>(piece(k0 + k) + (first_row + sr) * D)[col];
+      acc.x = fmaf(y.x, w, acc.x);
+      acc.y = fmaf(y.y, w, acc.y);
+      acc.z = fmaf(y.z, w, acc.z);
+      acc.w = fmaf(y.w, w, acc.w);
+    }
+    __syncthreads();
+  }
+  if (warp < NR) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) inv_sum[wr] = sum == 0.f ? 0.f : 1.f / sum;
+  }
+  sums[grp][sr][col] = acc;
+  __syncthreads();
+  for (int i = threadIdx.x; i < NR * L; i += 256) {
+    const int rr = i / L, c = i % L, r = first_row + rr;
+    if (r >= n_rows) break;
+    float4 v = sums[0][rr][c];
+#pragma unroll
+    for (int g = 1; g < G; ++g) {
+      const float4 y = sums[g][rr][c];
+      v.x += y.x;
+      v.y += y.y;
+      v.z += y.z;
+      v.w += y.w;
+    }
+    const float inv = inv_sum[rr];
     const int gr = block * RB + r;
     const int tok = gr / a.group, gq = gr - tok * a.group;
-    a.o[(int64_t)(row0 + tok) * a.o_stride + (head * a.group + gq) * D + d] =
-        to_out<BF>(sum == 0.f ? 0.f : acc / sum);
+    uint16_t* o = a.o + (int64_t)(row0 + tok) * a.o_stride + (head * a.group + gq) * D + 4 * c;
+    *reinterpret_cast<uint2*>(o) =
+        make_uint2(to_out<BF>(v.x * inv) | (uint32_t)to_out<BF>(v.y * inv) << 16,
+                   to_out<BF>(v.z * inv) | (uint32_t)to_out<BF>(v.w * inv) << 16);
   }
 }
 
@@ -1017,7 +1199,7 @@ sam3_status_t launch_cached(sam3_ctx_t* ctx, const CUtensorMap& mk, const CUtens
   if (st != SAM3_OK) return st;
   const long long blocks = ((long long)a.max_new * a.group + RB - 1) / RB;
   const long long tiles = (capacity + C::TT - 1) / C::TT;
-  if (blocks * a.kv_heads * a.n_seqs * tiles > 0x7FFFFFFFll)
+  if (blocks * a.kv_heads * a.n_seqs * (tiles + ITEM_COST) > 0x7FFFFFFFll)
     return set_error(ctx, SAM3_ERR_SHAPE, "attention_cached: too much work for one call");
   a.whole = tiles <= UNIT_TILES;
   const int ctas = 2 * ctx->num_sms;
@@ -1025,7 +1207,7 @@ sam3_status_t launch_cached(sam3_ctx_t* ctx, const CUtensorMap& mk, const CUtens
                              ctx->stream, mk, mv, a);
   st = check_launch_ret(ctx, e, "cached_attn_kernel");
   if (st != SAM3_OK || a.whole) return st;  // whole items: nothing to join
-  e = launch_pdl(cached_join_kernel<D, RB, BF>, dim3(ctas), dim3(256), 0, ctx->stream, a, ctas);
+  e = launch_pdl(cached_join_kernel<D, RB, BF>, dim3(ctas, 4), dim3(256), 0, ctx->stream, a, ctas);
   return check_launch_ret(ctx, e, "cached_join_kernel");
 }
 
@@ -1071,7 +1253,7 @@ sam3_status_t attention_cached(sam3_ctx_t* ctx, const sam3_kv_cache_t* c, int dt
       (!cu_new && (max_new != 1 || rows < n_seqs)))
     return set_error(ctx, SAM3_ERR_SHAPE, "attention_cached: bad shape (at most %d sequences)",
                      MAX_SEQS);
-  if ((most + 31) / 32 * c->kv_heads * n_seqs * ((capacity + 127) / 128) > 0x7FFFFFFFll)
+  if ((most + 31) / 32 * c->kv_heads * n_seqs * ((capacity + 127) / 128 + ITEM_COST) > 0x7FFFFFFFll)
     return set_error(ctx, SAM3_ERR_SHAPE, "attention_cached: too much work for one call");
   CachedArgs a{};
   a.group = heads / c->kv_heads;

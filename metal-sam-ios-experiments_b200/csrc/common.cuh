@@ -70,6 +70,19 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
+// Whether the phase with the given parity is complete, without waiting.
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // Wait for the phase with the given parity. Returns false if the CTA-wide
 // abort flag is raised or the wait exceeds kWaitTimeoutNs (then it raises the
 // abort flag and records `code` in *err).
@@ -214,6 +227,20 @@ __device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t saddr) {
   return d;
 }
 
+// Same again with lines of W = 32, 64 or 128 bytes along M/N (8 lines per group,
+// W-byte swizzle; layout 6, 4 or 2).
+template <int W>
+__device__ __forceinline__ uint64_t umma_desc_mn(uint32_t saddr) {
+  static_assert(W == 32 || W == 64 || W == 128, "swizzle width");
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(1u) << 16;
+  d |= static_cast<uint64_t>((8u * W) >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(W == 128 ? 2u : W == 64 ? 4u : 6u) << 61;
+  return d;
+}
+
 // The same descriptor `bytes` further on in shared memory: the start address
 // sits in bits [0,14) as addr >> 4, and shared addresses stay below 256 KB,
 // so a 32-bit add on the low word never carries out of the field. (The MMA
@@ -230,9 +257,11 @@ __host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n, int b_mn_maj
          (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-// Instruction descriptor, kind::f8f6f4: D f32, A/B e4m3, B K-major.
-__host__ __device__ constexpr uint32_t umma_idesc_e4m3(int m, int n, int a_mn_major) {
-  return (1u << 4) | (static_cast<uint32_t>(a_mn_major & 1) << 15) |
+// Instruction descriptor, kind::f8f6f4: D f32, A/B e4m3, both K-major or both
+// M/N-major.
+__host__ __device__ constexpr uint32_t umma_idesc_e4m3(int m, int n, int mn_major) {
+  return (1u << 4) | (static_cast<uint32_t>(mn_major & 1) << 15) |
+         (static_cast<uint32_t>(mn_major & 1) << 16) |
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
