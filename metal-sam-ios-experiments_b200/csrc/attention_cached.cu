@@ -278,9 +278,6 @@ __global__ void __launch_bounds__(THREADS, 2)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 4);
   volatile int* softmax_failed = reinterpret_cast<volatile int*>(misc + 8);
-  int* total_slot = reinterpret_cast<int*>(misc + 12);
-  volatile int* start_slot = reinterpret_cast<volatile int*>(misc + 16);  // seq, at
-  int* warp_sums = reinterpret_cast<int*>(misc + 32);                     // [8]
   volatile int* raw_stage = reinterpret_cast<volatile int*>(misc + 64);
   volatile int* k_nan = reinterpret_cast<volatile int*>(misc + 68);       // [ST]
   float4* scales = reinterpret_cast<float4*>(smem + C::OFF_SCALE);
@@ -313,7 +310,6 @@ __global__ void __launch_bounds__(THREADS, 2)
     for (int s = 0; s < ST; ++s) k_nan[s] = kNever;
     *abort_flag = 0;
     *softmax_failed = 0;
-    *total_slot = 0;
     fence_mbar_init();
     prefetch_tmap(&map_k);
     prefetch_tmap(&map_v);
@@ -330,87 +326,50 @@ __global__ void __launch_bounds__(THREADS, 2)
   griddep_launch_dependents();  // behind the allocation: the next kernel allocates too
   griddep_wait();  // lengths, pages, codes and queries may be earlier kernels' outputs
 
-  // ------------------------------------------------- this CTA's run of units
-  int tiles_of[MAX_SEQS / THREADS], items_of[MAX_SEQS / THREADS];
-  int mine = 0;
-#pragma unroll
-  for (int k = 0; k < MAX_SEQS / THREADS; ++k) {
-    const int i = k * THREADS + threadIdx.x;
-    tiles_of[k] = items_of[k] = 0;
-    if (i < a.n_seqs) {
-      const Seq s = load_seq(a, i, blockIdx.x == 0);
-      if (s.fresh) {
-        tiles_of[k] = (s.len + C::TT - 1) / C::TT;
-        items_of[k] = (s.fresh * a.group + RB - 1) / RB * a.kv_heads;
-      }
-      mine += (tiles_of[k] + UNIT_TILES - 1) / UNIT_TILES * items_of[k];
-    }
+  // ------------------------------------------------- this CTA's run
+  // Each warp plans for itself (no barrier): lane l sums the costs of the
+  // sequences [l * m, l * m + m).
+  const int m = (a.n_seqs + 31) / 32;
+  auto cost_of = [&](int i, bool few, bool report) {
+    if (i >= a.n_seqs) return 0;
+    const Seq s = load_seq(a, i, report);
+    if (s.fresh == 0) return 0;
+    const int tiles = (s.len + C::TT - 1) / C::TT;
+    const int items = (s.fresh * a.group + RB - 1) / RB * a.kv_heads;
+    return (few ? (tiles + UNIT_TILES - 1) / UNIT_TILES : tiles + ITEM_COST) * items;
+  };
+  int sums[2] = {0, 0};
+  for (int j = 0; j < m; ++j) {
+    sums[0] += cost_of(lane * m + j, false, blockIdx.x == 0 && warp == 0);
+    sums[1] += cost_of(lane * m + j, true, false);
   }
-  {
-    int sum = mine;  // the host has seen to it that all costs fit 31 bits
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0 && sum) atomicAdd(total_slot, sum);
-  }
-  if (threadIdx.x == 0) a.meta[blockIdx.x * 4] = 0;
-  __syncthreads();
   // Few tiles: runs of whole units of UNIT_TILES, so that short items are not cut
   // (a piece costs a join, about as much as four tiles), as long as no CTA gets
   // more than one. Else single tiles, for balance.
-  const int big = *total_slot;
-  const bool few = a.whole || big <= (int)gridDim.x;
+  const bool few = a.whole || __reduce_add_sync(0xffffffffu, sums[1]) <= (int)gridDim.x;
   const int ut = few ? UNIT_TILES : 1, extra = few ? 0 : ITEM_COST;
-  int before = 0, total = big;
-  if (!few) {
-    __syncthreads();
-    if (threadIdx.x == 0) *total_slot = 0;
-    __syncthreads();
-    int sum = 0;
+  const int own = few ? sums[1] : sums[0];
+  int upto = own;
 #pragma unroll
-    for (int k = 0; k < MAX_SEQS / THREADS; ++k)
-      sum += tiles_of[k] ? (tiles_of[k] + extra) * items_of[k] : 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0 && sum) atomicAdd(total_slot, sum);
-    __syncthreads();
-    total = *total_slot;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
   }
+  const int total = __shfl_sync(0xffffffffu, upto, 31);
   // equal runs, without a gap between the CTAs that have one (the join's order)
   const int busy_ctas = min((int)gridDim.x, total), cta = min((int)blockIdx.x, busy_ctas);
   const int x0 = busy_ctas ? (int)((long long)cta * total / busy_ctas) : 0;
   const int x1 = cta < busy_ctas ? (int)((long long)(cta + 1) * total / busy_ctas) : x0;
-#pragma unroll
-  for (int k = 0; k < MAX_SEQS / THREADS; ++k) {
-    if (k * THREADS >= a.n_seqs) break;
-    const int u = tiles_of[k] ? ((tiles_of[k] + ut - 1) / ut + extra) * items_of[k] : 0;
-    int incl = u;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    if (lane == 31) warp_sums[warp] = incl;
-    __syncthreads();
-    int base = before, all = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
-      if (w < warp) base += warp_sums[w];
-      all += warp_sums[w];
-    }
-    incl += base;
-    if (x0 < incl && x0 >= incl - u) {  // one thread at most
-      start_slot[0] = k * THREADS + threadIdx.x;
-      start_slot[1] = x0 - (incl - u);
-    }
-    before += all;
-    __syncthreads();
-  }
+  Run<D, RB> run;
   bool busy = x1 > x0;
-  if (busy) {  // a run may lie inside one item's extra part
-    Run<D, RB> r;
-    r.start(a, start_slot[0], start_slot[1], x1 - x0, ut, extra);
-    busy = r.left > 0;
+  if (busy) {
+    const int l = __ffs(__ballot_sync(0xffffffffu, upto > x0)) - 1;  // whose sequences x0 is in
+    int at = x0 - __shfl_sync(0xffffffffu, upto - own, l), seq = l * m;
+    for (int cost; at >= (cost = cost_of(seq, few, false)); ++seq) at -= cost;
+    run.start(a, seq, at, x1 - x0, ut, extra);
+    busy = run.left > 0;  // a run may lie inside one item's extra part
   }
+  if (threadIdx.x == 64) a.meta[blockIdx.x * 4] = 0;  // warp 2 knows better later
 
   if (busy && warp == 0) {
     // ------------------------------------------------------------- producer
@@ -420,8 +379,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     int stage = 0;
     uint32_t phase = 0, used = 0, raws = 0;
     bool ok = true;
-    Run<D, RB> r;
-    r.start(a, start_slot[0], start_slot[1], x1 - x0, ut, extra);
+    Run<D, RB>& r = run;
     // Pages come in windows of 32, one per lane, with their scales. Loads run
     // ahead of their use: page numbers two windows, scales one; and where a
     // sequence fits one window, the next head's scales while this one's tiles
@@ -469,7 +427,6 @@ __global__ void __launch_bounds__(THREADS, 2)
         if (!one_window) sc1 = load_scales(slot1, head);
       }
       if (one_window && head + 1 < a.kv_heads) sc1 = load_scales(slot, head + 1);
-      float ks = sc0.k * a.scale_log2, lvs = __log2f(sc0.v), ivs = 1.f / sc0.v;
       for (int tile = tile0; tile < tile1 && ok; ++tile) {
         const int first = tile * per;
         if (first >= window + 32) {
@@ -479,9 +436,6 @@ __global__ void __launch_bounds__(THREADS, 2)
           slot2 = load_slot(row, window + 64, pages);
           sc0 = sc1;
           sc1 = load_scales(slot1, head);
-          ks = sc0.k * a.scale_log2;
-          lvs = __log2f(sc0.v);
-          ivs = 1.f / sc0.v;
         }
         ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, a.err, kDevErrTimeoutCached);
         ok = __all_sync(0xffffffffu, ok);
@@ -492,12 +446,6 @@ __global__ void __launch_bounds__(THREADS, 2)
         const bool copies = (lane & 15) < per && my_page < pages && my_slot >= 0;
         const uint32_t n_copies = __popc(__ballot_sync(0xffffffffu, copies) & 0xFFFFu);
         const bool hole = __any_sync(0xffffffffu, (lane & 15) < per && my_page < pages && my_slot < 0);
-        const int sp = (first + (((lane & 15) * 16) >> a.page_shift)) & 31;
-        // .w: the page is there; the tokens of one that is not count as masked
-        const float4 sc = make_float4(__shfl_sync(0xffffffffu, ks, sp),
-                                      __shfl_sync(0xffffffffu, lvs, sp),
-                                      __shfl_sync(0xffffffffu, ivs, sp),
-                                      __shfl_sync(0xffffffffu, slot, sp) >= 0 ? 1.f : 0.f);
         // a line of this tile may hold a K code that not all rows see of it
         const int tile_end = (tile + 1) * C::TT;
         const bool raw = TPL == 2 && ((len & 1 && len < tile_end && len >= tile * C::TT) ||
@@ -509,7 +457,27 @@ __global__ void __launch_bounds__(THREADS, 2)
           ++raws;
         }
         const uint32_t bar_k_tile = raw ? bar_raw : bar_k + 8 * stage;
-        if (lane < C::GRAN) scales[stage * C::GRAN + lane] = sc;
+        if (lane == 0) {
+          mbar_expect_tx(bar_k_tile, n_copies * copy_bytes);
+          mbar_arrive_expect_tx(bar_v + 8 * stage, n_copies * copy_bytes);
+        }
+        __syncwarp();
+        if (copies) {
+          const int which = lane >> 4;
+          const uint32_t dst =
+              sbase + (stage * 2 + which) * TILE + (uint32_t)(lane & 15) * copy_bytes;
+          const long long at = ((long long)my_slot * a.kv_heads + head) << a.page_shift;
+          tma_load_2d(dst, which ? &map_v : &map_k, which ? bar_v + 8 * stage : bar_k_tile, 0,
+                      (int)(at / TPL));
+        }
+        // the scales may still be on their way
+        const int sp = (first + (((lane & 15) * 16) >> a.page_shift)) & 31;
+        const float ks = __shfl_sync(0xffffffffu, sc0.k, sp), vs = __shfl_sync(0xffffffffu, sc0.v, sp);
+        const bool there = __shfl_sync(0xffffffffu, slot, sp) >= 0;
+        // .w: the page is there; the tokens of one that is not count as masked
+        if (lane < C::GRAN)
+          scales[stage * C::GRAN + lane] =
+              make_float4(ks * a.scale_log2, __log2f(vs), 1.f / vs, there ? 1.f : 0.f);
         if (lane == 0) {
           int flags = 0;
           if (tile == tile0) flags |= kFirst;
@@ -522,19 +490,7 @@ __global__ void __launch_bounds__(THREADS, 2)
             k_nan[stage] = kNever;
         }
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive_expect_tx(bar_k_tile, n_copies * copy_bytes);
-          mbar_arrive_expect_tx(bar_v + 8 * stage, n_copies * copy_bytes);
-        }
-        __syncwarp();
-        if (copies) {
-          const int which = lane >> 4;
-          const uint32_t dst =
-              sbase + (stage * 2 + which) * TILE + (uint32_t)(lane & 15) * copy_bytes;
-          const long long at = ((long long)my_slot * a.kv_heads + head) << a.page_shift;
-          tma_load_2d(dst, which ? &map_v : &map_k, which ? bar_v + 8 * stage : bar_k_tile, 0,
-                      (int)(at / TPL));
-        }
+        if (lane == 0) mbar_arrive(bar_k_tile);
         used = min(used + 1, (uint32_t)ST);
         if (++stage == ST) {
           stage = 0;
@@ -590,6 +546,26 @@ __global__ void __launch_bounds__(THREADS, 2)
       // its item's queries too) or this tile's P V.
       while (ok) {
         bool did = false;
+        if (n_pv < n_qk) {
+          have_p = have_p || mbar_test(bar_p, n_pv & 1u);
+          if (have_p && mbar_test(bar_v + 8 * pv.st, pv.ph)) {
+            const int flags = infos[pv.st].z;
+            tc_fence_after();
+            const uint64_t dv = umma_desc_mn<128>(sbase + (pv.st * 2 + 1) * TILE);
+            const uint64_t dp = umma_desc_mn<C::PW>(sbase + C::OFF_P);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_f8_ss(o_col, desc_advance(dv, k * 4096), desc_advance(dp, k * 32 * C::PW),
+                         IDESC_O, !(flags & kFirst) || k != 0);
+            umma_commit(bar_o);
+            umma_commit(bar_empty + 8 * pv.st);
+            pv.step();
+            ++n_pv;
+            have_p = false;
+            did = true;
+            if (flags & kFinal) break;
+          }
+        }
         if (!all_qk) {
           have_s = have_s || mbar_test(bar_s_free, (n_qk - 1) & 1u);
           have_k = have_k || mbar_test(bar_k + 8 * qk.st, qk.ph);
@@ -613,26 +589,6 @@ __global__ void __launch_bounds__(THREADS, 2)
             }
           }
         }
-        if (n_pv < n_qk) {
-          have_p = have_p || mbar_test(bar_p, n_pv & 1u);
-          if (have_p && mbar_test(bar_v + 8 * pv.st, pv.ph)) {
-            const int flags = infos[pv.st].z;
-            tc_fence_after();
-            const uint64_t dv = umma_desc_mn<128>(sbase + (pv.st * 2 + 1) * TILE);
-            const uint64_t dp = umma_desc_mn<C::PW>(sbase + C::OFF_P);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_f8_ss(o_col, desc_advance(dv, k * 4096), desc_advance(dp, k * 32 * C::PW),
-                         IDESC_O, !(flags & kFirst) || k != 0);
-            umma_commit(bar_o);
-            umma_commit(bar_empty + 8 * pv.st);
-            pv.step();
-            ++n_pv;
-            have_p = false;
-            did = true;
-            if (flags & kFinal) break;
-          }
-        }
         if (did) {
           since = global_timer_ns();
         } else if (*abort_flag) {
@@ -651,8 +607,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   } else if (busy && warp == 2) {
     // ------------------------------------------------------------- queries
     constexpr int EPL = D / 32;  // elements per lane
-    Run<D, RB> r;
-    r.start(a, start_slot[0], start_slot[1], x1 - x0, ut, extra);
+    Run<D, RB>& r = run;
     uint32_t w[RB][EPL / 2];  // this lane's elements of an item's rows
     int n_rows = 0, lim = 0;  // lane i: of row i
     int64_t out = 0;
