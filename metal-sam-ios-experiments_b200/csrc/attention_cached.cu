@@ -137,10 +137,11 @@ __device__ __forceinline__ bool vote_any(bool p) {  // over warps 4-7
 __device__ __forceinline__ void compute_barrier() {
   asm volatile("barrier.cta.sync 2, 128;" ::: "memory");
 }
+// Largest of the warp, by the integer order of floats (its own inverse).
+__device__ __forceinline__ int float_order(int b) { return b ^ ((b >> 31) & 0x7FFFFFFF); }
 __device__ __forceinline__ float warp_max(float v) {
-  float r;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
+  return __int_as_float(
+      float_order(__reduce_max_sync(0xffffffffu, float_order(__float_as_int(v)))));
 }
 // Sums of RB values over the warp: lane i returns that of value i * RB / 32.
 template <int RB>
@@ -207,19 +208,19 @@ struct Run {
   Seq s;
   int units, blocks, tiles;  // of the sequence
 
-  __device__ __forceinline__ void enter(const CachedArgs& a) {
-    s = load_seq(a, seq, false);
-    blocks = (s.fresh * a.group + RB - 1) / RB;
+  __device__ __forceinline__ void enter(const Seq& seq_, int group) {
+    s = seq_;
+    blocks = (s.fresh * group + RB - 1) / RB;
     tiles = s.fresh ? (s.len + Cfg<D, RB>::TT - 1) / Cfg<D, RB>::TT : 0;
     units = (tiles + unit_tiles - 1) / unit_tiles;
   }
   // `at`: cost of the sequence before the run's begin
-  __device__ __forceinline__ void start(const CachedArgs& a, int seq_, int at, int cost, int ut,
-                                        int ex) {
+  __device__ __forceinline__ void start(int seq_, const Seq& first, int at, int cost, int ut, int ex,
+                                        int group) {
     seq = seq_;
     unit_tiles = ut;
     extra = ex;
-    enter(a);
+    enter(first, group);
     sub = at / (units + extra);
     const int f = at - sub * (units + extra);
     unit = max(0, f - extra);
@@ -240,7 +241,7 @@ struct Run {
         left = 0;
         return;
       }
-      enter(a);
+      enter(load_seq(a, seq, false), a.group);
     } while (units == 0);
   }
 };
@@ -328,27 +329,28 @@ __global__ void __launch_bounds__(THREADS, 2)
 
   // ------------------------------------------------- this CTA's run
   // Each warp plans for itself (no barrier): lane l sums the costs of the
-  // sequences [l * m, l * m + m).
+  // sequences [l * m, l * m + m), as single tiles and as units of UNIT_TILES.
   const int m = (a.n_seqs + 31) / 32;
-  auto cost_of = [&](int i, bool few, bool report) {
-    if (i >= a.n_seqs) return 0;
-    const Seq s = load_seq(a, i, report);
+  auto cost_of = [&](const Seq& s, bool units) {
     if (s.fresh == 0) return 0;
     const int tiles = (s.len + C::TT - 1) / C::TT;
     const int items = (s.fresh * a.group + RB - 1) / RB * a.kv_heads;
-    return (few ? (tiles + UNIT_TILES - 1) / UNIT_TILES : tiles + ITEM_COST) * items;
+    return (units ? (tiles + UNIT_TILES - 1) / UNIT_TILES : tiles + ITEM_COST) * items;
   };
-  int sums[2] = {0, 0};
+  int sum_tiles = 0, sum_units = 0;
+#pragma unroll 4
   for (int j = 0; j < m; ++j) {
-    sums[0] += cost_of(lane * m + j, false, blockIdx.x == 0 && warp == 0);
-    sums[1] += cost_of(lane * m + j, true, false);
+    Seq s{0, 0, 0};
+    if (lane * m + j < a.n_seqs) s = load_seq(a, lane * m + j, blockIdx.x == 0 && warp == 0);
+    sum_tiles += cost_of(s, false);
+    sum_units += cost_of(s, true);
   }
   // Few tiles: runs of whole units of UNIT_TILES, so that short items are not cut
   // (a piece costs a join, about as much as four tiles), as long as no CTA gets
   // more than one. Else single tiles, for balance.
-  const bool few = a.whole || __reduce_add_sync(0xffffffffu, sums[1]) <= (int)gridDim.x;
+  const bool few = a.whole || __reduce_add_sync(0xffffffffu, sum_units) <= (int)gridDim.x;
   const int ut = few ? UNIT_TILES : 1, extra = few ? 0 : ITEM_COST;
-  const int own = few ? sums[1] : sums[0];
+  const int own = few ? sum_units : sum_tiles;
   int upto = own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -357,16 +359,29 @@ __global__ void __launch_bounds__(THREADS, 2)
   }
   const int total = __shfl_sync(0xffffffffu, upto, 31);
   // equal runs, without a gap between the CTAs that have one (the join's order)
-  const int busy_ctas = min((int)gridDim.x, total), cta = min((int)blockIdx.x, busy_ctas);
-  const int x0 = busy_ctas ? (int)((long long)cta * total / busy_ctas) : 0;
-  const int x1 = cta < busy_ctas ? (int)((long long)(cta + 1) * total / busy_ctas) : x0;
+  const int ctas = min((int)gridDim.x, total), cta = min((int)blockIdx.x, ctas);
+  const int each = total / max(1, ctas), more = total - each * ctas;
+  const int x0 = cta * each + min(cta, more);
+  const int cost = cta < ctas ? each + (cta < more) : 0;
   Run<D, RB> run;
-  bool busy = x1 > x0;
+  bool busy = cost > 0;
   if (busy) {
     const int l = __ffs(__ballot_sync(0xffffffffu, upto > x0)) - 1;  // whose sequences x0 is in
-    int at = x0 - __shfl_sync(0xffffffffu, upto - own, l), seq = l * m;
-    for (int cost; at >= (cost = cost_of(seq, few, false)); ++seq) at -= cost;
-    run.start(a, seq, at, x1 - x0, ut, extra);
+    int at = x0 - (upto - own), seq = lane * m;
+    Seq s{0, 0, 0};
+    if (lane == l) {
+      for (;; ++seq) {
+        s = load_seq(a, seq, false);
+        const int c = cost_of(s, few);
+        if (at < c) break;
+        at -= c;
+      }
+    }
+    s.len = __shfl_sync(0xffffffffu, s.len, l);
+    s.row0 = __shfl_sync(0xffffffffu, s.row0, l);
+    s.fresh = __shfl_sync(0xffffffffu, s.fresh, l);
+    run.start(__shfl_sync(0xffffffffu, seq, l), s, __shfl_sync(0xffffffffu, at, l), cost, ut, extra,
+              a.group);
     busy = run.left > 0;  // a run may lie inside one item's extra part
   }
   if (threadIdx.x == 64) a.meta[blockIdx.x * 4] = 0;  // warp 2 knows better later
@@ -968,47 +983,50 @@ __global__ void __launch_bounds__(THREADS, 2)
         const float sums = warp_add<RB>(l);
         if (lane % (32 / RB) == 0)
           reinterpret_cast<float*>(wmax + lane / (32 / RB))[warp - 4] = sums;
-        float* other = reinterpret_cast<float*>(pb);  // the weights have been read
-        if (TPL == 2 && half) {
+        // rows of [token half][column] in the weights' buffer, which has been read
+        float* rows = reinterpret_cast<float*>(pb);
 #pragma unroll
-          for (int r = 0; r < RB; ++r) other[r * 64 + d] = v[r];
-        }
+        for (int r = 0; r < RB; ++r) rows[r * 128 + line] = v[r];
         compute_barrier();
         poison[line] = 0;
         const ItemInfo it = *item_info(b);
-        if (TPL == 1 || !half) {
-          // a piece that continues an earlier CTA's item goes to slot 0, one
-          // that begins here and ends elsewhere to slot 1
-          float* part = a.part + ((size_t)blockIdx.x * 2 + (it.starts ? 1 : 0)) * kCachedPartFloats;
-          const bool whole = it.starts && it.ends;
-          // lane r of each warp: row r's sum
-          const float4 w4 = wmax[lane & (RB - 1)];
+        const bool whole = it.starts && it.ends;
+        // a piece that continues an earlier CTA's item goes to slot 0, one that
+        // begins here and ends elsewhere to slot 1
+        float* part = a.part + ((size_t)blockIdx.x * 2 + (it.starts ? 1 : 0)) * kCachedPartFloats;
+#pragma unroll
+        for (int k = 0; k < (RB * D / 4 + 127) / 128; ++k) {
+          const int r = (k * 128 + line) / (D / 4), c = line % (D / 4);
+          if (r >= it.n_rows) break;
+          float4 y = reinterpret_cast<const float4*>(rows + r * 128)[c];
+          if (TPL == 2) {
+            const float4 z = reinterpret_cast<const float4*>(rows + r * 128 + 64)[c];
+            y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
+          }
+          if (!whole) {
+            reinterpret_cast<float4*>(part + r * D)[c] = y;
+            continue;
+          }
+          const float4 w4 = wmax[r];
           const float sum = (w4.x + w4.y) + (w4.z + w4.w);
-          const float inv = sum == 0.f ? 0.f : whole ? __fdividef(1.f, sum) : 1.f;
-          uint16_t* o = a.o + d;
+          const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
+          *reinterpret_cast<uint2*>(a.o + item_out(b)[r] + 4 * c) =
+              make_uint2(to_out<BF>(y.x * inv) | (uint32_t)to_out<BF>(y.y * inv) << 16,
+                         to_out<BF>(y.z * inv) | (uint32_t)to_out<BF>(y.w * inv) << 16);
+        }
+        if (!whole && line < it.n_rows) {
+          const float4 w4 = wmax[line];
+          const float sum = (w4.x + w4.y) + (w4.z + w4.w);
+          float top = 0.f;
 #pragma unroll
-          for (int r = 0; r < RB; ++r) {
-            if (TPL == 2) v[r] += other[r * 64 + d];
-            v[r] *= __shfl_sync(0xffffffffu, inv, r);
-            if (r < it.n_rows) {
-              if (whole)
-                o[item_out(b)[r]] = to_out<BF>(v[r]);
-              else
-                part[r * D + d] = v[r];
-            }
-          }
-          if (!whole && line < it.n_rows) {
-            // a row that saw nothing has no maximum
-            float top = 0.f;
-#pragma unroll
-            for (int r = 0; r < RB; ++r) top = lane == r ? P_EXP - off[r] : top;
-            part[kCachedPartRows * 128 + line] = sum == 0.f ? -INFINITY : top;
-            part[kCachedPartRows * 129 + line] = sum;
-          }
+          for (int r = 0; r < RB; ++r) top = line == r ? P_EXP - off[r] : top;
+          // a row that saw nothing has no maximum
+          part[kCachedPartRows * 128 + line] = sum == 0.f ? -INFINITY : top;
+          part[kCachedPartRows * 129 + line] = sum;
         }
         tc_fence_before();
         mbar_arrive(bar_q_empty + 8 * b);
-        compute_barrier();  // `other`, wmax and poison may be written again
+        compute_barrier();  // `rows`, wmax and poison may be written again
         ++items;
         if (info.z & kFinal) break;
       }
