@@ -55,11 +55,9 @@ struct PK {
   static constexpr int OFF_K = T * TILE;
   static constexpr int OFF_V = OFF_K + KST * TILE;
   static constexpr int OFF_BAR = OFF_V + VST * TILE;
-  // q_full[T], k_full/k_empty[KST], v_full/v_empty[VST], v_raw, s_full[T],
-  // s_free, p_full[T], o_full, o_done[T], drain
-  static constexpr int BARS = 4 * T + 2 * KST + 2 * VST + 4;
-  static constexpr int OFF_MISC = OFF_BAR + BARS * 8;
-  static constexpr int MISC = 80;
+  static constexpr int BARS = 4 * T + 2 * KST + 2 * VST + 9;
+  static constexpr int OFF_MISC = (OFF_BAR + BARS * 8 + 15) / 16 * 16;
+  static constexpr int MISC = 128;
   static constexpr int SMEM = OFF_MISC + MISC + 1024;
   static constexpr uint32_t COLS = D == 128 ? 512 : 256;
   static constexpr uint32_t S(int t) { return 128u * t; }
@@ -85,7 +83,7 @@ struct PackedArgs {
 };
 
 struct Item {
-  int row0, len, tile;
+  int row0, len, tile, unit;  // tile < 0: no more
 };
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -108,14 +106,20 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
   return __vcmpeq2(w & E, E);
 }
 
-// Which sequence and tile of `span` rows the CTA's tile number means, counted
-// from the last tile backwards (in a causal sequence the last tiles have the
-// most keys). By one warp; tile < 0: none.
-__device__ Item find_item(const PackedArgs& a, int span, int number) {
-  const int lane = threadIdx.x & 31;
-  auto tiles = [&](int i, int& r0, int& len) {
-    r0 = len = 0;
-    if (i >= a.n_seqs) return 0;
+// The tiles of `span` rows of all sequences, in the order they are worked on:
+// those with the most keys first, so that the last ones to finish are short (a
+// causal tile's keys grow with its place in the sequence, another's with its
+// sequence). Up to 4 sequences per lane of the warp are kept in registers and a
+// tile is found by bisection over its key count; with more sequences the tiles
+// come sequence by sequence, from the last backwards.
+struct Finder {
+  static constexpr int KEEP = 4;
+  int row0[KEEP], len[KEEP], tiles[KEEP];
+  int span, most;
+
+  __device__ __forceinline__ int load(const PackedArgs& a, int i, int& r0, int& n) const {
+    r0 = n = 0;
+    if (i < 0 || i >= a.n_seqs) return 0;
     r0 = a.cu[i];
     const int r1 = a.cu[i + 1];
     if (!rows_fit(r0, r1, a.rows)) {
@@ -123,33 +127,118 @@ __device__ Item find_item(const PackedArgs& a, int span, int number) {
       r0 = 0;
       return 0;
     }
-    len = r1 - r0;
-    return (len + span - 1) / span;
-  };
-  int seen = 0;
-  for (int i0 = (a.n_seqs - 1) / 32 * 32; i0 >= 0; i0 -= 32) {
-    int r0, len;
-    const int mine = tiles(i0 + 31 - lane, r0, len);  // lane 0 has the last sequence
-    int sum = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += u;
-    }
-    const uint32_t hit = __ballot_sync(0xffffffffu, seen + sum > number);
-    if (hit) {
-      const int l = __ffs(hit) - 1;
-      Item it;
-      it.row0 = __shfl_sync(0xffffffffu, r0, l);
-      it.len = __shfl_sync(0xffffffffu, len, l);
-      const int end = seen + __shfl_sync(0xffffffffu, sum, l);
-      it.tile = end - 1 - number;
-      return it;
-    }
-    seen += __shfl_sync(0xffffffffu, sum, 31);
+    n = r1 - r0;
+    return (n + span - 1) / span;
   }
-  return {0, 0, -1};
+  __device__ __forceinline__ void init(const PackedArgs& a, int span_) {
+    span = span_;
+    most = 0;
+    if (a.n_seqs > 32 * KEEP) return;
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k) {
+      tiles[k] = 32 * k < a.n_seqs ? load(a, 32 * k + (threadIdx.x & 31), row0[k], len[k]) : 0;
+      most = max(most, tiles[k]);
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+  }
+  // tiles with at least `keys` key tiles
+  __device__ __forceinline__ int at_least(bool causal, int keys) const {
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k)
+      n += causal ? max(0, tiles[k] - keys + 1) : tiles[k] >= keys ? tiles[k] : 0;
+    return __reduce_add_sync(0xffffffffu, n);
+  }
+  __device__ __forceinline__ Item find(const PackedArgs& a, int number) const {
+    const int lane = threadIdx.x & 31;
+    if (a.n_seqs <= 32 * KEEP) {
+      int lo = 0, hi = most;  // the largest count with more than `number` tiles at or above it
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (at_least(a.causal, mid) > number)
+          lo = mid;
+        else
+          hi = mid - 1;
+      }
+      if (lo == 0) return {0, 0, -1, 0};
+      int rank = number - at_least(a.causal, lo + 1), tile = lo - 1;
+      if (!a.causal) {
+        tile = rank % lo;
+        rank /= lo;
+      }
+#pragma unroll
+      for (int k = 0; k < KEEP; ++k) {
+        const bool in = a.causal ? tiles[k] >= lo : tiles[k] == lo;
+        const uint32_t set = __ballot_sync(0xffffffffu, in);
+        const int n = __popc(set);
+        if (rank < n) {
+          const uint32_t hit =
+              __ballot_sync(0xffffffffu, in && __popc(set & ((1u << lane) - 1)) == rank);
+          const int l = __ffs(hit) - 1;
+          return {__shfl_sync(0xffffffffu, row0[k], l), __shfl_sync(0xffffffffu, len[k], l), tile, 0};
+        }
+        rank -= n;
+      }
+      return {0, 0, -1, 0};
+    }
+    int seen = 0;
+    for (int i0 = (a.n_seqs - 1) / 32 * 32; i0 >= 0; i0 -= 32) {
+      int r0, n;
+      const int mine = load(a, i0 + 31 - lane, r0, n);  // lane 0 has the last sequence
+      int sum = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += u;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, seen + sum > number);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        return {__shfl_sync(0xffffffffu, r0, l), __shfl_sync(0xffffffffu, n, l),
+                seen + __shfl_sync(0xffffffffu, sum, l) - 1 - number, 0};
+      }
+      seen += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return {0, 0, -1, 0};
+  }
+};
+
+// What an item means to a CTA: per query tile its head, first row in the
+// sequence and key tiles.
+struct Work {
+  int row0, len, head0, kv_head, qt[2], n[2], nmax;
+  bool ph;
+};
+template <int T>
+__device__ __forceinline__ Work work_of(const PackedArgs& a, const Item& it) {
+  Work w;
+  w.row0 = it.row0;
+  w.len = it.len;
+  w.ph = T == 2 && a.pair_heads;
+  w.head0 = w.ph ? 2 * it.unit : it.unit;
+  w.kv_head = w.head0 / a.group;
+  w.qt[0] = T == 2 && !w.ph ? it.tile * 256 : it.tile * 128;
+  w.qt[1] = w.ph ? w.qt[0] : w.qt[0] + 128;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int keys = a.causal ? min(w.len, w.qt[t] + BQ) : w.len;
+    w.n[t] = t < T && w.qt[t] < w.len ? (keys + BKV - 1) / BKV : 0;
+  }
+  w.nmax = max(w.n[0], w.n[1]);
+  return w;
 }
+// Tile c of a stream through a ring of N stages.
+template <int N>
+struct Ring {
+  int st = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void step() {
+    if (++st == N) {
+      st = 0;
+      ph ^= 1;
+    }
+  }
+};
 
 template <int D, bool BF>
 __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
@@ -166,8 +255,11 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
   const uint32_t sbase = smem_u32(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  const uint32_t bar_q = sbase + C::OFF_BAR;
-  const uint32_t bar_k_full = bar_q + 8 * T;
+  const uint32_t bar_item = sbase + C::OFF_BAR;  // [2] an item is told
+  const uint32_t bar_item_free = bar_item + 16;     // [2] and done with
+  const uint32_t bar_q = bar_item_free + 16;        // [T] queries are there
+  const uint32_t bar_q_free = bar_q + 8 * T;        // the item's last Q K^T is done
+  const uint32_t bar_k_full = bar_q_free + 8;
   const uint32_t bar_k_empty = bar_k_full + 8 * KST;
   const uint32_t bar_v_full = bar_k_empty + 8 * KST;
   const uint32_t bar_v_empty = bar_v_full + 8 * VST;
@@ -176,15 +268,21 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
   const uint32_t bar_s_free = bar_s_full + 8 * T;    // scores are in registers (P apart)
   const uint32_t bar_p_full = bar_s_free + 8;        // [T] P written
   const uint32_t bar_o_full = bar_p_full + 8 * T;    // P V done (P apart)
-  const uint32_t bar_o_done = bar_o_full + 8;        // [T] after the last P V
+  const uint32_t bar_o_done = bar_o_full + 8;        // [T] after an item's last P V
   const uint32_t bar_drain = bar_o_done + 8 * T;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
-  volatile int* item_slot = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
-  int* fix_tile = reinterpret_cast<int*>(smem + C::OFF_MISC + 20);         // [2]
-  uint32_t* fix_rows = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC + 28);  // [2][4]
+  // [2] items; of each the V tiles looked through and the rows with infinities
+  Item* items = reinterpret_cast<Item*>(smem + C::OFF_MISC + 16);
+  int* fix_tile = reinterpret_cast<int*>(smem + C::OFF_MISC + 48);            // [2][2]
+  uint32_t* fix_rows = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC + 64);  // [2][2][4]
 
   if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar_item + 8 * i, 1);
+      mbar_init(bar_item_free + 8 * i, 1 + 4 * T);  // the issuer and the softmax warps
+    }
+    mbar_init(bar_q_free, 1);
     for (int t = 0; t < T; ++t) {
       mbar_init(bar_q + 8 * t, 1);
       mbar_init(bar_s_full + 8 * t, 1);
@@ -204,8 +302,6 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
     mbar_init(bar_o_full, 1);
     mbar_init(bar_drain, 1);
     *abort_flag = 0;
-    for (int i = 0; i < 2; ++i) fix_tile[i] = 0;
-    for (int i = 0; i < 8; ++i) fix_rows[i] = 0;
     fence_mbar_init();
     prefetch_tmap(&map_q);
     prefetch_tmap(&map_k);
@@ -221,70 +317,74 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
   const uint32_t tmem = *tmem_slot;
   griddep_launch_dependents();  // behind the allocation: the next kernel allocates too
   griddep_wait();  // offsets and rows may be earlier kernels' outputs
-  const int unit = blockIdx.x % a.units;
+
   if (warp == 0) {
-    const Item it = find_item(a, T == 2 && !a.pair_heads ? 256 : 128, blockIdx.x / a.units);
-    if (lane == 0) {
-      item_slot[0] = it.row0;
-      item_slot[1] = it.len;
-      item_slot[2] = it.tile;
-    }
-  }
-  __syncthreads();
-  const int row0 = item_slot[0], len = item_slot[1], tile = item_slot[2];
-
-  if (tile >= 0) {
-    // per query tile: head, first row in the sequence, key tiles
-    const bool ph = T == 2 && a.pair_heads;
-    const int head0 = ph ? 2 * unit : unit;
-    const int q0 = T == 2 && !ph ? tile * 256 : tile * 128;
-    const int qt[2] = {q0, ph ? q0 : q0 + 128};
-    int n[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int keys = a.causal ? min(len, qt[t] + BQ) : len;
-      n[t] = t < T && qt[t] < len ? (keys + BKV - 1) / BKV : 0;
-    }
-    const int nmax = max(n[0], n[1]);
-    const int kv_head = head0 / a.group;
-
-    if (warp == 0) {
-      // ----------------------------------------------------------- producer
-      uint32_t k_bits = 0, k_par = 0, v_bits = 0, v_par = 0;  // loads to drain on abort
-      uint32_t raw_uses = 0;
-      bool ok = true;
+    // ----------------------------------------------------------- producer
+    Finder finder;
+    finder.init(a, T == 2 && !a.pair_heads ? 256 : 128);
+    uint32_t k_bits = 0, k_par = 0, v_bits = 0, v_par = 0;  // loads to drain on abort
+    uint32_t raw_uses = 0, q_par = 0;
+    Ring<KST> rk;
+    Ring<VST> rv;
+    bool ok = true;
+    for (uint32_t i = 0; ok; ++i) {
+      // the rounds over the tiles go to and fro, so that no CTA always gets the
+      // longer ones
+      const int number = (int)(i * gridDim.x + (i & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x));
+      Item it = finder.find(a, number / a.units);
+      it.unit = number % a.units;
+      const int slot = i & 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(bar_item_free + 8 * slot, (i >> 1 & 1) ^ 1, abort_flag,
+                                             a.err, kDevErrTimeoutPacked));
+      if (!ok) break;
+      if (lane == 0) items[slot] = it;
+      if (lane < 2) fix_tile[slot * 2 + lane] = 0;
+      if (lane < 8) fix_rows[slot * 8 + lane] = 0;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_item + 8 * slot);
+      if (it.tile < 0) break;
+      const Work w = work_of<T>(a, it);
       if (lane == 0) {
-        for (int t = 0; t < T; ++t)
-          if (n[t]) {
-            mbar_arrive_expect_tx(bar_q + 8 * t, C::TILE);
-            tma_load_3d(sbase + t * C::TILE, &map_q, bar_q + 8 * t, 0, row0 + qt[t],
-                        (ph ? head0 + t : head0) * C::HALVES);
+        ok = mbar_wait(bar_q_free, (i & 1) ^ 1, abort_flag, a.err, kDevErrTimeoutPacked);
+        for (int t = 0; t < T && ok; ++t) {
+          if (!w.n[t]) {  // nothing to load, but a phase like every item's
+            mbar_arrive(bar_q + 8 * t);
+            continue;
           }
+          mbar_arrive_expect_tx(bar_q + 8 * t, C::TILE);
+          tma_load_3d(sbase + t * C::TILE, &map_q, bar_q + 8 * t, 0, w.row0 + w.qt[t],
+                      (w.ph ? w.head0 + t : w.head0) * C::HALVES);
+        }
+        if (ok) q_par = i + 1;
       }
-      for (int j = 0; j < nmax && ok; ++j) {
-        const int ks = j % KST, vs = j % VST;
-        const uint32_t kph = (uint32_t)(j / KST) & 1u, vph = (uint32_t)(j / VST) & 1u;
+      int fixes = 0;
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+      for (int j = 0; j < w.nmax && ok; ++j) {
         // does some query of the CTA see a part of this tile only?
-        const bool diag = a.causal && (j == n[0] - 1 || j == n[1] - 1);
-        const bool fix = diag || (j + 1) * BKV > len;
+        const bool diag = a.causal && (j == w.n[0] - 1 || j == w.n[1] - 1);
+        const bool fix = diag || (j + 1) * BKV > w.len;
         if (lane == 0) {
-          ok = mbar_wait(bar_k_empty + 8 * ks, kph ^ 1, abort_flag, a.err, kDevErrTimeoutPacked);
+          ok = mbar_wait(bar_k_empty + 8 * rk.st, rk.ph ^ 1, abort_flag, a.err,
+                         kDevErrTimeoutPacked);
           if (ok) {
-            mbar_arrive_expect_tx(bar_k_full + 8 * ks, C::TILE);
-            tma_load_3d(sbase + C::OFF_K + ks * C::TILE, &map_k, bar_k_full + 8 * ks, 0,
-                        row0 + j * BKV, kv_head * C::HALVES);
-            k_bits |= 1u << ks;
-            k_par = (k_par & ~(1u << ks)) | (kph << ks);
-            ok = mbar_wait(bar_v_empty + 8 * vs, vph ^ 1, abort_flag, a.err, kDevErrTimeoutPacked);
+            mbar_arrive_expect_tx(bar_k_full + 8 * rk.st, C::TILE);
+            tma_load_3d(sbase + C::OFF_K + rk.st * C::TILE, &map_k, bar_k_full + 8 * rk.st, 0,
+                        w.row0 + j * BKV, w.kv_head * C::HALVES);
+            k_bits |= 1u << rk.st;
+            k_par = (k_par & ~(1u << rk.st)) | (rk.ph << rk.st);
+            ok = mbar_wait(bar_v_empty + 8 * rv.st, rv.ph ^ 1, abort_flag, a.err,
+                           kDevErrTimeoutPacked);
           }
           if (ok) {
-            const uint32_t bar = fix ? bar_v_raw : bar_v_full + 8 * vs;
+            const uint32_t bar = fix ? bar_v_raw : bar_v_full + 8 * rv.st;
             mbar_arrive_expect_tx(bar, C::TILE);
-            tma_load_3d(sbase + C::OFF_V + vs * C::TILE, &map_v, bar, 0, row0 + j * BKV,
-                        kv_head * C::HALVES);
+            tma_load_3d(sbase + C::OFF_V + rv.st * C::TILE, &map_v, bar, 0, w.row0 + j * BKV,
+                        w.kv_head * C::HALVES);
             if (!fix) {
-              v_bits |= 1u << vs;
-              v_par = (v_par & ~(1u << vs)) | (vph << vs);
+              v_bits |= 1u << rv.st;
+              v_par = (v_par & ~(1u << rv.st)) | (rv.ph << rv.st);
+            } else {
+              v_bits &= ~(1u << rv.st);
             }
           }
         }
@@ -296,57 +396,66 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
             *abort_flag = 1;
             atomicExch(a.err, kDevErrTimeoutPacked);
           }
-          const int nth = raw_uses ? 1 : 0;  // at most two such tiles per CTA
           ++raw_uses;
+          const int nth = slot * 2 + fixes;  // at most two such tiles per item
+          ++fixes;
           if (lane == 0) fix_tile[nth] = j;
           __syncwarp();
-          uint4* vt = reinterpret_cast<uint4*>(smem + C::OFF_V + vs * C::TILE);
-          const int held = len - j * BKV;  // rows of the sequence in this tile
-#pragma unroll 4
-          for (int i = lane; i < C::TILE / 16; i += 32) {
-            const int r = (i >> 3) & (BKV - 1);
+          uint4* vt = reinterpret_cast<uint4*>(smem + C::OFF_V + rv.st * C::TILE);
+          const int held = w.len - j * BKV;  // rows of the sequence in this tile
+#pragma unroll 8
+          for (int e = lane; e < C::TILE / 16; e += 32) {
+            const int r = (e >> 3) & (BKV - 1);
             if (r >= held) {
-              vt[i] = make_uint4(0, 0, 0, 0);
+              vt[e] = make_uint4(0, 0, 0, 0);
             } else if (diag) {
-              const uint4 w = vt[i];
-              const uint4 b = make_uint4(not_finite<BF>(w.x), not_finite<BF>(w.y),
-                                         not_finite<BF>(w.z), not_finite<BF>(w.w));
+              const uint4 x = vt[e];
+              const uint4 b = make_uint4(not_finite<BF>(x.x), not_finite<BF>(x.y),
+                                         not_finite<BF>(x.z), not_finite<BF>(x.w));
               if (b.x | b.y | b.z | b.w) {
-                vt[i] = make_uint4(w.x & ~b.x, w.y & ~b.y, w.z & ~b.z, w.w & ~b.w);
+                vt[e] = make_uint4(x.x & ~b.x, x.y & ~b.y, x.z & ~b.z, x.w & ~b.w);
                 atomicOr(&fix_rows[nth * 4 + (r >> 5)], 1u << (r & 31));
               }
             }
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar_v_full + 8 * vs);
+          if (lane == 0) mbar_arrive(bar_v_full + 8 * rv.st);
         }
+        rk.step();
+        rv.step();
       }
-      if (lane == 0 && *abort_flag) {
-        for (int t = 0; t < T; ++t)
-          if (n[t]) mbar_wait_drain(bar_q + 8 * t, 0);
-        for (int s = 0; s < KST; ++s)
-          if (k_bits & (1u << s)) mbar_wait_drain(bar_k_full + 8 * s, (k_par >> s) & 1u);
-        for (int s = 0; s < VST; ++s)
-          if (v_bits & (1u << s)) mbar_wait_drain(bar_v_full + 8 * s, (v_par >> s) & 1u);
-      }
-    } else if (warp == 1) {
-      // ----------------------------------------------------------- MMA issuer
-      if (lane == 0) {
-        bool ok = true;
-        auto wait = [&](uint32_t bar, uint32_t par) {
-          return mbar_wait(bar, par, abort_flag, a.err, kDevErrTimeoutPacked);
-        };
-        auto wait_k = [&](int j) {
-          return wait(bar_k_full + 8 * (j % KST), (uint32_t)(j / KST) & 1u);
-        };
-        auto wait_v = [&](int j) {
-          return wait(bar_v_full + 8 * (j % VST), (uint32_t)(j / VST) & 1u);
-        };
-        auto last_of = [&](int j) { return T == 2 && j < n[1] ? 1 : 0; };
+    }
+    if (lane == 0 && *abort_flag) {
+      for (int t = 0; t < T; ++t)
+        if (q_par) mbar_wait_drain(bar_q + 8 * t, (q_par - 1) & 1u);
+      for (int s = 0; s < KST; ++s)
+        if (k_bits & (1u << s)) mbar_wait_drain(bar_k_full + 8 * s, (k_par >> s) & 1u);
+      for (int s = 0; s < VST; ++s)
+        if (v_bits & (1u << s)) mbar_wait_drain(bar_v_full + 8 * s, (v_par >> s) & 1u);
+    }
+  } else if (warp == 1) {
+    // ----------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      bool ok = true, issued = false;
+      auto wait = [&](uint32_t bar, uint32_t par) {
+        return mbar_wait(bar, par, abort_flag, a.err, kDevErrTimeoutPacked);
+      };
+      Ring<KST> rk;   // of the next Q K^T
+      Ring<VST> rv;   // of the next P V
+      uint32_t n_p[2] = {0, 0};  // P tiles waited for
+      uint32_t n_s = 0;          // S tiles issued (P apart)
+      for (uint32_t i = 0; ok; ++i) {
+        ok = wait(bar_item + 8 * (i & 1), i >> 1 & 1);
+        if (!ok) break;
+        const Item it = items[i & 1];
+        mbar_arrive(bar_item_free + 8 * (i & 1));
+        if (it.tile < 0) break;
+        const Work w = work_of<T>(a, it);
+        auto last_of = [&](int j) { return T == 2 && j < w.n[1] ? 1 : 0; };
         auto issue_qk = [&](int t, int j) {
           const uint64_t dq = umma_desc_sw128(sbase + t * C::TILE);
-          const uint64_t dk = umma_desc_sw128(sbase + C::OFF_K + (j % KST) * C::TILE);
+          const uint64_t dk = umma_desc_sw128(sbase + C::OFF_K + rk.st * C::TILE);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off = (kk / 4) * C::HALF + (kk % 4) * 32;
@@ -354,100 +463,111 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
                         kk != 0);
           }
           umma_commit(bar_s_full + 8 * t);
-          if (t == last_of(j)) umma_commit(bar_k_empty + 8 * (j % KST));
+          issued = true;
+          if (t == last_of(j)) {
+            umma_commit(bar_k_empty + 8 * rk.st);
+            rk.step();
+            if (j == w.nmax - 1) umma_commit(bar_q_free);
+          }
         };
         auto issue_pv = [&](int t, int j) {
           // V tile: keys along K, head_dim along N in 64-wide groups HALF apart
-          uint64_t dv = umma_desc_sw128_mn(sbase + C::OFF_V + (j % VST) * C::TILE);
+          uint64_t dv = umma_desc_sw128_mn(sbase + C::OFF_V + rv.st * C::TILE);
           dv = (dv & ~(0x3FFFull << 16)) | ((uint64_t)(C::HALF >> 4) << 16);
 #pragma unroll
           for (int kk = 0; kk < BKV / 16; ++kk)
             umma_f16_ts(tmem + C::O(t), tmem + C::P(t) + kk * 8, desc_advance(dv, kk * 2048),
                         IDESC_O, (j | kk) != 0);
           if (!C::OVERLAY) umma_commit(bar_o_full);
-          if (t == last_of(j)) umma_commit(bar_v_empty + 8 * (j % VST));
+          if (t == last_of(j)) {
+            umma_commit(bar_v_empty + 8 * rv.st);
+            rv.step();
+          }
+          if (j == w.n[t] - 1) umma_commit(bar_o_done + 8 * t);
         };
+        ok = wait(bar_q, i & 1) && wait(bar_k_full + 8 * rk.st, rk.ph);
         if (C::OVERLAY) {
-          ok = wait(bar_q, 0) && wait_k(0);
           if (ok) {
             tc_fence_after();
             issue_qk(0, 0);
+            if (w.n[1]) {
+              ok = wait(bar_q + 8 * (T - 1), i & 1);
+              if (ok) issue_qk(1, 0);
+            }
           }
-          if (ok && n[1]) {
-            ok = wait(bar_q + 8 * (T - 1), 0);
-            if (ok) issue_qk(1, 0);
-          }
-          for (int j = 0; j < nmax && ok; ++j) {
+          for (int j = 0; j < w.nmax && ok; ++j) {
             bool v_here = false, k_here = false;
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-              if (j >= n[t] || !ok) continue;
-              ok = wait(bar_p_full + 8 * t, (uint32_t)j & 1u) && (v_here || wait_v(j));
+              if (j >= w.n[t] || !ok) continue;
+              ok = wait(bar_p_full + 8 * t, n_p[t]++ & 1u) &&
+                   (v_here || wait(bar_v_full + 8 * rv.st, rv.ph));
               if (!ok) continue;
               v_here = true;
               tc_fence_after();
               issue_pv(t, j);
-              if (j + 1 < n[t]) {
-                ok = k_here || wait_k(j + 1);
+              if (j + 1 < w.n[t]) {
+                ok = k_here || wait(bar_k_full + 8 * rk.st, rk.ph);
                 if (!ok) continue;
                 k_here = true;
                 tc_fence_after();
                 issue_qk(t, j + 1);
-              } else {
-                umma_commit(bar_o_done + 8 * t);
               }
             }
           }
         } else {
-          ok = wait(bar_q, 0) && wait_k(0);
-          if (ok) {
+          // S is free once the softmax has read the tile before
+          auto next_s = [&](int j) {
+            ok = wait(bar_k_full + 8 * rk.st, rk.ph) && (n_s == 0 || wait(bar_s_free, (n_s - 1) & 1u));
+            if (!ok) return;
             tc_fence_after();
-            issue_qk(0, 0);
-          }
-          if (ok && nmax > 1) {
-            ok = wait_k(1) && wait(bar_s_free, 0);
-            if (ok) {
-              tc_fence_after();
-              issue_qk(0, 1);
-            }
-          }
-          for (int j = 0; j < nmax && ok; ++j) {
-            ok = wait(bar_p_full, (uint32_t)j & 1u) && wait_v(j);
+            issue_qk(0, j);
+            ++n_s;
+          };
+          if (ok) next_s(0);
+          if (ok && w.nmax > 1) next_s(1);
+          for (int j = 0; j < w.nmax && ok; ++j) {
+            ok = wait(bar_p_full, n_p[0]++ & 1u) && wait(bar_v_full + 8 * rv.st, rv.ph);
             if (!ok) break;
             tc_fence_after();
             issue_pv(0, j);
-            if (j + 2 < nmax) {
-              ok = wait_k(j + 2) && wait(bar_s_free, (uint32_t)(j + 1) & 1u);
-              if (!ok) break;
-              tc_fence_after();
-              issue_qk(0, j + 2);
-            }
+            if (j + 2 < w.nmax) next_s(j + 2);
           }
-          if (ok) umma_commit(bar_o_done);
-        }
-        if (*abort_flag) {
-          umma_commit(bar_drain);
-          mbar_wait_drain(bar_drain, 0);
         }
       }
-    } else {
-      // ----------------------------------------------------------- softmax rows
-      constexpr float kRescaleLog2 = 8.0f;
-      const int t = T == 2 ? (warp - 2) >> 2 : 0;
-      const int quad = warp & 3;  // this warp's TMEM lane quadrant
-      const int r = quad * 32 + lane;
-      const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
-      const uint32_t s_col = lane_base + C::S(t), p_col = lane_base + C::P(t),
-                     o_col = lane_base + C::O(t);
-      const int pos = qt[t] + r;                              // row in the sequence
-      const int lim = a.causal ? min(len, pos + 1) : len;     // keys it sees
-      const int lim_min = a.causal ? min(len, qt[t] + 1) : len;  // that all rows of the tile see
-      const float c = a.c;
+      if (*abort_flag && issued) {
+        umma_commit(bar_drain);
+        mbar_wait_drain(bar_drain, 0);
+      }
+    }
+  } else {
+    // ----------------------------------------------------------- softmax rows
+    constexpr float kRescaleLog2 = 8.0f;
+    const int t = T == 2 ? (warp - 2) >> 2 : 0;
+    const int quad = warp & 3;  // this warp's TMEM lane quadrant
+    const int r = quad * 32 + lane;
+    const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
+    const uint32_t s_col = lane_base + C::S(t), p_col = lane_base + C::P(t),
+                   o_col = lane_base + C::O(t);
+    const float c = a.c;
+    auto wait = [&](uint32_t bar, uint32_t par) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, par, abort_flag, a.err, kDevErrTimeoutPacked));
+    };
+    uint32_t tiles = 0, outs = 0;  // key tiles and items of this query tile so far
+    for (uint32_t i = 0;; ++i) {
+      if (!wait(bar_item + 8 * (i & 1), i >> 1 & 1)) break;
+      const Item it = items[i & 1];
+      if (it.tile < 0) break;
+      const Work w = work_of<T>(a, it);
+      const int n = T == 2 && t ? w.n[1] : w.n[0], q0 = T == 2 && t ? w.qt[1] : w.qt[0];
+      const int len = w.len;
+      const int pos = q0 + r;                              // row in the sequence
+      const int lim = a.causal ? min(len, pos + 1) : len;  // keys it sees
+      const int lim_min = a.causal ? min(len, q0 + 1) : len;  // that all rows of the tile see
       float m_run = -INFINITY, l_run = 0.f;
       bool ok = true;
-      for (int j = 0; j < n[t] && ok; ++j) {
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_s_full + 8 * t, (uint32_t)j & 1u, abort_flag,
-                                               a.err, kDevErrTimeoutPacked));
+      for (int j = 0; j < n; ++j, ++tiles) {
+        ok = wait(bar_s_full + 8 * t, tiles & 1u);
         if (!ok) break;
         tc_fence_after();
         uint32_t v[BKV];
@@ -494,9 +614,8 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
           ls[e & 3] += p0 + p1;
           pk[e] = pack2<BF>(p0, p1);
         }
-        if (!C::OVERLAY && j > 0) {  // P V of the tile before still reads P
-          ok = __all_sync(0xffffffffu, mbar_wait(bar_o_full, (uint32_t)(j - 1) & 1u, abort_flag,
-                                                 a.err, kDevErrTimeoutPacked));
+        if (!C::OVERLAY && tiles > 0) {  // P V of the tile before still reads P
+          ok = wait(bar_o_full, (tiles - 1) & 1u);
           if (!ok) break;
           tc_fence_after();
         }
@@ -526,14 +645,13 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
         tc_fence_before();
         mbar_arrive(bar_p_full + 8 * t);
       }
-      if (ok && n[t])
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_o_done + 8 * t, 0u, abort_flag, a.err,
-                                               kDevErrTimeoutPacked));
-      if (ok && n[t]) {
+      if (!ok) break;
+      if (n) {
+        if (!wait(bar_o_done + 8 * t, outs++ & 1u)) break;
         tc_fence_after();
         const float inv = 1.f / l_run;
-        const int head = ph ? head0 + t : head0;
-        uint16_t* drow = a.o + (int64_t)(row0 + pos) * a.o_stride + head * D;
+        const int head = w.ph ? w.head0 + t : w.head0;
+        uint16_t* drow = a.o + (int64_t)(w.row0 + pos) * a.o_stride + head * D;
 #pragma unroll
         for (int h = 0; h < C::HALVES; ++h) {
           uint32_t o[64];
@@ -545,17 +663,19 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
           for (int d = 0; d < 64; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * inv);
           // infinities and NaN that warp 0 took out of the diagonal V tiles
           for (int f = 0; f < 8; ++f) {
-            uint32_t bits = fix_rows[f];
+            uint32_t bits = fix_rows[(i & 1) * 8 + f];
             while (bits) {
-              const int key = fix_tile[f >> 2] * BKV + (f & 3) * 32 + __ffs(bits) - 1;
+              const int key =
+                  fix_tile[(i & 1) * 2 + (f >> 2)] * BKV + (f & 3) * 32 + __ffs(bits) - 1;
               bits &= bits - 1;
               if (key >= lim) continue;
-              const uint16_t* vr = a.v + (int64_t)(row0 + key) * a.v_stride + kv_head * D + 64 * h;
+              const uint16_t* vr =
+                  a.v + (int64_t)(w.row0 + key) * a.v_stride + w.kv_head * D + 64 * h;
 #pragma unroll
               for (int d = 0; d < 64; ++d) {
-                const uint32_t w = vr[d];
-                const float x = BF ? __uint_as_float(w << 16) : unpack_half2(w).x;
-                if (not_finite<BF>(w) & 0xFFFFu)
+                const uint32_t x16 = vr[d];
+                const float x = BF ? __uint_as_float(x16 << 16) : unpack_half2(x16).x;
+                if (not_finite<BF>(x16) & 0xFFFFu)
                   o[d] = __float_as_uint(__uint_as_float(o[d]) + x);
               }
             }
@@ -563,26 +683,29 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
           if (a.o32) {  // 32-byte stores: whole sectors
 #pragma unroll
             for (int c16 = 0; c16 < 4; ++c16) {
-              uint32_t w[8];
+              uint32_t x[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e)
-                w[e] = pack2<BF>(__uint_as_float(o[16 * c16 + 2 * e]),
+                x[e] = pack2<BF>(__uint_as_float(o[16 * c16 + 2 * e]),
                                  __uint_as_float(o[16 * c16 + 2 * e + 1]));
-              st_global_v8(drow + 64 * h + 16 * c16, w);
+              st_global_v8(drow + 64 * h + 16 * c16, x);
             }
           } else {
 #pragma unroll
             for (int c8 = 0; c8 < 8; ++c8) {
-              uint32_t w[4];
+              uint32_t x[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                w[e] = pack2<BF>(__uint_as_float(o[8 * c8 + 2 * e]),
+                x[e] = pack2<BF>(__uint_as_float(o[8 * c8 + 2 * e]),
                                  __uint_as_float(o[8 * c8 + 2 * e + 1]));
-              *reinterpret_cast<uint4*>(drow + 64 * h + 8 * c8) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4*>(drow + 64 * h + 8 * c8) = make_uint4(x[0], x[1], x[2], x[3]);
             }
           }
         }
+        tc_fence_before();  // O has been read before the next item's P is told
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_item_free + 8 * (i & 1));
     }
   }
 
@@ -631,8 +754,13 @@ sam3_status_t launch_packed(sam3_ctx_t* ctx, const uint16_t* q, int64_t q_stride
   const long long tiles = a.rows / span + std::min(a.n_seqs, a.rows);
   if (tiles * a.units > 0x7FFFFFFFll)
     return set_error(ctx, SAM3_ERR_SHAPE, "attention_packed: too many rows for one call");
-  const cudaError_t e = launch_pdl(packed_attn_kernel<D, BF>, dim3((unsigned)(tiles * a.units)),
-                                   dim3(C::THREADS), C::SMEM, ctx->stream, mq, mk, mv, a);
+  // 128: one CTA per SM stays and takes items in turn, the next item's loads and
+  // first MMAs under this one's last tiles. 64: a CTA per item; the other CTA of
+  // the SM covers its begin and end.
+  const long long items = tiles * a.units;
+  const unsigned grid = (unsigned)(D == 128 ? std::min<long long>(items, ctx->num_sms) : items);
+  const cudaError_t e = launch_pdl(packed_attn_kernel<D, BF>, dim3(grid), dim3(C::THREADS), C::SMEM,
+                                   ctx->stream, mq, mk, mv, a);
   return check_launch_ret(ctx, e, "packed_attn_kernel");
 }
 
