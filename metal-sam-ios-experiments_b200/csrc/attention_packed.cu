@@ -42,22 +42,26 @@ namespace sam3 {
 namespace {
 
 constexpr int BQ = 128, BKV = 128;
-constexpr int KST = 3, VST = 2;
+constexpr int VST = 2;
 
 template <int D>
 struct PK {
   static constexpr int T = D == 128 ? 2 : 1;     // query tiles per CTA
   static constexpr bool OVERLAY = D == 128;      // P in its S's columns
   static constexpr int HALVES = D / 64;          // 128-byte wide parts of a tile
-  static constexpr int THREADS = 64 + 128 * T;
+  static constexpr bool ONE = D == 64;           // a CTA takes one item, else items in turn
+  static constexpr bool CHECKER = D == 128;      // warps 10 and 11 look through V
+  static constexpr int THREADS = 64 + 128 * T + (CHECKER ? 64 : 0);
+  static constexpr int KST = D == 128 ? 2 : 3;   // K tiles in shared memory
   static constexpr int TILE = BKV * D * 2;       // bytes of a Q, K or V tile
   static constexpr int HALF = BKV * 128;
   static constexpr int OFF_K = T * TILE;
   static constexpr int OFF_V = OFF_K + KST * TILE;
-  static constexpr int OFF_BAR = OFF_V + VST * TILE;
-  static constexpr int BARS = 4 * T + 2 * KST + 2 * VST + 9;
+  static constexpr int OFF_OUT = OFF_V + VST * TILE;  // [T] 128 rows of 64 outputs
+  static constexpr int OFF_BAR = OFF_OUT + (T == 2 ? T * HALF : 0);
+  static constexpr int BARS = 4 * T + 2 * KST + 2 * VST + 10;
   static constexpr int OFF_MISC = (OFF_BAR + BARS * 8 + 15) / 16 * 16;
-  static constexpr int MISC = 128;
+  static constexpr int MISC = 160;
   static constexpr int SMEM = OFF_MISC + MISC + 1024;
   static constexpr uint32_t COLS = D == 128 ? 512 : 256;
   static constexpr uint32_t S(int t) { return 128u * t; }
@@ -246,7 +250,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
                        const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const PackedArgs a) {
   using C = PK<D>;
-  constexpr int T = C::T;
+  constexpr int T = C::T, KST = C::KST;
   constexpr uint32_t FMT = BF ? (1u << 7) | (1u << 10) : 0u;  // bf16 operands
   constexpr uint32_t IDESC_S = umma_idesc_f16(128, BKV, 0) | FMT;
   constexpr uint32_t IDESC_O = umma_idesc_f16(128, D, 1) | FMT;
@@ -270,12 +274,16 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
   const uint32_t bar_o_full = bar_p_full + 8 * T;    // P V done (P apart)
   const uint32_t bar_o_done = bar_o_full + 8;        // [T] after an item's last P V
   const uint32_t bar_drain = bar_o_done + 8 * T;
+  const uint32_t bar_raw_free = bar_drain + 8;       // warps 10 and 11 may take the next
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
   // [2] items; of each the V tiles looked through and the rows with infinities
   Item* items = reinterpret_cast<Item*>(smem + C::OFF_MISC + 16);
   int* fix_tile = reinterpret_cast<int*>(smem + C::OFF_MISC + 48);            // [2][2]
   uint32_t* fix_rows = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC + 64);  // [2][2][4]
+  // the V tile to look through: stage (-1: no more), rows of the sequence in it,
+  // whether some query sees a part of it only, its place in fix_tile, its number
+  volatile int* raw = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 128);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -301,6 +309,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
     mbar_init(bar_s_free, 128);
     mbar_init(bar_o_full, 1);
     mbar_init(bar_drain, 1);
+    mbar_init(bar_raw_free, 1);
     *abort_flag = 0;
     fence_mbar_init();
     prefetch_tmap(&map_q);
@@ -318,6 +327,36 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
   griddep_launch_dependents();  // behind the allocation: the next kernel allocates too
   griddep_wait();  // offsets and rows may be earlier kernels' outputs
 
+  // Looks through a V tile before the MMA reads it (by `threads` threads of one or
+  // two warps, `id` among them): rows behind the sequence's end become 0, and so
+  // do infinities and NaN on the diagonal, whose rows are noted.
+  auto look_through = [&](int st, int held, bool diag, int nth, int id, int threads) {
+    uint4* vt = reinterpret_cast<uint4*>(smem + C::OFF_V + st * C::TILE);
+    for (int e = id; e < C::TILE / 16; e += threads)
+      if (((e >> 3) & (BKV - 1)) >= held) vt[e] = make_uint4(0, 0, 0, 0);
+    if (diag) {
+      bool found = false;
+#pragma unroll 8
+      for (int e = id; e < C::TILE / 16; e += threads) {
+        const uint4 x = vt[e];
+        found |= (not_finite<BF>(x.x) | not_finite<BF>(x.y) | not_finite<BF>(x.z) |
+                  not_finite<BF>(x.w)) != 0;
+      }
+      if (found)
+        for (int e = id; e < C::TILE / 16; e += threads) {
+          const int r = (e >> 3) & (BKV - 1);
+          const uint4 x = vt[e];
+          const uint4 b = make_uint4(not_finite<BF>(x.x), not_finite<BF>(x.y), not_finite<BF>(x.z),
+                                     not_finite<BF>(x.w));
+          if (b.x | b.y | b.z | b.w) {
+            vt[e] = make_uint4(x.x & ~b.x, x.y & ~b.y, x.z & ~b.z, x.w & ~b.w);
+            atomicOr(&fix_rows[nth * 4 + (r >> 5)], 1u << (r & 31));
+          }
+        }
+    }
+    fence_proxy_async_smem();
+  };
+
   if (warp == 0) {
     // ----------------------------------------------------------- producer
     Finder finder;
@@ -327,7 +366,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
     Ring<KST> rk;
     Ring<VST> rv;
     bool ok = true;
-    for (uint32_t i = 0; ok; ++i) {
+    for (uint32_t i = 0; ok && !(C::ONE && i); ++i) {
       // the rounds over the tiles go to and fro, so that no CTA always gets the
       // longer ones
       const int number = (int)(i * gridDim.x + (i & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x));
@@ -375,6 +414,15 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
             ok = mbar_wait(bar_v_empty + 8 * rv.st, rv.ph ^ 1, abort_flag, a.err,
                            kDevErrTimeoutPacked);
           }
+          if (ok && fix) {
+            if (C::CHECKER)
+              ok = mbar_wait(bar_raw_free, (raw_uses & 1u) ^ 1, abort_flag, a.err,
+                             kDevErrTimeoutPacked);
+            raw[0] = rv.st;
+            raw[1] = w.len - j * BKV;
+            raw[2] = diag | (slot * 2 + fixes) << 1;  // at most two such tiles per item
+            raw[3] = j;
+          }
           if (ok) {
             const uint32_t bar = fix ? bar_v_raw : bar_v_full + 8 * rv.st;
             mbar_arrive_expect_tx(bar, C::TILE);
@@ -390,43 +438,33 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
         }
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
         if (ok && fix) {
-          // drained here also on abort: the wait ignores the flag
-          ok = __all_sync(0xffffffffu, mbar_wait_drain(bar_v_raw, raw_uses & 1u));
-          if (!ok && lane == 0) {
-            *abort_flag = 1;
-            atomicExch(a.err, kDevErrTimeoutPacked);
-          }
           ++raw_uses;
-          const int nth = slot * 2 + fixes;  // at most two such tiles per item
-          ++fixes;
-          if (lane == 0) fix_tile[nth] = j;
-          __syncwarp();
-          uint4* vt = reinterpret_cast<uint4*>(smem + C::OFF_V + rv.st * C::TILE);
-          const int held = w.len - j * BKV;  // rows of the sequence in this tile
-#pragma unroll 8
-          for (int e = lane; e < C::TILE / 16; e += 32) {
-            const int r = (e >> 3) & (BKV - 1);
-            if (r >= held) {
-              vt[e] = make_uint4(0, 0, 0, 0);
-            } else if (diag) {
-              const uint4 x = vt[e];
-              const uint4 b = make_uint4(not_finite<BF>(x.x), not_finite<BF>(x.y),
-                                         not_finite<BF>(x.z), not_finite<BF>(x.w));
-              if (b.x | b.y | b.z | b.w) {
-                vt[e] = make_uint4(x.x & ~b.x, x.y & ~b.y, x.z & ~b.z, x.w & ~b.w);
-                atomicOr(&fix_rows[nth * 4 + (r >> 5)], 1u << (r & 31));
-              }
+          if (!C::CHECKER) {
+            // drained here also on abort: the wait ignores the flag
+            ok = __all_sync(0xffffffffu, mbar_wait_drain(bar_v_raw, (raw_uses - 1) & 1u));
+            if (!ok && lane == 0) {
+              *abort_flag = 1;
+              atomicExch(a.err, kDevErrTimeoutPacked);
             }
+            if (lane == 0) fix_tile[slot * 2 + fixes] = j;
+            __syncwarp();
+            look_through(rv.st, w.len - j * BKV, diag, slot * 2 + fixes, lane, 32);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_v_full + 8 * rv.st);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar_v_full + 8 * rv.st);
+          ++fixes;
         }
         rk.step();
         rv.step();
       }
     }
+    if (C::CHECKER && ok && lane == 0 &&
+        mbar_wait(bar_raw_free, (raw_uses & 1u) ^ 1, abort_flag, a.err, kDevErrTimeoutPacked)) {
+      raw[0] = -1;  // warps 10 and 11 may go
+      mbar_arrive(bar_v_raw);
+    }
     if (lane == 0 && *abort_flag) {
+      if (C::CHECKER && raw_uses) mbar_wait_drain(bar_v_raw, (raw_uses - 1) & 1u);
       for (int t = 0; t < T; ++t)
         if (q_par) mbar_wait_drain(bar_q + 8 * t, (q_par - 1) & 1u);
       for (int s = 0; s < KST; ++s)
@@ -445,7 +483,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
       Ring<VST> rv;   // of the next P V
       uint32_t n_p[2] = {0, 0};  // P tiles waited for
       uint32_t n_s = 0;          // S tiles issued (P apart)
-      for (uint32_t i = 0; ok; ++i) {
+      for (uint32_t i = 0; ok && !(C::ONE && i); ++i) {
         ok = wait(bar_item + 8 * (i & 1), i >> 1 & 1);
         if (!ok) break;
         const Item it = items[i & 1];
@@ -500,19 +538,18 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
 #pragma unroll
             for (int t = 0; t < T; ++t) {
               if (j >= w.n[t] || !ok) continue;
-              ok = wait(bar_p_full + 8 * t, n_p[t]++ & 1u) &&
-                   (v_here || wait(bar_v_full + 8 * rv.st, rv.ph));
-              if (!ok) continue;
+              // V and the next K are early as a rule: their waits come first, so that
+              // nothing stands between P and its MMAs
+              const bool more = j + 1 < w.n[t];
+              ok = (v_here || wait(bar_v_full + 8 * rv.st, rv.ph)) &&
+                   (!more || k_here || wait(bar_k_full + 8 * rk.st, rk.ph));
               v_here = true;
+              k_here |= more;
+              ok = ok && wait(bar_p_full + 8 * t, n_p[t]++ & 1u);
+              if (!ok) continue;
               tc_fence_after();
               issue_pv(t, j);
-              if (j + 1 < w.n[t]) {
-                ok = k_here || wait(bar_k_full + 8 * rk.st, rk.ph);
-                if (!ok) continue;
-                k_here = true;
-                tc_fence_after();
-                issue_qk(t, j + 1);
-              }
+              if (more) issue_qk(t, j + 1);
             }
           }
         } else {
@@ -540,6 +577,26 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
         mbar_wait_drain(bar_drain, 0);
       }
     }
+  } else if (C::CHECKER && warp >= 2 + 4 * T) {
+    // ----------------------------------------------------------- V tiles
+    const int id = threadIdx.x - 32 * (2 + 4 * T);
+    for (uint32_t u = 0;; ++u) {
+      const bool there = __all_sync(
+          0xffffffffu, mbar_wait(bar_v_raw, u & 1u, abort_flag, a.err, kDevErrTimeoutPacked));
+      if (id == 0) raw[4] = there;  // one decision for both warps
+      asm volatile("barrier.cta.sync 3, 64;" ::: "memory");
+      const int st = raw[0], held = raw[1], flags = raw[2], j = raw[3];
+      const bool go = raw[4] && st >= 0;
+      asm volatile("barrier.cta.sync 3, 64;" ::: "memory");
+      if (!go) break;
+      if (id == 0) fix_tile[flags >> 1] = j;
+      look_through(st, held, flags & 1, flags >> 1, id, 64);
+      asm volatile("barrier.cta.sync 3, 64;" ::: "memory");
+      if (id == 0) {
+        mbar_arrive(bar_v_full + 8 * st);
+        mbar_arrive(bar_raw_free);
+      }
+    }
   } else {
     // ----------------------------------------------------------- softmax rows
     constexpr float kRescaleLog2 = 8.0f;
@@ -553,20 +610,30 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
     auto wait = [&](uint32_t bar, uint32_t par) {
       return __all_sync(0xffffffffu, mbar_wait(bar, par, abort_flag, a.err, kDevErrTimeoutPacked));
     };
+    uint8_t* out = smem + C::OFF_OUT + t * C::HALF;
     uint32_t tiles = 0, outs = 0;  // key tiles and items of this query tile so far
-    for (uint32_t i = 0;; ++i) {
+    for (uint32_t i = 0; !(C::ONE && i); ++i) {
       if (!wait(bar_item + 8 * (i & 1), i >> 1 & 1)) break;
-      const Item it = items[i & 1];
-      if (it.tile < 0) break;
-      const Work w = work_of<T>(a, it);
-      const int n = T == 2 && t ? w.n[1] : w.n[0], q0 = T == 2 && t ? w.qt[1] : w.qt[0];
-      const int len = w.len;
-      const int pos = q0 + r;                              // row in the sequence
-      const int lim = a.causal ? min(len, pos + 1) : len;  // keys it sees
-      const int lim_min = a.causal ? min(len, q0 + 1) : len;  // that all rows of the tile see
+      // What the key loop needs of the item and no more: its registers are scarce.
+      // The item is read again for its end.
+      auto item = [&]() {
+        const volatile Item& s = items[i & 1];
+        return Item{s.row0, s.len, s.tile, s.unit};
+      };
+      int n, lim, lim_min;
+      {
+        const Item it = item();
+        if (it.tile < 0) break;
+        const Work w = work_of<T>(a, it);
+        const int q0 = T == 2 && t ? w.qt[1] : w.qt[0];
+        n = T == 2 && t ? w.n[1] : w.n[0];
+        lim = a.causal ? min(w.len, q0 + r + 1) : w.len;    // keys that the row sees
+        lim_min = a.causal ? min(w.len, q0 + 1) : w.len;    // that all rows of the tile see
+      }
       float m_run = -INFINITY, l_run = 0.f;
       bool ok = true;
       for (int j = 0; j < n; ++j, ++tiles) {
+        if (C::ONE) tiles = j;
         ok = wait(bar_s_full + 8 * t, tiles & 1u);
         if (!ok) break;
         tc_fence_after();
@@ -614,42 +681,46 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
           ls[e & 3] += p0 + p1;
           pk[e] = pack2<BF>(p0, p1);
         }
+        // tcgen05.ld/st are warp-wide: the whole warp takes the branch when any
+        // of its rows grew (alpha is 1 for the others)
+        auto rescale = [&]() {
+          if (j > 0 && __any_sync(0xffffffffu, grow)) {
+#pragma unroll
+            for (int h = 0; h < D / 32; ++h) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(o_col + 32 * h, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int d = 0; d < 32; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * alpha);
+#pragma unroll
+              for (int q = 0; q < 2; ++q)
+                tmem_st_32x32b_x16(o_col + 32 * h + q * 16,
+                                   *reinterpret_cast<uint32_t(*)[16]>(o + 16 * q));
+            }
+          }
+        };
         if (!C::OVERLAY && tiles > 0) {  // P V of the tile before still reads P
           ok = wait(bar_o_full, (tiles - 1) & 1u);
           if (!ok) break;
           tc_fence_after();
         }
 #pragma unroll
-        for (int q = 0; q < BKV / 32; ++q)
+        for (int q = 0; q < 4; ++q)
           tmem_st_32x32b_x16(p_col + q * 16, *reinterpret_cast<uint32_t(*)[16]>(pk + 16 * q));
-        l_run = fmaf(l_run, alpha, (ls[0] + ls[1]) + (ls[2] + ls[3]));
-        m_run = m_use;
-        // tcgen05.ld/st are warp-wide: the whole warp takes the branch when any
-        // of its rows grew (alpha is 1 for the others)
-        if (j > 0 && __any_sync(0xffffffffu, grow)) {
-#pragma unroll
-          for (int h = 0; h < C::HALVES; ++h) {
-            uint32_t o[64];
-            tmem_ld_32x32b_x32(o_col + 64 * h, *reinterpret_cast<uint32_t(*)[32]>(o));
-            tmem_ld_32x32b_x32(o_col + 64 * h + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
-            tmem_wait_ld();
-#pragma unroll
-            for (int d = 0; d < 64; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * alpha);
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              tmem_st_32x32b_x16(o_col + 64 * h + q * 16,
-                                 *reinterpret_cast<uint32_t(*)[16]>(o + 16 * q));
-          }
-        }
+        rescale();
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(bar_p_full + 8 * t);
+        l_run = fmaf(l_run, alpha, (ls[0] + ls[1]) + (ls[2] + ls[3]));
+        m_run = m_use;
       }
       if (!ok) break;
       if (n) {
         if (!wait(bar_o_done + 8 * t, outs++ & 1u)) break;
         tc_fence_after();
         const float inv = 1.f / l_run;
+        const Work w = work_of<T>(a, item());
+        const int q0 = T == 2 && t ? w.qt[1] : w.qt[0], pos = q0 + r, len = w.len;
         const int head = w.ph ? w.head0 + t : w.head0;
         uint16_t* drow = a.o + (int64_t)(w.row0 + pos) * a.o_stride + head * D;
 #pragma unroll
@@ -658,7 +729,6 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
           tmem_ld_32x32b_x32(o_col + 64 * h, *reinterpret_cast<uint32_t(*)[32]>(o));
           tmem_ld_32x32b_x32(o_col + 64 * h + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
           tmem_wait_ld();
-          if (pos >= len) continue;
 #pragma unroll
           for (int d = 0; d < 64; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * inv);
           // infinities and NaN that warp 0 took out of the diagonal V tiles
@@ -680,25 +750,38 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
               }
             }
           }
-          if (a.o32) {  // 32-byte stores: whole sectors
+          uint32_t x[32];
 #pragma unroll
-            for (int c16 = 0; c16 < 4; ++c16) {
-              uint32_t x[8];
+          for (int e = 0; e < 32; ++e)
+            x[e] = pack2<BF>(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
+          if (C::T == 2) {
+            // Through shared memory (the warp's own 32 rows, 16-byte groups swizzled
+            // by row), so that a store of the warp is four whole 128-byte lines and
+            // not parts of 32.
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                x[e] = pack2<BF>(__uint_as_float(o[16 * c16 + 2 * e]),
-                                 __uint_as_float(o[16 * c16 + 2 * e + 1]));
-              st_global_v8(drow + 64 * h + 16 * c16, x);
+            for (int c8 = 0; c8 < 8; ++c8)
+              *reinterpret_cast<uint4*>(out + r * 128 + ((c8 ^ (r & 7)) << 4)) =
+                  make_uint4(x[4 * c8], x[4 * c8 + 1], x[4 * c8 + 2], x[4 * c8 + 3]);
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int rr = quad * 32 + k * 4 + lane / 8, c8 = lane & 7;
+              if (q0 + rr < len)
+                *reinterpret_cast<uint4*>(a.o + (int64_t)(w.row0 + q0 + rr) * a.o_stride +
+                                          head * D + 64 * h + 8 * c8) =
+                    *reinterpret_cast<const uint4*>(out + rr * 128 + ((c8 ^ (rr & 7)) << 4));
             }
-          } else {
+            __syncwarp();
+          } else if (pos < len) {
+            if (a.o32) {  // 32-byte stores: whole sectors
 #pragma unroll
-            for (int c8 = 0; c8 < 8; ++c8) {
-              uint32_t x[4];
+              for (int c16 = 0; c16 < 4; ++c16)
+                st_global_v8(drow + 16 * c16, *reinterpret_cast<uint32_t(*)[8]>(x + 8 * c16));
+            } else {
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                x[e] = pack2<BF>(__uint_as_float(o[8 * c8 + 2 * e]),
-                                 __uint_as_float(o[8 * c8 + 2 * e + 1]));
-              *reinterpret_cast<uint4*>(drow + 64 * h + 8 * c8) = make_uint4(x[0], x[1], x[2], x[3]);
+              for (int c8 = 0; c8 < 8; ++c8)
+                *reinterpret_cast<uint4*>(drow + 8 * c8) =
+                    make_uint4(x[4 * c8], x[4 * c8 + 1], x[4 * c8 + 2], x[4 * c8 + 3]);
             }
           }
         }
@@ -758,7 +841,7 @@ sam3_status_t launch_packed(sam3_ctx_t* ctx, const uint16_t* q, int64_t q_stride
   // first MMAs under this one's last tiles. 64: a CTA per item; the other CTA of
   // the SM covers its begin and end.
   const long long items = tiles * a.units;
-  const unsigned grid = (unsigned)(D == 128 ? std::min<long long>(items, ctx->num_sms) : items);
+  const unsigned grid = (unsigned)(C::ONE ? items : std::min<long long>(items, ctx->num_sms));
   const cudaError_t e = launch_pdl(packed_attn_kernel<D, BF>, dim3(grid), dim3(C::THREADS), C::SMEM,
                                    ctx->stream, mq, mk, mv, a);
   return check_launch_ret(ctx, e, "packed_attn_kernel");
