@@ -83,7 +83,6 @@ struct PackedArgs {
   int units;       // heads, or pairs of heads
   int causal;
   float c;         // scale * log2(e)
-  int o32;         // o's rows are 32-byte aligned
 };
 
 struct Item {
@@ -248,7 +247,8 @@ template <int D, bool BF>
 __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
     packed_attn_kernel(const __grid_constant__ CUtensorMap map_q,
                        const __grid_constant__ CUtensorMap map_k,
-                       const __grid_constant__ CUtensorMap map_v, const PackedArgs a) {
+                       const __grid_constant__ CUtensorMap map_v,
+                       const __grid_constant__ CUtensorMap map_o, const PackedArgs a) {
   using C = PK<D>;
   constexpr int T = C::T, KST = C::KST;
   constexpr uint32_t FMT = BF ? (1u << 7) | (1u << 10) : 0u;  // bf16 operands
@@ -315,6 +315,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
     prefetch_tmap(&map_q);
     prefetch_tmap(&map_k);
     prefetch_tmap(&map_v);
+    prefetch_tmap(&map_o);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), C::COLS);
@@ -610,7 +611,8 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
     auto wait = [&](uint32_t bar, uint32_t par) {
       return __all_sync(0xffffffffu, mbar_wait(bar, par, abort_flag, a.err, kDevErrTimeoutPacked));
     };
-    uint8_t* out = smem + C::OFF_OUT + t * C::HALF;
+    // this warp's rows of 64 outputs (head_dim 64: in the queries' place)
+    uint8_t* out = smem + (T == 2 ? C::OFF_OUT + t * C::HALF : 0) + quad * 4096;
     uint32_t tiles = 0, outs = 0;  // key tiles and items of this query tile so far
     for (uint32_t i = 0; !(C::ONE && i); ++i) {
       if (!wait(bar_item + 8 * (i & 1), i >> 1 & 1)) break;
@@ -722,8 +724,12 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
         const Work w = work_of<T>(a, item());
         const int q0 = T == 2 && t ? w.qt[1] : w.qt[0], pos = q0 + r, len = w.len;
         const int head = w.ph ? w.head0 + t : w.head0;
-        uint16_t* drow = a.o + (int64_t)(w.row0 + pos) * a.o_stride + head * D;
+        uint32_t fixes = 0;
 #pragma unroll
+        for (int f = 0; f < 8; ++f) fixes |= fix_rows[(i & 1) * 8 + f];
+        // (Not unrolled: this runs once per item, and fetching its code is what it
+        // costs.)
+#pragma unroll 1
         for (int h = 0; h < C::HALVES; ++h) {
           uint32_t o[64];
           tmem_ld_32x32b_x32(o_col + 64 * h, *reinterpret_cast<uint32_t(*)[32]>(o));
@@ -732,7 +738,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
 #pragma unroll
           for (int d = 0; d < 64; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * inv);
           // infinities and NaN that warp 0 took out of the diagonal V tiles
-          for (int f = 0; f < 8; ++f) {
+          for (int f = 0; f < 8 && __builtin_expect(fixes != 0, 0); ++f) {
             uint32_t bits = fix_rows[(i & 1) * 8 + f];
             while (bits) {
               const int key =
@@ -754,35 +760,33 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             x[e] = pack2<BF>(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1]));
+          // Through shared memory (the warp's own 32 rows, 128-byte swizzle): one
+          // TMA store takes them, and nobody waits for it. Where the sequence ends
+          // among the rows, lanes store what is there, four whole lines at a time.
           if (C::T == 2) {
-            // Through shared memory (the warp's own 32 rows, 16-byte groups swizzled
-            // by row), so that a store of the warp is four whole 128-byte lines and
-            // not parts of 32.
-#pragma unroll
-            for (int c8 = 0; c8 < 8; ++c8)
-              *reinterpret_cast<uint4*>(out + r * 128 + ((c8 ^ (r & 7)) << 4)) =
-                  make_uint4(x[4 * c8], x[4 * c8 + 1], x[4 * c8 + 2], x[4 * c8 + 3]);
+            if (lane == 0) bulk_wait_read();  // the store before has read the buffer
             __syncwarp();
+          }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const int rr = quad * 32 + k * 4 + lane / 8, c8 = lane & 7;
-              if (q0 + rr < len)
-                *reinterpret_cast<uint4*>(a.o + (int64_t)(w.row0 + q0 + rr) * a.o_stride +
-                                          head * D + 64 * h + 8 * c8) =
-                    *reinterpret_cast<const uint4*>(out + rr * 128 + ((c8 ^ (rr & 7)) << 4));
-            }
+          for (int c8 = 0; c8 < 8; ++c8)
+            *reinterpret_cast<uint4*>(out + lane * 128 + ((c8 ^ (lane & 7)) << 4)) =
+                make_uint4(x[4 * c8], x[4 * c8 + 1], x[4 * c8 + 2], x[4 * c8 + 3]);
+          if (q0 + quad * 32 + 32 <= len) {
+            fence_proxy_async_smem();
             __syncwarp();
-          } else if (pos < len) {
-            if (a.o32) {  // 32-byte stores: whole sectors
-#pragma unroll
-              for (int c16 = 0; c16 < 4; ++c16)
-                st_global_v8(drow + 16 * c16, *reinterpret_cast<uint32_t(*)[8]>(x + 8 * c16));
-            } else {
-#pragma unroll
-              for (int c8 = 0; c8 < 8; ++c8)
-                *reinterpret_cast<uint4*>(drow + 8 * c8) =
-                    make_uint4(x[4 * c8], x[4 * c8 + 1], x[4 * c8 + 2], x[4 * c8 + 3]);
+            if (lane == 0) {
+              tma_store_3d(&map_o, smem_u32(out), 0, w.row0 + q0 + quad * 32,
+                           head * C::HALVES + h);
+              bulk_commit();
             }
+          } else {
+            __syncwarp();
+#pragma unroll 1
+            for (int rr = lane / 8; rr < 32 && q0 + quad * 32 + rr < len; rr += 4)
+              *reinterpret_cast<uint4*>(a.o + (int64_t)(w.row0 + q0 + quad * 32 + rr) * a.o_stride +
+                                        head * D + 64 * h + 8 * (lane & 7)) =
+                  *reinterpret_cast<const uint4*>(out + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+            __syncwarp();
           }
         }
         tc_fence_before();  // O has been read before the next item's P is told
@@ -790,6 +794,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_item_free + 8 * (i & 1));
     }
+    if (lane == 0) bulk_wait();
   }
 
   tc_fence_before();
@@ -800,13 +805,14 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
   }
 }
 
-// Rows [rows, heads * D] as (64, rows, heads * D / 64): one box brings 128 rows
-// of one head, its 64-wide parts one after another.
+// Rows [rows, heads * D] as (64, rows, heads * D / 64): one box holds some rows of
+// one head, its 64-wide parts one after another.
 template <int D>
-bool rows_map(CUtensorMap* map, const uint16_t* x, int rows, int heads, int64_t stride, bool bf) {
+bool rows_map(CUtensorMap* map, const uint16_t* x, int rows, int heads, int64_t stride, bool bf,
+              int box_rows, int box_parts) {
   cuuint64_t dims[3] = {64, (cuuint64_t)rows, (cuuint64_t)heads * (D / 64)};
   cuuint64_t strides[2] = {(cuuint64_t)stride * 2, 128};
-  cuuint32_t box[3] = {64, BKV, D / 64};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_rows, (cuuint32_t)box_parts};
   cuuint32_t es[3] = {1, 1, 1};
   return encode_tiled()(map,
                         bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
@@ -821,10 +827,11 @@ sam3_status_t launch_packed(sam3_ctx_t* ctx, const uint16_t* q, int64_t q_stride
                             const uint16_t* k, int64_t k_stride, PackedArgs& a, int heads,
                             int kv_heads) {
   using C = PK<D>;
-  CUtensorMap mq, mk, mv;
-  if (!rows_map<D>(&mq, q, a.rows, heads, q_stride, BF) ||
-      !rows_map<D>(&mk, k, a.rows, kv_heads, k_stride, BF) ||
-      !rows_map<D>(&mv, a.v, a.rows, kv_heads, a.v_stride, BF))
+  CUtensorMap mq, mk, mv, mo;
+  if (!rows_map<D>(&mq, q, a.rows, heads, q_stride, BF, BQ, C::HALVES) ||
+      !rows_map<D>(&mk, k, a.rows, kv_heads, k_stride, BF, BKV, C::HALVES) ||
+      !rows_map<D>(&mv, a.v, a.rows, kv_heads, a.v_stride, BF, BKV, C::HALVES) ||
+      !rows_map<D>(&mo, a.o, a.rows, heads, a.o_stride, BF, 32, 1))
     return set_error(ctx, SAM3_ERR_CUDA, "attention_packed: cuTensorMapEncodeTiled failed");
   const uint32_t bit = (uint32_t)kSmemPacked << ((D == 128) * 2 + BF);
   const sam3_status_t st = ensure_smem_attr(ctx, bit, packed_attn_kernel<D, BF>, C::SMEM,
@@ -843,7 +850,7 @@ sam3_status_t launch_packed(sam3_ctx_t* ctx, const uint16_t* q, int64_t q_stride
   const long long items = tiles * a.units;
   const unsigned grid = (unsigned)(C::ONE ? items : std::min<long long>(items, ctx->num_sms));
   const cudaError_t e = launch_pdl(packed_attn_kernel<D, BF>, dim3(grid), dim3(C::THREADS), C::SMEM,
-                                   ctx->stream, mq, mk, mv, a);
+                                   ctx->stream, mq, mk, mv, mo, a);
   return check_launch_ret(ctx, e, "packed_attn_kernel");
 }
 
@@ -887,7 +894,6 @@ sam3_status_t attention_packed(sam3_ctx_t* ctx, int dtype, const uint16_t* q, in
   a.group = heads / kv_heads;
   a.causal = causal != 0;
   a.c = scale * 1.4426950408889634f;
-  a.o32 = (reinterpret_cast<uintptr_t>(o) & 31u) == 0 && o_stride % 16 == 0;
   // lengths stay on the device: the work counted here is the rows read and written
   ProfScope prof(ctx, SAM3_PROF_ATTENTION, 0.0, 4.0 * rows * (wide + narrow));
   const bool bf = dtype == SAM3_BF16;
