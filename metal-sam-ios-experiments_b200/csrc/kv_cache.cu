@@ -40,6 +40,7 @@ struct AppendArgs {
   const int32_t* lens; // [n] tokens of each sequence with the new ones
   const int32_t* table;
   int table_stride, num_pages, kv_heads, page_shift, rows, max_new;
+  int groups;  // CTAs per page: its units over the units per CTA
   int* err;
 };
 
@@ -72,16 +73,18 @@ __device__ __forceinline__ float finite_abs(float x) {
   return a <= 3.402823466e38f ? a : 0.f;  // infinities and NaN set no scale
 }
 
-// UNIT_WARPS warps hold one unit, VEC vectors of 8 elements per lane. The
-// CTA's 8 warps take the units of consecutive (head, K or V) of one page, whose
-// rows are neighbours in the source.
-template <int D, int UNIT_WARPS, int VEC, bool BF>
-__global__ void __launch_bounds__(THREADS) kv_append_kernel(const AppendArgs a) {
-  constexpr int VPR = D / 8;  // vectors per token
+// UNIT_WARPS warps hold one unit, VEC vectors of 8 elements per lane; or one warp
+// UNITS of them one after another. The CTA's 8 warps take the units of
+// consecutive (head, K or V) of one page, whose rows are neighbours in the source.
+template <int D, int UNIT_WARPS, int UNITS, int VEC, bool BF>
+__global__ void __launch_bounds__(THREADS, 4) kv_append_kernel(const AppendArgs a) {
+  constexpr int VPR = D / 8;                     // vectors per token
+  constexpr int STEP = 32 * UNIT_WARPS / VPR;    // tokens between a lane's vectors
   __shared__ float warp_max[THREADS / 32];
   griddep_launch_dependents();
   griddep_wait();  // rows, lengths and pages may be earlier kernels' outputs
-  const int seq = blockIdx.z;
+  const int seq = blockIdx.y;
+  const int page_no = blockIdx.x / a.groups, group = blockIdx.x - page_no * a.groups;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int page = 1 << a.page_shift;
   const int len = a.lens[seq];
@@ -93,105 +96,113 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(const AppendArgs a) 
   }
   const int fresh = row1 - row0;
   const int start = len - fresh;  // position of the first new token
-  const int page_at = (start >> a.page_shift) + blockIdx.x;
+  const int page_at = (start >> a.page_shift) + page_no;
   if (fresh == 0 || page_at > (len - 1) >> a.page_shift) return;
   const int pos0 = page_at << a.page_shift;
   const int slot = a.table[(size_t)seq * a.table_stride + page_at];
+  const int held = max(0, start - pos0);   // tokens of the page that were there
+  const int last = min(page, len - pos0);  // tokens of the page now
+  // vector i of this lane: token tok0 + i * STEP of the page, the same part of it
+  const int v0 = (warp % UNIT_WARPS) * 32 + lane;
+  const int tok0 = v0 / VPR;
+  const int lo = held - tok0, hi = last - tok0;  // i * STEP of new tokens
+  const int unit0 = (group * (THREADS / 32 / UNIT_WARPS) + warp / UNIT_WARPS) * UNITS;
+  uint4 x[UNITS][VEC];
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) {
+    const int unit = unit0 + u;
+    const bool on = unit < 2 * a.kv_heads, is_v = unit >= a.kv_heads;
+    const int64_t stride = is_v ? a.v_stride : a.k_stride;
+    const uint16_t* src = (is_v ? a.v : a.k) + (unit - (is_v ? a.kv_heads : 0)) * D +
+                          (v0 % VPR) * 8 + ((int64_t)row0 + pos0 + tok0 - start) * stride;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      x[u][i] = make_uint4(0, 0, 0, 0);
+      if (on && i * STEP >= lo && i * STEP < hi) x[u][i] = *reinterpret_cast<const uint4*>(src);
+      src += STEP * stride;
+    }
+  }
+  // the page's number is first needed here: it travels with the rows
   if (!page_fits(slot, a.num_pages)) {
     if (threadIdx.x == 0) atomicExch(a.err, kDevErrBadPage);
     return;
   }
-  const int unit = blockIdx.y * (THREADS / 32 / UNIT_WARPS) + warp / UNIT_WARPS;
-  const bool on = unit < 2 * a.kv_heads;
-  const int which = on && unit >= a.kv_heads;
-  const int head = on ? unit - which * a.kv_heads : 0;
-  const int held = max(0, start - pos0);        // tokens of the page that were there
-  const int last = min(page, len - pos0);       // tokens of the page now
-  const int v0 = (warp % UNIT_WARPS) * 32 + lane;
-  const uint16_t* src = (which ? a.v : a.k) + head * D;
-  const int64_t stride = which ? a.v_stride : a.k_stride;
-  float* scale = (which ? a.v_scale : a.k_scale) + (size_t)slot * a.kv_heads + head;
-  uint4 x[VEC];
-  float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    const int v = v0 + i * 32 * UNIT_WARPS;
-    const int tok = v / VPR;
-    if (on && tok >= held && tok < last)
-      x[i] = *reinterpret_cast<const uint4*>(src + (row0 + pos0 + tok - start) * stride +
-                                             (v % VPR) * 8);
-    else
-      x[i] = make_uint4(0, 0, 0, 0);
-  }
+  for (int u = 0; u < UNITS; ++u) {
+    const int unit = unit0 + u;
+    const bool on = unit < 2 * a.kv_heads, is_v = unit >= a.kv_heads;
+    const size_t at = (size_t)slot * a.kv_heads + (on ? unit - (is_v ? a.kv_heads : 0) : 0);
+    float* scale = (is_v ? a.v_scale : a.k_scale) + at;
+    const int was = held > 0 && on ? __float_as_int(*scale) : 0;
+    float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float2 p = unpack2<BF>(w[q]);
-      top = fmaxf(top, fmaxf(finite_abs(p.x), finite_abs(p.y)));
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const int was = held > 0 && on ? __float_as_int(*scale) : 0;
-  if (UNIT_WARPS > 1) {
-    if (lane == 0) warp_max[warp] = top;
-    __syncthreads();  // also: every thread has read the old scale
-    const int first = warp / UNIT_WARPS * UNIT_WARPS;
-#pragma unroll
-    for (int i = 0; i < UNIT_WARPS; ++i) top = fmaxf(top, warp_max[first + i]);
-  } else {
-    __syncwarp();
-  }
-  if (!on) return;
-  int e = scale_exp(top);
-  const int e_was = min(max(((was >> 23) & 255) - 127, kScaleExpMin), kScaleExpMax);
-  if (held > 0) e = max(e, e_was);
-  const float inv = exp2_int(-e);
-  uint8_t* dst =
-      (which ? a.v_codes : a.k_codes) + (((size_t)slot * a.kv_heads + head) << a.page_shift) * D;
-  const bool grow = held > 0 && e > e_was;
-  const float shrink = exp2_int(max(e_was - e, -126));
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    const int v = v0 + i * 32 * UNIT_WARPS;
-    const int tok = v / VPR;
-    uint2* p = reinterpret_cast<uint2*>(dst + (size_t)v * 8);
-    if (tok >= held && tok < last) {
-      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-      uint32_t c[4];
+    for (int i = 0; i < VEC; ++i) {
+      const uint32_t w[4] = {x[u][i].x, x[u][i].y, x[u][i].z, x[u][i].w};
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float2 f = unpack2<BF>(w[q]);
-        c[q] = to_e4m3x2(f.x * inv, f.y * inv);
+        const float2 p = unpack2<BF>(w[q]);
+        top = fmaxf(top, fmaxf(finite_abs(p.x), finite_abs(p.y)));
       }
-      *p = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
-    } else if (grow && tok < held) {
-      const uint2 old = *p;
-      const uint32_t w[2] = {old.x, old.y};
-      uint32_t c[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float2 f = from_e4m3x2((uint16_t)(w[q >> 1] >> (16 * (q & 1))));
-        c[q] = to_e4m3x2(f.x * shrink, f.y * shrink);
-      }
-      *p = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
     }
+    // floats that are not negative compare like their bits
+    top = __int_as_float(__reduce_max_sync(0xffffffffu, __float_as_int(top)));
+    if (UNIT_WARPS > 1) {
+      if (lane == 0) warp_max[warp] = top;
+      __syncthreads();  // also: every thread has read the old scale
+      const int first = warp / UNIT_WARPS * UNIT_WARPS;
+#pragma unroll
+      for (int i = 0; i < UNIT_WARPS; ++i) top = fmaxf(top, warp_max[first + i]);
+    }
+    if (!on) return;
+    int e = scale_exp(top);
+    const int e_was = min(max(((was >> 23) & 255) - 127, kScaleExpMin), kScaleExpMax);
+    if (held > 0) e = max(e, e_was);
+    const float inv = exp2_int(-e);
+    uint8_t* dst = (is_v ? a.v_codes : a.k_codes) + (at << a.page_shift) * D + (size_t)v0 * 8;
+    const bool grow = held > 0 && e > e_was;
+    const float shrink = exp2_int(max(e_was - e, -126));
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      uint2* p = reinterpret_cast<uint2*>(dst + i * 32 * UNIT_WARPS * 8);
+      if (i * STEP >= lo && i * STEP < hi) {
+        const uint32_t w[4] = {x[u][i].x, x[u][i].y, x[u][i].z, x[u][i].w};
+        uint32_t c[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float2 f = unpack2<BF>(w[q]);
+          c[q] = to_e4m3x2(f.x * inv, f.y * inv);
+        }
+        *p = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+      } else if (grow && i * STEP < lo) {
+        const uint2 old = *p;
+        const uint32_t w[2] = {old.x, old.y};
+        uint32_t c[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float2 f = from_e4m3x2((uint16_t)(w[q >> 1] >> (16 * (q & 1))));
+          c[q] = to_e4m3x2(f.x * shrink, f.y * shrink);
+        }
+        *p = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+      }
+    }
+    __syncwarp();  // every lane has read the old scale
+    if (warp % UNIT_WARPS == 0 && lane == 0) *scale = exp2_int(e);
   }
-  if (warp % UNIT_WARPS == 0 && lane == 0) *scale = exp2_int(e);
 }
 
-template <int D, int UNIT_WARPS, int VEC>
-cudaError_t launch_append(sam3_ctx_t* ctx, bool bf, const AppendArgs& a, int n_seqs) {
-  const int per_cta = THREADS / 32 / UNIT_WARPS;
+template <int D, int UNIT_WARPS, int UNITS, int VEC>
+cudaError_t launch_append(sam3_ctx_t* ctx, bool bf, AppendArgs& a, int n_seqs) {
+  const int per_cta = THREADS / 32 / UNIT_WARPS * UNITS;
   // the most pages that max_new tokens can touch
-  const int pages = (a.max_new - 1 + (1 << a.page_shift) - 1) / (1 << a.page_shift) + 1;
-  const dim3 grid(pages, (2 * a.kv_heads + per_cta - 1) / per_cta, n_seqs);
+  const long long pages = ((long long)a.max_new - 1 + (1 << a.page_shift) - 1 >> a.page_shift) + 1;
+  // heads before pages: CTAs that run together read whole rows
+  a.groups = (2 * a.kv_heads + per_cta - 1) / per_cta;
+  if (pages * a.groups > 0x7FFFFFFFll) return cudaErrorInvalidConfiguration;
+  const dim3 grid((unsigned)(pages * a.groups), n_seqs);
   if (bf)
-    return launch_pdl(kv_append_kernel<D, UNIT_WARPS, VEC, true>, grid, dim3(THREADS), 0,
+    return launch_pdl(kv_append_kernel<D, UNIT_WARPS, UNITS, VEC, true>, grid, dim3(THREADS), 0,
                       ctx->stream, a);
-  return launch_pdl(kv_append_kernel<D, UNIT_WARPS, VEC, false>, grid, dim3(THREADS), 0,
+  return launch_pdl(kv_append_kernel<D, UNIT_WARPS, UNITS, VEC, false>, grid, dim3(THREADS), 0,
                     ctx->stream, a);
 }
 
@@ -259,23 +270,23 @@ sam3_status_t kv_append(sam3_ctx_t* ctx, const sam3_kv_cache_t* c, int dtype, co
   ProfScope prof(ctx, SAM3_PROF_OTHER, 0.0, 6.0 * rows * width);
   const bool bf = dtype == SAM3_BF16;
   cudaError_t e;
-  // A lane holds up to 64 elements (8 vectors), a unit as few warps as that
-  // allows, so that the vectors of one unit are in flight together.
+  // A lane holds 64 elements (8 vectors): a unit takes as many warps as that
+  // makes, or a warp two of the smallest units.
   switch (c->page_size * c->head_dim) {
-    case 16 * 64: e = launch_append<64, 1, 4>(ctx, bf, a, n_seqs); break;
+    case 16 * 64: e = launch_append<64, 1, 2, 4>(ctx, bf, a, n_seqs); break;
     case 32 * 64:
-      e = c->head_dim == 64 ? launch_append<64, 1, 8>(ctx, bf, a, n_seqs)
-                            : launch_append<128, 1, 8>(ctx, bf, a, n_seqs);
+      e = c->head_dim == 64 ? launch_append<64, 1, 1, 8>(ctx, bf, a, n_seqs)
+                            : launch_append<128, 1, 1, 8>(ctx, bf, a, n_seqs);
       break;
     case 64 * 64:
-      e = c->head_dim == 64 ? launch_append<64, 2, 8>(ctx, bf, a, n_seqs)
-                            : launch_append<128, 2, 8>(ctx, bf, a, n_seqs);
+      e = c->head_dim == 64 ? launch_append<64, 2, 1, 8>(ctx, bf, a, n_seqs)
+                            : launch_append<128, 2, 1, 8>(ctx, bf, a, n_seqs);
       break;
     case 128 * 64:
-      e = c->head_dim == 64 ? launch_append<64, 4, 8>(ctx, bf, a, n_seqs)
-                            : launch_append<128, 4, 8>(ctx, bf, a, n_seqs);
+      e = c->head_dim == 64 ? launch_append<64, 4, 1, 8>(ctx, bf, a, n_seqs)
+                            : launch_append<128, 4, 1, 8>(ctx, bf, a, n_seqs);
       break;
-    default: e = launch_append<128, 8, 8>(ctx, bf, a, n_seqs); break;
+    default: e = launch_append<128, 8, 1, 8>(ctx, bf, a, n_seqs); break;
   }
   return check_launch_ret(ctx, e, "kv_append_kernel");
 }
