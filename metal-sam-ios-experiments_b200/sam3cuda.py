@@ -172,13 +172,12 @@ class SAM3Error(RuntimeError):
 
 def ptr(x):
     """Device address of a DeviceBuffer / tensor-like / int; None stays None."""
-    if x is None:
-        return None
-    if isinstance(x, DeviceBuffer):
-        return x.ptr
-    if hasattr(x, "data_ptr"):
+    if x is None or type(x) is int:
+        return x
+    try:
         return x.data_ptr()
-    return int(x)
+    except AttributeError:
+        return x.ptr if isinstance(x, DeviceBuffer) else int(x)
 
 
 def default_config(**overrides) -> EncoderConfig:
