@@ -309,8 +309,8 @@ sam3_status_t sam3_kv_append(sam3_ctx_t* ctx, const sam3_kv_cache_t* cache, int3
  * its tokens in the cache, the newest among them (sam3_kv_append comes first,
  * with the same cu_new, max_new, page_table and seq_lens). With causal != 0 a
  * new token sees the tokens up to itself, else all of its sequence. Made for
- * one or a few new tokens per sequence: up to 64 query rows (new tokens times
- * heads per K/V head) read the cache once, more read it again for each 64.
+ * one or a few new tokens per sequence: up to 16 query rows (new tokens times
+ * heads per K/V head) read the cache once, more read it again for each 16.
  * Sequences may share pages. n_seqs <= SAM3_CACHED_MAX_SEQS. */
 sam3_status_t sam3_attention_cached(sam3_ctx_t* ctx, const sam3_kv_cache_t* cache, int32_t dtype,
                                     const uint16_t* q, int64_t q_stride, const int32_t* cu_new,

@@ -106,11 +106,11 @@ sam3_status_t device_error_status(sam3_ctx_t* ctx, int err);
 enum : uint32_t {
   kSmemAttn = 1u, kSmemWs = 2u, kSmemWsc = 4u, kSmemGemm = 8u /* << MODE */, kSmemPrune = 64u,
   kSmemAttnPP = 128u, kSmemPacked = 256u /* << variant, 4 of them */,
-  kSmemCached = 4096u /* << variant, 16 of them */
+  kSmemCached = 4096u /* << variant, 12 of them */
 };
-// One piece: 32 rows of up to 128 unnormalised outputs, then their 32 running
-// maxima and 32 row sums.
-constexpr int kCachedPartRows = 32;
+// One piece: 16 rows of up to 128 unnormalised outputs, then their 16 running
+// maxima and 16 row sums.
+constexpr int kCachedPartRows = 16;
 constexpr int kCachedPartFloats = kCachedPartRows * 128 + 2 * kCachedPartRows;
 template <typename Kernel>
 sam3_status_t ensure_smem_attr(sam3_ctx_t* ctx, uint32_t bit, Kernel kernel, int bytes,
