@@ -59,9 +59,9 @@ struct PK {
   static constexpr int OFF_V = OFF_K + KST * TILE;
   static constexpr int OFF_OUT = OFF_V + VST * TILE;  // [T] 128 rows of 64 outputs
   static constexpr int OFF_BAR = OFF_OUT + (T == 2 ? T * HALF : 0);
-  static constexpr int BARS = 4 * T + 2 * KST + 2 * VST + 10;
+  static constexpr int BARS = 4 * T + 2 * KST + 2 * VST + 11;
   static constexpr int OFF_MISC = (OFF_BAR + BARS * 8 + 15) / 16 * 16;
-  static constexpr int MISC = 160;
+  static constexpr int MISC = 192;
   static constexpr int SMEM = OFF_MISC + MISC + 1024;
   static constexpr uint32_t COLS = D == 128 ? 512 : 256;
   static constexpr uint32_t S(int t) { return 128u * t; }
@@ -275,6 +275,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
   const uint32_t bar_o_done = bar_o_full + 8;        // [T] after an item's last P V
   const uint32_t bar_drain = bar_o_done + 8 * T;
   const uint32_t bar_raw_free = bar_drain + 8;       // warps 10 and 11 may take the next
+  const uint32_t bar_next = bar_raw_free + 8;        // which CTA's item comes next
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
   // [2] items; of each the V tiles looked through and the rows with infinities
@@ -284,6 +285,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
   // the V tile to look through: stage (-1: no more), rows of the sequence in it,
   // whether some query sees a part of it only, its place in fix_tile, its number
   volatile int* raw = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 128);
+  const uint32_t next_slot = sbase + C::OFF_MISC + 160;  // the answer of cta_try_cancel
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -310,6 +312,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
     mbar_init(bar_o_full, 1);
     mbar_init(bar_drain, 1);
     mbar_init(bar_raw_free, 1);
+    mbar_init(bar_next, 1);
     *abort_flag = 0;
     fence_mbar_init();
     prefetch_tmap(&map_q);
@@ -363,15 +366,38 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
     Finder finder;
     finder.init(a, T == 2 && !a.pair_heads ? 256 : 128);
     uint32_t k_bits = 0, k_par = 0, v_bits = 0, v_par = 0;  // loads to drain on abort
-    uint32_t raw_uses = 0, q_par = 0;
+    uint32_t raw_uses = 0, q_par = 0, asked = 0;
+    int number = blockIdx.x;
     Ring<KST> rk;
     Ring<VST> rv;
     bool ok = true;
     for (uint32_t i = 0; ok && !(C::ONE && i); ++i) {
-      // the rounds over the tiles go to and fro, so that no CTA always gets the
-      // longer ones
-      const int number = (int)(i * gridDim.x + (i & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x));
-      Item it = finder.find(a, number / a.units);
+      // the first item is the CTA's own, the others' owners are never launched
+      if (i) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_next, (asked - 1) & 1u, abort_flag, a.err,
+                                               kDevErrTimeoutPacked));
+        if (!ok) break;
+        number = cta_cancelled(next_slot);
+        __syncwarp();
+      }
+      Item it{0, 0, -1, 0};
+      while (number >= 0) {
+        it = finder.find(a, number / a.units);
+        if (C::ONE) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar_next, 16);
+          cta_try_cancel(next_slot, bar_next);
+        }
+        ++asked;
+        if (it.tile >= 0) break;
+        // a number behind the last tile: the grid is an upper bound
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_next, (asked - 1) & 1u, abort_flag, a.err,
+                                               kDevErrTimeoutPacked));
+        if (!ok) break;
+        number = cta_cancelled(next_slot);
+        __syncwarp();
+      }
+      if (!ok) break;
       it.unit = number % a.units;
       const int slot = i & 1;
       ok = __all_sync(0xffffffffu, mbar_wait(bar_item_free + 8 * slot, (i >> 1 & 1) ^ 1, abort_flag,
@@ -465,6 +491,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
       mbar_arrive(bar_v_raw);
     }
     if (lane == 0 && *abort_flag) {
+      if (asked) mbar_wait_drain(bar_next, (asked - 1) & 1u);
       if (C::CHECKER && raw_uses) mbar_wait_drain(bar_v_raw, (raw_uses - 1) & 1u);
       for (int t = 0; t < T; ++t)
         if (q_par) mbar_wait_drain(bar_q + 8 * t, (q_par - 1) & 1u);
@@ -844,11 +871,11 @@ sam3_status_t launch_packed(sam3_ctx_t* ctx, const uint16_t* q, int64_t q_stride
   const long long tiles = a.rows / span + std::min(a.n_seqs, a.rows);
   if (tiles * a.units > 0x7FFFFFFFll)
     return set_error(ctx, SAM3_ERR_SHAPE, "attention_packed: too many rows for one call");
-  // 128: one CTA per SM stays and takes items in turn, the next item's loads and
-  // first MMAs under this one's last tiles. 64: a CTA per item; the other CTA of
-  // the SM covers its begin and end.
+  // 64: a CTA per item; the other CTA of the SM covers its begin and end. 128: one
+  // CTA per SM, which takes over the items of CTAs not yet launched, the next
+  // item's loads and first MMAs under this one's last tiles.
   const long long items = tiles * a.units;
-  const unsigned grid = (unsigned)(C::ONE ? items : std::min<long long>(items, ctx->num_sms));
+  const unsigned grid = (unsigned)items;
   const cudaError_t e = launch_pdl(packed_attn_kernel<D, BF>, dim3(grid), dim3(C::THREADS), C::SMEM,
                                    ctx->stream, mq, mk, mv, mo, a);
   return check_launch_ret(ctx, e, "packed_attn_kernel");

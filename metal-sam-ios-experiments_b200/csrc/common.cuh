@@ -115,6 +115,38 @@ __device__ __forceinline__ bool mbar_wait_drain(uint32_t bar, uint32_t parity) {
   return true;
 }
 
+__device__ __forceinline__ void fence_proxy_async_smem() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// ---- taking over CTAs that have not started ---------------------------------------
+// Asks for the grid's next CTA that has not been launched; the 16-byte answer
+// arrives in shared memory and completes 16 bytes of the mbarrier's phase.
+__device__ __forceinline__ void cta_try_cancel(uint32_t answer, uint32_t bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128"
+      " [%0], [%1];" ::"r"(answer),
+      "r"(bar)
+      : "memory");
+}
+// The answer: that CTA's blockIdx.x, which will not be launched, or -1 (none is
+// left; do not ask again).
+__device__ __forceinline__ int cta_cancelled(uint32_t answer) {
+  uint64_t lo, hi;
+  asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(lo), "=l"(hi) : "r"(answer) : "memory");
+  int x;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
+      "mov.b128 r, {%1, %2};\n\t"
+      "mov.b32 %0, -1;\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, r;\n\t}\n"
+      : "=r"(x)
+      : "l"(lo), "l"(hi));
+  fence_proxy_async_smem();  // read before the next answer is written
+  return x;
+}
+
 // ---- TMA (tiled, no multicast) --------------------------------------------------
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
                                             int32_t x, int32_t y) {
@@ -158,9 +190,6 @@ __device__ __forceinline__ void griddep_launch_dependents() {
 }
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-__device__ __forceinline__ void fence_proxy_async_smem() {
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
 
 // ---- tcgen05 -------------------------------------------------------------------
 __device__ __forceinline__ void tmem_alloc(uint32_t slot_smem, uint32_t ncols) {
