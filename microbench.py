@@ -10,6 +10,9 @@
     python microbench.py neck --batch 8          (restoreSpatial + neck, 72x72, 1024 -> 256)
     python microbench.py windowed --batch 8      (checkpoint-faithful encoder, 32 blocks, 1008^2)
     python microbench.py encoder --batch 8 [--blocks 32]  (pruned encoder, device buffers)
+    python microbench.py packed --batch 8 --seq 2592 --heads 32 --kv-heads 8 --dim 128 [--causal]
+    python microbench.py cached --batch 64 --seq 4096 --heads 32 --kv-heads 8 --dim 128 --page 64
+                                                 (the prompts' kv_append, then one token each)
 
 Inputs are synthetic device tensors (torch is used only to allocate and fill
 them); each iteration calls the operator through the C ABI; timings are CUDA
@@ -44,7 +47,7 @@ def main():
 
     ap = argparse.ArgumentParser()
     ap.add_argument("op", choices=("gemm", "attention", "layernorm", "prune", "dequant", "patch",
-                                   "preprocess", "neck", "windowed", "encoder"))
+                                   "preprocess", "neck", "windowed", "encoder", "packed", "cached"))
     ap.add_argument("--rgba", action="store_true",
                     help="patch: f32 RGBA frames, normalisation fused into the patch gather")
     ap.add_argument("--m", type=int, default=41472)
@@ -56,6 +59,10 @@ def main():
     ap.add_argument("--heads", type=int, default=16)
     ap.add_argument("--hidden", type=int, default=4096, help="windowed: MLP width (checkpoint 4736)")
     ap.add_argument("--blocks", type=int, default=32, help="encoder: blocks (pruned after half)")
+    ap.add_argument("--kv-heads", type=int, default=8, help="packed, cached: K/V heads")
+    ap.add_argument("--dim", type=int, default=128, help="packed, cached: head_dim (64 or 128)")
+    ap.add_argument("--page", type=int, default=64, help="cached: tokens per page")
+    ap.add_argument("--causal", action="store_true", help="packed: causal")
     ap.add_argument("--iters", type=int, default=10)
     ap.add_argument("--warmup", type=int, default=3)
     a = ap.parse_args()
@@ -115,6 +122,46 @@ def main():
         tf = prof["flops"] / prof["launches"] / (ms * 1e-3) / 1e12
         print(json.dumps({"op": "attention", "batch": a.batch, "seq": a.seq, "heads": a.heads,
                           "us": ms * 1e3, "tflops": tf, "frac_burst_peak": tf / tf_peak}))
+    elif a.op in ("packed", "cached"):
+        rows, h, kv, d = a.batch * a.seq, a.heads, a.kv_heads, a.dim
+        k, v = (torch.randn((rows, kv, d), generator=g, device=dev).bfloat16() for _ in range(2))
+        cu = torch.arange(a.batch + 1, device=dev, dtype=torch.int32) * a.seq
+        if a.op == "packed":
+            q = torch.randn((rows, h, d), generator=g, device=dev).bfloat16()
+            o = torch.empty_like(q)
+            prof = run(lambda: ctx.attention_packed(
+                sam3.BF16, q, h * d, k, kv * d, v, kv * d, cu, a.batch, rows, h, kv, d, d ** -0.5,
+                a.causal, o, h * d))["attention"]
+            ms = prof["ms"] / prof["launches"]
+            pairs = a.batch * (a.seq * (a.seq + 1) // 2 if a.causal else a.seq * a.seq)
+            tf = 4.0 * d * h * pairs / (ms * 1e-3) / 1e12
+            print(json.dumps({"op": "packed", "batch": a.batch, "seq": a.seq, "heads": h,
+                              "kv_heads": kv, "dim": d, "causal": a.causal, "us": ms * 1e3,
+                              "tflops": tf, "frac_burst_peak": tf / tf_peak}))
+        else:
+            wide = -(-a.seq // a.page)
+            pages = a.batch * wide
+            codes = [torch.empty((pages, kv, a.page, d), dtype=torch.uint8, device=dev) for _ in range(2)]
+            scales = [torch.empty((pages, kv), device=dev) for _ in range(2)]
+            cache = sam3.kv_cache(*codes, *scales, pages, a.page, kv, d)
+            table = torch.randperm(pages, generator=g, device=dev).int().reshape(a.batch, wide)
+            lens = torch.full((a.batch,), a.seq, dtype=torch.int32, device=dev)
+            q = torch.randn((a.batch, h, d), generator=g, device=dev).bfloat16()
+            o = torch.empty_like(q)
+            prof = run(lambda: ctx.kv_append(cache, sam3.BF16, k, kv * d, v, kv * d, cu, a.batch,
+                                             rows, a.seq, table, wide, lens))["other"]
+            ms = prof["ms"] / prof["launches"]
+            gbs = prof["bytes"] / prof["launches"] / (ms * 1e-3) / 1e9
+            print(json.dumps({"op": "kv_append", "rows": rows, "kv_heads": kv, "dim": d,
+                              "page": a.page, "us": ms * 1e3, "gbs": gbs, "frac_hbm": gbs / bw_peak}))
+            prof = run(lambda: ctx.attention_cached(
+                cache, sam3.BF16, q, h * d, None, a.batch, a.batch, 1, table, wide, lens, h,
+                d ** -0.5, True, o, h * d))["attention"]
+            ms = prof["ms"] / prof["launches"]
+            gbs = 2.0 * rows * kv * d / (ms * 1e-3) / 1e9
+            print(json.dumps({"op": "attention_cached", "batch": a.batch, "seq": a.seq, "heads": h,
+                              "kv_heads": kv, "dim": d, "page": a.page, "us": ms * 1e3, "gbs": gbs,
+                              "frac_hbm": gbs / bw_peak}))
     elif a.op == "neck":
         ctx.close()
         ctx = sam3.Context(0, max_batch=a.batch)
