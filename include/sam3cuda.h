@@ -257,7 +257,9 @@ sam3_status_t sam3_attention(sam3_ctx_t* ctx, const uint16_t* qkv, int32_t batch
  * q, k and v may be parts of one projection's rows. Row strides are in elements,
  * multiples of 8; all pointers to rows are 16-byte aligned. dtype is one of
  * sam3_dtype_t, the same for all rows of a call. heads is a multiple of
- * kv_heads: heads [i * heads / kv_heads, ...) share K/V head i. scale > 0.
+ * kv_heads: heads [i * heads / kv_heads, ...) share K/V head i. scale > 0. Scores
+ * and sums are fp32, so bf16 rows have its room too: products and sums of the
+ * row's largest values, and 2^8 of v's for each key, must stay below 2^127.
  *
  * Sequences: cu (int32 [n_seqs + 1], on the device) gives each sequence's first
  * row and the end of the last; rows is the row count of the buffers, cu[n_seqs]
@@ -295,7 +297,8 @@ sam3_status_t sam3_attention_packed(sam3_ctx_t* ctx, int32_t dtype, const uint16
  * are value / scale rounded to the nearest e4m3, ties to even; infinities and
  * values beyond 448 scales become +-448, NaN stays NaN. Calling again with the
  * same arguments leaves the cache as it is. Pages that receive tokens must
- * belong to one sequence each (shared pages: copy before writing). */
+ * stand once in the table and belong to one sequence each (shared pages: copy
+ * before writing). */
 sam3_status_t sam3_kv_append(sam3_ctx_t* ctx, const sam3_kv_cache_t* cache, int32_t dtype,
                              const uint16_t* k, int64_t k_stride, const uint16_t* v,
                              int64_t v_stride, const int32_t* cu_new, int32_t n_seqs,
@@ -311,7 +314,9 @@ sam3_status_t sam3_kv_append(sam3_ctx_t* ctx, const sam3_kv_cache_t* cache, int3
  * new token sees the tokens up to itself, else all of its sequence. Made for
  * one or a few new tokens per sequence: up to 16 query rows (new tokens times
  * heads per K/V head) read the cache once, more read it again for each 16.
- * Sequences may share pages. n_seqs <= SAM3_CACHED_MAX_SEQS. */
+ * Sequences may share pages. The weights are rounded to fp16's 11 bits before
+ * they multiply v's codes; an infinity in a row of q makes its result NaN.
+ * n_seqs <= SAM3_CACHED_MAX_SEQS. o must not overlap q. */
 sam3_status_t sam3_attention_cached(sam3_ctx_t* ctx, const sam3_kv_cache_t* cache, int32_t dtype,
                                     const uint16_t* q, int64_t q_stride, const int32_t* cu_new,
                                     int32_t n_seqs, int32_t rows, int32_t max_new,

@@ -61,6 +61,7 @@ constexpr int TILE = LINES * 128;      // bytes of K or V per tile
 constexpr int UNIT_TILES = 4;          // tiles per unit of small jobs
 constexpr int ITEM_COST = 2;           // what an item costs besides its tiles, in tiles
 constexpr float P_EXP = 6.f;           // the weight at the running maximum is 2^6
+constexpr float NO_MAX = 1e30f;        // P_EXP - M of a row that has seen nothing
 constexpr float P_TOP = 8.8f;          // and may grow to 2^8.8 < 448 before M moves
 constexpr float T1 = 1.f / 16, T2 = 1.f / 256;  // weights of the second and third term
 enum : int { kFirst = 1, kLast = 2, kFinal = 4, kCheck = 8 };
@@ -665,9 +666,10 @@ __global__ void __launch_bounds__(THREADS, 2)
           top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
         }
         top = warp_max(top);
-        // the power of two that brings the largest to [128, 256)
+        // the power of two that brings the largest to [128, 256); a row with an
+        // infinity becomes NaN, like its softmax (the codes would saturate)
         const int e2 = min(max(((__float_as_int(top) >> 23) & 255) - 127 - 7, -120), 120);
-        const float down = __int_as_float((127 - e2) << 23);
+        const float down = top == INFINITY ? NAN : __int_as_float((127 - e2) << 23);
         if (lane == (i & 31)) rs = __int_as_float((127 + e2) << 23);
         uint16_t t[EPL / 2][3];
 #pragma unroll
@@ -850,8 +852,9 @@ __global__ void __launch_bounds__(THREADS, 2)
           const float4 w = wmax[r];
           const float m = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w));
           if (first) {
-            // a row that sees nothing in its first tile sees nothing after it
-            off[r] = P_EXP - (m == -INFINITY ? 0.f : m);
+            // a row that sees nothing yet (its page may not exist): anything that
+            // it sees later exceeds M
+            off[r] = m == -INFINITY ? NO_MAX : P_EXP - m;
             l[r] = 0.f;
             alpha[r] = 1.f;
           } else {
@@ -1210,8 +1213,8 @@ sam3_status_t attention_cached(sam3_ctx_t* ctx, const sam3_kv_cache_t* c, int dt
     return set_error(ctx, SAM3_ERR_INVALID_ARG, "attention_cached: unknown dtype %d", dtype);
   if (!aligned16(q) || !aligned16(o))
     return set_error(ctx, SAM3_ERR_INVALID_ARG, "attention_cached: rows must be 16-byte aligned");
-  if (!(scale > 0.f) || scale > 3.402823466e38f)
-    return set_error(ctx, SAM3_ERR_INVALID_ARG, "attention_cached: scale must be positive");
+  if (!scale_ok(scale))
+    return set_error(ctx, SAM3_ERR_INVALID_ARG, "attention_cached: scale must be positive and finite");
   if (heads <= 0 || heads > 1024 || heads % c->kv_heads)
     return set_error(ctx, SAM3_ERR_SHAPE, "attention_cached: %d heads over %d K/V heads", heads,
                      c->kv_heads);
@@ -1249,7 +1252,7 @@ sam3_status_t attention_cached(sam3_ctx_t* ctx, const sam3_kv_cache_t* c, int dt
   a.rows = rows;
   a.max_new = max_new;
   a.causal = causal != 0;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale * kLog2E;
   const long long lines =
       (long long)c->num_pages * c->kv_heads * c->page_size * c->head_dim / 128;
   const int box = c->page_size * c->head_dim / 128;

@@ -659,7 +659,9 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
         lim = a.causal ? min(w.len, q0 + r + 1) : w.len;    // keys that the row sees
         lim_min = a.causal ? min(w.len, q0 + 1) : w.len;    // that all rows of the tile see
       }
-      float m_run = -INFINITY, l_run = 0.f;
+      // Not -inf: while a row's scores are all -inf (keys that hold infinities) its
+      // weights are 0, not 2^(-inf + inf).
+      float m_run = -3.402823466e38f, l_run = 0.f;
       bool ok = true;
       for (int j = 0; j < n; ++j, ++tiles) {
         if (C::ONE) tiles = j;
@@ -894,8 +896,8 @@ sam3_status_t attention_packed(sam3_ctx_t* ctx, int dtype, const uint16_t* q, in
     return set_error(ctx, SAM3_ERR_INVALID_ARG, "attention_packed: unknown dtype %d", dtype);
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o))
     return set_error(ctx, SAM3_ERR_INVALID_ARG, "attention_packed: rows must be 16-byte aligned");
-  if (!(scale > 0.f) || scale > 3.402823466e38f)
-    return set_error(ctx, SAM3_ERR_INVALID_ARG, "attention_packed: scale must be positive");
+  if (!scale_ok(scale))
+    return set_error(ctx, SAM3_ERR_INVALID_ARG, "attention_packed: scale must be positive and finite");
   if (head_dim != 64 && head_dim != 128)
     return set_error(ctx, SAM3_ERR_SHAPE, "attention_packed: head_dim must be 64 or 128 (got %d)",
                      head_dim);
@@ -920,7 +922,7 @@ sam3_status_t attention_packed(sam3_ctx_t* ctx, int dtype, const uint16_t* q, in
   a.rows = rows;
   a.group = heads / kv_heads;
   a.causal = causal != 0;
-  a.c = scale * 1.4426950408889634f;
+  a.c = scale * kLog2E;
   // lengths stay on the device: the work counted here is the rows read and written
   ProfScope prof(ctx, SAM3_PROF_ATTENTION, 0.0, 4.0 * rows * (wide + narrow));
   const bool bf = dtype == SAM3_BF16;

@@ -189,6 +189,9 @@ sam3_status_t check_kv_cache(sam3_ctx_t* ctx, const sam3_kv_cache_t* c, const ch
 inline bool stride_ok(int64_t stride, int64_t width) {
   return stride % 8 == 0 && stride >= width && stride <= (1ll << 31);
 }
+// A score's scale: positive, and finite in base 2 too.
+constexpr float kLog2E = 1.4426950408889634f;
+inline bool scale_ok(float scale) { return scale > 0.f && scale * kLog2E <= 3.402823466e38f; }
 
 // Launch with programmatic stream serialization: the kernel may start while
 // the previous kernel in the stream finishes (its prologue overlapping that

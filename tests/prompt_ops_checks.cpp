@@ -96,6 +96,7 @@ int main() {
   PACKED(p.scale = -1.f, ARG);
   PACKED(p.scale = __builtin_nanf(""), ARG);
   PACKED(p.scale = __builtin_inff(), ARG);
+  PACKED(p.scale = 3e38f, ARG);  // infinite in base 2
   PACKED(p.dim = 96, SHAPE);
   PACKED(p.dim = 0, SHAPE);
   PACKED(p.kv = 3, SHAPE);
@@ -148,6 +149,7 @@ int main() {
   ATTEND(p.o = 0, ARG);
   ATTEND(p.q += 2, ARG);
   ATTEND(p.scale = 0.f, ARG);
+  ATTEND(p.scale = 3e38f, ARG);
   ATTEND(p.heads = 6, SHAPE);
   ATTEND(p.heads = 0, SHAPE);
   ATTEND(p.qs = 256, SHAPE);

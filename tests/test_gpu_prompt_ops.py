@@ -110,6 +110,25 @@ def test_packed_infinities_and_nan_in_masked_places(ctx, sam3, dim, heads, kv, d
     assert np.isnan(g[300:450]).all()
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim,heads,kv", [(64, 2, 1), (128, 2, 1), (128, 1, 1)])
+def test_packed_scores_of_minus_infinity(ctx, sam3, dim, heads, kv, dtype):
+    rng = np.random.default_rng(26)
+    n, dead, scale = 400, 300, dim ** -0.5  # the first 300 keys: two whole tiles and more
+    q, k, v = (_rows(rng, n, h, dim, dtype) for h in (heads, kv, kv))
+    q[:, :, 1] = np.abs(q[:, :, 1]) + 0.125
+    q = P.rounded(q, dtype)
+    k[:dead, :, 1] = -np.inf
+    for causal in (True, False):
+        got, _ = run_packed(ctx, sam3, q, k, v, _cu([n]), dtype, causal, scale)
+        g = P.from_bits(got, dtype)
+        # their weight is 0: the result is that of the other keys alone
+        o, tol = P.attend(q[dead:], k[dead:], v[dead:], scale, 0 if causal else None, dtype, dtype)
+        assert (np.abs(g[dead:] - o) <= tol).all()
+        if causal:
+            assert np.isnan(g[:dead]).all()  # nothing but -inf
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 def test_packed_growing_scores_rescale(ctx, sam3, dim):
     rng = np.random.default_rng(7)
@@ -147,6 +166,56 @@ def test_packed_many_short_sequences(ctx, sam3):
     q, k, v = (_rows(rng, rows, n, 64, "f16") for n in (2, 2, 2))
     got, _ = run_packed(ctx, sam3, q, k, v, cu, "f16", True, 0.125)
     check_packed(got, q, k, v, cu, "f16", True, 0.125)
+
+
+@pytest.mark.parametrize("heads,kv", [(2, 1), (3, 3)])
+def test_packed_many_sequences_of_several_tiles(ctx, sam3, heads, kv):
+    rng = np.random.default_rng(29)
+    lens = rng.integers(0, 400, 150)
+    cu, rows = _cu(lens), int(lens.sum()) + 7
+    q, k, v = (_rows(rng, rows, n, 128, "bf16") for n in (heads, kv, kv))
+    for causal in (True, False):
+        got, _ = run_packed(ctx, sam3, q, k, v, cu, "bf16", causal, 0.09)
+        check_packed(got, q, k, v, cu, "bf16", causal, 0.09)
+    bad = cu.copy()
+    bad[0] = rows + 1  # the sequence that is looked at last
+    with pytest.raises(sam3.SAM3Error) as e:
+        run_packed(ctx, sam3, q, k, v, bad, "bf16", True, 0.09)
+    assert e.value.status == sam3.ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_packed_captured_and_replayed_with_other_lengths(sam3, dim):
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(30)
+    heads, kv, rows = 4, 2, 1000
+    with sam3.Context(0, embed_dim=256, num_heads=4, mlp_hidden=512, num_blocks=0, image_size=112,
+                      prune_after_block=0, max_batch=1) as ctx:
+        q, k, v = (_rows(rng, rows, n, dim, "f16") for n in (heads, kv, kv))
+        dev = [torch.from_numpy(_bits(x, "f16").view(np.int16)).cuda() for x in (q, k, v)]
+        o = torch.empty_like(dev[0])
+        cu = torch.zeros(5, dtype=torch.int32, device="cuda")
+        stream = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        ctx.set_stream(stream.cuda_stream)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(stream):
+            graph.capture_begin()
+            for _ in range(2):  # two in a row: the second begins under the first's end
+                ctx.attention_packed(sam3.F16, dev[0], heads * dim, dev[1], kv * dim, dev[2], kv * dim,
+                                     cu, 4, rows, heads, kv, dim, 0.1, True, o, heads * dim)
+            graph.capture_end()
+        for lens in ([1000, 0, 0, 0], [1, 1, 1, 1], [0, 500, 3, 497], [0, 0, 0, 0], [129, 383, 256, 200]):
+            with torch.cuda.stream(stream):
+                cu.copy_(torch.from_numpy(_cu(lens)))
+                o.fill_(0x5A5A)
+                graph.replay()
+                got = o.cpu().numpy().view(np.uint16).reshape(rows, heads, dim)
+            check_packed(got, q, k, v, _cu(lens), "f16", True, 0.1)
+            assert (got[sum(lens):] == GUARD).all()
+        ctx.sync()
+        ctx.set_stream(None)
+        del graph
 
 
 def test_packed_agrees_with_the_encoders_attention(ctx, sam3):
@@ -428,6 +497,56 @@ def test_cached_nan_among_the_new_tokens(ctx, sam3, dim):
     keep = np.arange(dim) != 9
     assert np.array_equal(got[3:6][..., keep], clean[3:6][..., keep])
     assert np.array_equal(got[6:10], clean[6:10]) and np.isnan(g[10:]).all()
+    dc.free()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_cached_queries_that_are_not_finite(ctx, sam3, dim, dtype):
+    rng = np.random.default_rng(27)
+    lens = [70, 200, 30]
+    host, table = filled(rng, ctx, sam3, lens, 2, 16, dim)
+    dc = DeviceCache(ctx, sam3, host, dim)
+    q = _rows(rng, 3, 4, dim, dtype)
+    clean = attend(ctx, sam3, dc, q, None, table, lens, dtype, True, 0.1)
+    q[0, 1, 3], q[1, 2, 0], q[2, 0, dim - 1] = np.inf, np.nan, -np.inf
+    got = attend(ctx, sam3, dc, q, None, table, lens, dtype, True, 0.1)
+    bad = np.zeros((3, 4), bool)
+    bad[0, 1] = bad[1, 2] = bad[2, 0] = True
+    assert np.isnan(P.from_bits(got, dtype)[bad]).all() and np.array_equal(got[~bad], clean[~bad])
+    dc.free()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n", [600, 20000])
+def test_cached_a_page_that_does_not_exist_hides_its_tokens(ctx, sam3, n, dim):
+    rng = np.random.default_rng(28)
+    page, heads, scale = 32, 2, 0.05
+    host, table = filled(rng, ctx, sam3, [n], 1, page, dim)
+    for p in range(-(-n // page)):  # scores far below 0, so that a maximum of 0 would lose all
+        m = min(page, n - p * page)
+        host.codes[0][table[0, p], :, :m] = P.to_codes(rng.uniform(100, 200, (1, m, dim)))
+    dc = DeviceCache(ctx, sam3, host, dim)
+    q = P.rounded(-rng.uniform(60, 70, (1, heads, dim)), "f16")
+    gone = [*range(10), 15]  # the first tile's pages and more
+    t = table.copy()
+    t[0, gone] = 1 << 30
+    bufs = [ctx.upload(_bits(q, "f16")), ctx.upload(t), ctx.upload(np.array([n], np.int32)),
+            ctx.upload(np.zeros((1, heads * dim), np.uint16))]
+    ctx.attention_cached(dc.c, sam3.F16, bufs[0], heads * dim, None, 1, 1, 1, bufs[1], t.shape[1],
+                         bufs[2], heads, scale, True, bufs[3], heads * dim)
+    with pytest.raises(sam3.SAM3Error) as e:
+        ctx.sync()
+    assert e.value.status == sam3.ERR_INVALID_ARG
+    got = P.from_bits(ctx.download(bufs[3], (1, heads, dim), np.uint16), "f16")
+    pages = table[0, :-(-n // page)]
+    seen = ~np.isin(np.arange(n) // page, gone)
+    k, v = (host.values(i, pages, n)[seen] for i in (0, 1))
+    assert (q[0, 0] @ k[0, 0]) * scale < -150
+    o, tol = P.attend(q, k, v, scale, None, "f16", "f16", vmax=float(host.scales[1][pages].max()))
+    assert (np.abs(got - o) <= tol).all()
+    for b in bufs:
+        b.free()
     dc.free()
 
 
