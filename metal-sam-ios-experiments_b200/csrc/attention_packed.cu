@@ -20,17 +20,40 @@
 // Warps: 0 TMA producer, 1 TMEM allocator and MMA issuer (one thread), then
 // four softmax warps per query tile, one thread per row: the row's 128 scores
 // to registers, maximum, exponentials, P back to TMEM. O is rescaled in place,
-// and only when a row's maximum grew by more than 2^8.
+// and only when a row's maximum grew by more than 2^8. For head_dim 128 two
+// more warps look through V tiles (below).
+//
+// Work: a tile of every sequence and head, longest first, so that the last to
+// finish are short (Finder). head_dim 64: a CTA each; the SM's other CTA covers
+// its begin and end. head_dim 128: the grid is as large, but a running CTA takes
+// over the items of CTAs that are not launched yet (clusterlaunchcontrol), so
+// that the next item's loads and first MMAs run under this one's last tiles:
+// 16 causal sequences of 17 to 2048 rows (7,445 in all, 32 heads on 8) take 108 us,
+// dealt out in the same order to one CTA per SM beforehand 114. Results leave
+// through shared memory and TMA stores, for which nobody waits (125 us to 114).
 //
 // Masked places: scores are replaced before the maximum, whatever they are. V
 // needs more, because 0 * inf is NaN: in a sequence's last key tile and in the
-// causal diagonal ones, warp 0 zeroes the V rows behind the sequence's end and,
-// on the diagonal, the infinities and NaN of rows that only some queries see,
-// before the MMA reads the tile; those are added to the rows that see them at
-// the end (rare; read again from global memory).
+// causal diagonal ones the V rows behind the sequence's end become 0 and, on
+// the diagonal, so do the infinities and NaN of rows that only some queries
+// see, before the MMA reads the tile; those are added to the rows that see them
+// at the end (rare; read again from global memory). head_dim 64: the producer
+// warp does this, head_dim 128: warps 10 and 11, since there the producer's
+// loads are late by it (8192 causal rows, 32 heads on 8: 525 against 500 us).
 //
 // P is rounded to the inputs' type, as tcgen05 takes both operands in one: half
 // a step (fp16 2^-11, bf16 2^-8) of each weight.
+//
+// Bounds, measured: head_dim 64 by the softmax warps' issue slots, of them the
+// exponentials alone (16 per clock and SM) 133 us where the MMAs need 94: four
+// images' tokens (2592, 1733, 5184 and 901 rows, 16 heads) 237 us, 645 TFLOP/s;
+// 16 times 5184 rows 2.63 ms, 717 TFLOP/s. head_dim 128 by the chain from the
+// scores through the softmax to the next MMAs of a tile, with only one other
+// tile to fill the pipe meanwhile: 8192 causal rows, 32 heads on 8, 488 us,
+// 1127 TFLOP/s, 69 % of cuBLAS's burst rate. Tried and slower at head_dim 128: P in two halves with its
+// own commits (526 -> 571 us), an issuer that polls for whatever is ready (487 ->
+// 705), a part of the exponentials as polynomials (1/8: 492, 1/4: 527), skipping
+// masked 32-key groups of diagonal tiles (505 -> 545, a branch in the loop).
 #include <algorithm>
 
 #include "common.cuh"
@@ -267,7 +290,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
   const uint32_t bar_k_empty = bar_k_full + 8 * KST;
   const uint32_t bar_v_full = bar_k_empty + 8 * KST;
   const uint32_t bar_v_empty = bar_v_full + 8 * VST;
-  const uint32_t bar_v_raw = bar_v_empty + 8 * VST;  // a V tile that warp 0 looks through
+  const uint32_t bar_v_raw = bar_v_empty + 8 * VST;  // a V tile to look through before its use
   const uint32_t bar_s_full = bar_v_raw + 8;         // [T] Q K^T done (and the P V before it)
   const uint32_t bar_s_free = bar_s_full + 8 * T;    // scores are in registers (P apart)
   const uint32_t bar_p_full = bar_s_free + 8;        // [T] P written
@@ -766,7 +789,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
           tmem_wait_ld();
 #pragma unroll
           for (int d = 0; d < 64; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * inv);
-          // infinities and NaN that warp 0 took out of the diagonal V tiles
+          // infinities and NaN taken out of the diagonal V tiles
           for (int f = 0; f < 8 && __builtin_expect(fixes != 0, 0); ++f) {
             uint32_t bits = fix_rows[(i & 1) * 8 + f];
             while (bits) {

@@ -17,7 +17,13 @@
 //
 // HBM bound: 2 bytes in and 1 byte out per element. One unit of work is one
 // (page, head, K or V); its elements stay in registers between the maximum and
-// the rounding, so each is read once.
+// the rounding, so each is read once. Measured: 8 prompts of 8192 tokens (8
+// heads of 128, pages of 128) 65 us, 6.2 TB/s, 94 % of a copy's rate (89 us with
+// two CTAs per SM and pages before heads in the grid); four images' tokens
+// (10,410 rows, 16 heads of 64, pages of 16) 14.2 us, 4.5 TB/s: the
+// same chain of loads at the begin and the end is a larger part of it. One token
+// each of 64 sequences: 5.4 us, a launch, three dependent loads (length, page,
+// scale) and a store.
 #include <algorithm>
 
 #include "common.cuh"
