@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t sbase = smem_u32(smem);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   const uint32_t bar_item = sbase + C::OFF_BAR;  // [2] an item is told
   const uint32_t bar_item_free = bar_item + 16;     // [2] and done with
@@ -525,26 +525,37 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
     }
   } else if (warp == 1) {
     // ----------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      bool ok = true, issued = false;
-      auto wait = [&](uint32_t bar, uint32_t par) {
-        return mbar_wait(bar, par, abort_flag, a.err, kDevErrTimeoutPacked);
-      };
-      Ring<KST> rk;   // of the next Q K^T
-      Ring<VST> rv;   // of the next P V
-      uint32_t n_p[2] = {0, 0};  // P tiles waited for
-      uint32_t n_s = 0;          // S tiles issued (P apart)
-      for (uint32_t i = 0; ok && !(C::ONE && i); ++i) {
-        ok = wait(bar_item + 8 * (i & 1), i >> 1 & 1);
-        if (!ok) break;
-        const Item it = items[i & 1];
-        mbar_arrive(bar_item_free + 8 * (i & 1));
-        if (it.tile < 0) break;
-        const Work w = work_of<T>(a, it);
-        auto last_of = [&](int j) { return T == 2 && j < w.n[1] ? 1 : 0; };
-        auto issue_qk = [&](int t, int j) {
-          const uint64_t dq = umma_desc_sw128(sbase + t * C::TILE);
-          const uint64_t dk = umma_desc_sw128(sbase + C::OFF_K + rk.st * C::TILE);
+    // The whole warp runs this and one elected thread issues, so that what the MMAs
+    // take (descriptors, columns) is uniform to the compiler.
+    bool ok = true, issued = false;
+    auto wait = [&](uint32_t bar, uint32_t par) {
+      return __all_sync(0xffffffffu,
+                        mbar_wait(bar, par, abort_flag, a.err, kDevErrTimeoutPacked)) != 0;
+    };
+    Ring<KST> rk;   // of the next Q K^T
+    Ring<VST> rv;   // of the next P V
+    uint32_t n_p[2] = {0, 0};  // P tiles waited for
+    uint32_t n_s = 0;          // S tiles issued (P apart)
+    const uint64_t desc_q = umma_desc_sw128(sbase), desc_k = umma_desc_sw128(sbase + C::OFF_K);
+    // V tile: keys along K, head_dim along N in 64-wide groups HALF apart
+    const uint64_t desc_v = (umma_desc_sw128_mn(sbase + C::OFF_V) & ~(0x3FFFull << 16)) |
+                            ((uint64_t)(C::HALF >> 4) << 16);
+    for (uint32_t i = 0; ok && !(C::ONE && i); ++i) {
+      ok = wait(bar_item + 8 * (i & 1), i >> 1 & 1);
+      if (!ok) break;
+      const Item it = items[i & 1];
+      const Work w = work_of<T>(a, it);
+      const bool none = __shfl_sync(0xffffffffu, it.tile, 0) < 0;
+      const int n0 = __shfl_sync(0xffffffffu, w.n[0], 0), n1 = __shfl_sync(0xffffffffu, w.n[1], 0);
+      const int nmax = max(n0, n1);
+      if (lane == 0) mbar_arrive(bar_item_free + 8 * (i & 1));
+      if (none) break;
+      auto last_of = [&](int j) { return T == 2 && j < n1 ? 1 : 0; };
+      auto issue_qk = [&](int t, int j) {
+        const uint64_t dq = desc_advance(desc_q, t * C::TILE);
+        const uint64_t dk = desc_advance(desc_k, rk.st * C::TILE);
+        const bool last = t == last_of(j);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off = (kk / 4) * C::HALF + (kk % 4) * 32;
@@ -552,81 +563,79 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
                         kk != 0);
           }
           umma_commit(bar_s_full + 8 * t);
-          issued = true;
-          if (t == last_of(j)) {
-            umma_commit(bar_k_empty + 8 * rk.st);
-            rk.step();
-            if (j == w.nmax - 1) umma_commit(bar_q_free);
-          }
-        };
-        auto issue_pv = [&](int t, int j) {
-          // V tile: keys along K, head_dim along N in 64-wide groups HALF apart
-          uint64_t dv = umma_desc_sw128_mn(sbase + C::OFF_V + rv.st * C::TILE);
-          dv = (dv & ~(0x3FFFull << 16)) | ((uint64_t)(C::HALF >> 4) << 16);
+          if (last) umma_commit(bar_k_empty + 8 * rk.st);
+          if (last && j == nmax - 1) umma_commit(bar_q_free);
+        }
+        issued = true;
+        if (last) rk.step();
+      };
+      auto issue_pv = [&](int t, int j) {
+        const uint64_t dv = desc_advance(desc_v, rv.st * C::TILE);
+        const bool last = t == last_of(j);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < BKV / 16; ++kk)
             umma_f16_ts(tmem + C::O(t), tmem + C::P(t) + kk * 8, desc_advance(dv, kk * 2048),
                         IDESC_O, (j | kk) != 0);
           if (!C::OVERLAY) umma_commit(bar_o_full);
-          if (t == last_of(j)) {
-            umma_commit(bar_v_empty + 8 * rv.st);
-            rv.step();
-          }
-          if (j == w.n[t] - 1) umma_commit(bar_o_done + 8 * t);
-        };
-        ok = wait(bar_q, i & 1) && wait(bar_k_full + 8 * rk.st, rk.ph);
-        if (C::OVERLAY) {
-          if (ok) {
-            tc_fence_after();
-            issue_qk(0, 0);
-            if (w.n[1]) {
-              ok = wait(bar_q + 8 * (T - 1), i & 1);
-              if (ok) issue_qk(1, 0);
-            }
-          }
-          for (int j = 0; j < w.nmax && ok; ++j) {
-            bool v_here = false, k_here = false;
-#pragma unroll
-            for (int t = 0; t < T; ++t) {
-              if (j >= w.n[t] || !ok) continue;
-              // V and the next K are early as a rule: their waits come first, so that
-              // nothing stands between P and its MMAs
-              const bool more = j + 1 < w.n[t];
-              ok = (v_here || wait(bar_v_full + 8 * rv.st, rv.ph)) &&
-                   (!more || k_here || wait(bar_k_full + 8 * rk.st, rk.ph));
-              v_here = true;
-              k_here |= more;
-              ok = ok && wait(bar_p_full + 8 * t, n_p[t]++ & 1u);
-              if (!ok) continue;
-              tc_fence_after();
-              issue_pv(t, j);
-              if (more) issue_qk(t, j + 1);
-            }
-          }
-        } else {
-          // S is free once the softmax has read the tile before
-          auto next_s = [&](int j) {
-            ok = wait(bar_k_full + 8 * rk.st, rk.ph) && (n_s == 0 || wait(bar_s_free, (n_s - 1) & 1u));
-            if (!ok) return;
-            tc_fence_after();
-            issue_qk(0, j);
-            ++n_s;
-          };
-          if (ok) next_s(0);
-          if (ok && w.nmax > 1) next_s(1);
-          for (int j = 0; j < w.nmax && ok; ++j) {
-            ok = wait(bar_p_full, n_p[0]++ & 1u) && wait(bar_v_full + 8 * rv.st, rv.ph);
-            if (!ok) break;
-            tc_fence_after();
-            issue_pv(0, j);
-            if (j + 2 < w.nmax) next_s(j + 2);
+          if (last) umma_commit(bar_v_empty + 8 * rv.st);
+          if (j == (t ? n1 : n0) - 1) umma_commit(bar_o_done + 8 * t);
+        }
+        if (last) rv.step();
+      };
+      ok = wait(bar_q, i & 1) && wait(bar_k_full + 8 * rk.st, rk.ph);
+      if (C::OVERLAY) {
+        if (ok) {
+          tc_fence_after();
+          issue_qk(0, 0);
+          if (n1) {
+            ok = wait(bar_q + 8 * (T - 1), i & 1);
+            if (ok) issue_qk(1, 0);
           }
         }
+        for (int j = 0; j < nmax && ok; ++j) {
+          bool v_here = false, k_here = false;
+#pragma unroll
+          for (int t = 0; t < T; ++t) {
+            const int n = t ? n1 : n0;
+            if (j >= n || !ok) continue;
+            // V and the next K are early as a rule: their waits come first, so that
+            // nothing stands between P and its MMAs
+            const bool more = j + 1 < n;
+            ok = (v_here || wait(bar_v_full + 8 * rv.st, rv.ph)) &&
+                 (!more || k_here || wait(bar_k_full + 8 * rk.st, rk.ph));
+            v_here = true;
+            k_here |= more;
+            ok = ok && wait(bar_p_full + 8 * t, n_p[t]++ & 1u);
+            if (!ok) continue;
+            tc_fence_after();
+            issue_pv(t, j);
+            if (more) issue_qk(t, j + 1);
+          }
+        }
+      } else {
+        // S is free once the softmax has read the tile before
+        auto next_s = [&](int j) {
+          ok = wait(bar_k_full + 8 * rk.st, rk.ph) && (n_s == 0 || wait(bar_s_free, (n_s - 1) & 1u));
+          if (!ok) return;
+          tc_fence_after();
+          issue_qk(0, j);
+          ++n_s;
+        };
+        if (ok) next_s(0);
+        if (ok && nmax > 1) next_s(1);
+        for (int j = 0; j < nmax && ok; ++j) {
+          ok = wait(bar_p_full, n_p[0]++ & 1u) && wait(bar_v_full + 8 * rv.st, rv.ph);
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(0, j);
+          if (j + 2 < nmax) next_s(j + 2);
+        }
       }
-      if (*abort_flag && issued) {
-        umma_commit(bar_drain);
-        mbar_wait_drain(bar_drain, 0);
-      }
+    }
+    if (*abort_flag && issued) {
+      if (elect_one()) umma_commit(bar_drain);
+      mbar_wait_drain(bar_drain, 0);
     }
   } else if (C::CHECKER && warp >= 2 + 4 * T) {
     // ----------------------------------------------------------- V tiles
