@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t sbase = smem_u32(smem);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   const uint32_t bar_k = sbase + C::OFF_BAR;    // [ST] K tile, scales and info are there
   const uint32_t bar_v = bar_k + 8 * ST;        // [ST] V tile is there
@@ -549,87 +549,96 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
   } else if (busy && warp == 1) {
     // ------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t IDESC_S = umma_idesc_e4m3(128, N, 0);
-      constexpr uint32_t IDESC_O = umma_idesc_e4m3(128, N, 1);
-      const uint32_t s_col = tmem, o_col = tmem + C::COLS / 2;
-      struct Slot {
-        int st = 0;
-        uint32_t ph = 0;
-        __device__ void step() {
-          if (++st == ST) {
-            st = 0;
-            ph ^= 1;
-          }
+    constexpr uint32_t IDESC_S = umma_idesc_e4m3(128, N, 0);
+    constexpr uint32_t IDESC_O = umma_idesc_e4m3(128, N, 1);
+    const uint32_t s_col = tmem, o_col = tmem + C::COLS / 2;
+    struct Slot {
+      int st = 0;
+      uint32_t ph = 0;
+      __device__ void step() {
+        if (++st == ST) {
+          st = 0;
+          ph ^= 1;
         }
-      } qk, pv;                     // stages of the next Q K^T and P V
-      uint32_t n_qk = 0, n_pv = 0;  // issued
-      uint32_t items = 0;           // begun by Q K^T
-      bool all_qk = false, ok = true;
-      // what the next of each waits for, as far as it has been seen to be there
-      bool have_k = false, have_s = true, have_p = false;
-      uint64_t since = global_timer_ns();
-      // Whichever is ready goes first: the next tile's scores (its K may be late,
-      // its item's queries too) or this tile's P V.
-      while (ok) {
-        bool did = false;
-        if (n_pv < n_qk) {
-          have_p = have_p || mbar_test(bar_p, n_pv & 1u);
-          if (have_p && mbar_test(bar_v + 8 * pv.st, pv.ph)) {
-            const int flags = infos[pv.st].z;
-            tc_fence_after();
-            const uint64_t dv = umma_desc_mn<128>(sbase + (pv.st * 2 + 1) * TILE);
-            const uint64_t dp = umma_desc_mn<C::PW>(sbase + C::OFF_P);
+      }
+    } qk, pv;                     // stages of the next Q K^T and P V
+    uint32_t n_qk = 0, n_pv = 0;  // issued
+    uint32_t items = 0;           // begun by Q K^T
+    bool all_qk = false, ok = true;
+    // what the next of each waits for, as far as it has been seen to be there
+    bool have_k = false, have_s = true, have_p = false;
+    uint64_t since = global_timer_ns();
+    // The whole warp runs this and one elected thread issues, so that what the MMAs
+    // take is uniform to the compiler.
+    auto here = [](uint32_t bar, uint32_t par) {
+      return __all_sync(0xffffffffu, mbar_test(bar, par)) != 0;
+    };
+    const uint64_t desc_q = umma_desc_sw128(sbase + C::OFF_Q), desc_k = umma_desc_sw128(sbase);
+    const uint64_t desc_v = umma_desc_mn<128>(sbase + TILE);
+    const uint64_t desc_p = umma_desc_mn<C::PW>(sbase + C::OFF_P);
+    // Whichever is ready goes first: the next tile's scores (its K may be late,
+    // its item's queries too) or this tile's P V.
+    while (ok) {
+      bool did = false;
+      if (n_pv < n_qk) {
+        have_p = have_p || here(bar_p, n_pv & 1u);
+        if (have_p && here(bar_v + 8 * pv.st, pv.ph)) {
+          const int flags = __shfl_sync(0xffffffffu, infos[pv.st].z, 0);
+          tc_fence_after();
+          const uint64_t dv = desc_advance(desc_v, pv.st * 2 * TILE);
+          if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              umma_f8_ss(o_col, desc_advance(dv, k * 4096), desc_advance(dp, k * 32 * C::PW),
+              umma_f8_ss(o_col, desc_advance(dv, k * 4096), desc_advance(desc_p, k * 32 * C::PW),
                          IDESC_O, !(flags & kFirst) || k != 0);
             umma_commit(bar_o);
             umma_commit(bar_empty + 8 * pv.st);
-            pv.step();
-            ++n_pv;
-            have_p = false;
-            did = true;
-            if (flags & kFinal) break;
           }
+          pv.step();
+          ++n_pv;
+          have_p = false;
+          did = true;
+          if (flags & kFinal) break;
         }
-        if (!all_qk) {
-          have_s = have_s || mbar_test(bar_s_free, (n_qk - 1) & 1u);
-          have_k = have_k || mbar_test(bar_k + 8 * qk.st, qk.ph);
-          if (have_s && have_k) {
-            const int flags = infos[qk.st].z;
-            if (!(flags & kFirst) || mbar_test(bar_q + 8 * (items & 1), (items >> 1) & 1u)) {
-              if (flags & kFirst) ++items;
-              const uint64_t dk = umma_desc_sw128(sbase + qk.st * 2 * TILE);
-              const uint64_t dq = umma_desc_sw128(sbase + C::OFF_Q + ((items - 1) & 1) * N * 128);
-              tc_fence_after();
+      }
+      if (!all_qk) {
+        have_s = have_s || here(bar_s_free, (n_qk - 1) & 1u);
+        have_k = have_k || here(bar_k + 8 * qk.st, qk.ph);
+        if (have_s && have_k) {
+          const int flags = __shfl_sync(0xffffffffu, infos[qk.st].z, 0);
+          if (!(flags & kFirst) || here(bar_q + 8 * (items & 1), (items >> 1) & 1u)) {
+            if (flags & kFirst) ++items;
+            const uint64_t dk = desc_advance(desc_k, qk.st * 2 * TILE);
+            const uint64_t dq = desc_advance(desc_q, ((items - 1) & 1) * N * 128);
+            tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 umma_f8_ss(s_col, desc_advance(dk, k * 32), desc_advance(dq, k * 32), IDESC_S,
                            k != 0);
               umma_commit(bar_s);
-              all_qk = flags & kFinal;
-              qk.step();
-              ++n_qk;
-              have_s = have_k = false;
-              did = true;
             }
+            all_qk = flags & kFinal;
+            qk.step();
+            ++n_qk;
+            have_s = have_k = false;
+            did = true;
           }
         }
-        if (did) {
-          since = global_timer_ns();
-        } else if (*abort_flag) {
-          ok = false;
-        } else if (global_timer_ns() - since > kWaitTimeoutNs) {
-          *abort_flag = 1;
-          atomicExch(a.err, kDevErrTimeoutCached);
-          ok = false;
-        }
       }
-      if (*abort_flag) {
-        umma_commit(bar_drain);
-        mbar_wait_drain(bar_drain, 0);
+      if (did) {
+        since = global_timer_ns();
+      } else if (__any_sync(0xffffffffu, *abort_flag)) {
+        ok = false;
+      } else if (__any_sync(0xffffffffu, global_timer_ns() - since > kWaitTimeoutNs)) {
+        *abort_flag = 1;
+        atomicExch(a.err, kDevErrTimeoutCached);
+        ok = false;
       }
+    }
+    if (__any_sync(0xffffffffu, *abort_flag)) {
+      if (elect_one()) umma_commit(bar_drain);
+      mbar_wait_drain(bar_drain, 0);
     }
   } else if (busy && warp == 2) {
     // ------------------------------------------------------------- queries

@@ -394,6 +394,13 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
     Ring<KST> rk;
     Ring<VST> rv;
     bool ok = true;
+    auto ask = [&]() {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar_next, 16);
+        cta_try_cancel(next_slot, bar_next);
+      }
+      ++asked;
+    };
     for (uint32_t i = 0; ok && !(C::ONE && i); ++i) {
       // the first item is the CTA's own, the others' owners are never launched
       if (i) {
@@ -406,14 +413,9 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
       Item it{0, 0, -1, 0};
       while (number >= 0) {
         it = finder.find(a, number / a.units);
-        if (C::ONE) break;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(bar_next, 16);
-          cta_try_cancel(next_slot, bar_next);
-        }
-        ++asked;
-        if (it.tile >= 0) break;
+        if (C::ONE || it.tile >= 0) break;
         // a number behind the last tile: the grid is an upper bound
+        ask();
         ok = __all_sync(0xffffffffu, mbar_wait(bar_next, (asked - 1) & 1u, abort_flag, a.err,
                                                kDevErrTimeoutPacked));
         if (!ok) break;
@@ -449,6 +451,9 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
       int fixes = 0;
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
       for (int j = 0; j < w.nmax && ok; ++j) {
+        // no earlier than the answer is needed, two tiles before the item's last MMA:
+        // until then it may fall to a CTA that is done before
+        if (!C::ONE && j == w.nmax - 1) ask();
         // does some query of the CTA see a part of this tile only?
         const bool diag = a.causal && (j == w.n[0] - 1 || j == w.n[1] - 1);
         const bool fix = diag || (j + 1) * BKV > w.len;
@@ -633,7 +638,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
         }
       }
     }
-    if (*abort_flag && issued) {
+    if (__any_sync(0xffffffffu, *abort_flag) && issued) {
       if (elect_one()) umma_commit(bar_drain);
       mbar_wait_drain(bar_drain, 0);
     }
