@@ -343,14 +343,22 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
     prefetch_tmap(&map_v);
     prefetch_tmap(&map_o);
   }
-  if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), C::COLS);
-    tmem_relinquish();
+  // The producer does not wait for the allocation: it finds its first item and
+  // starts its loads meanwhile.
+  uint32_t tmem = 0;
+  if (warp == 0) {
+    __syncwarp();
+    asm volatile("barrier.cta.arrive 1, %0;" ::"n"(C::THREADS) : "memory");
+  } else {
+    if (warp == 1) {
+      tmem_alloc(smem_u32(tmem_slot), C::COLS);
+      tmem_relinquish();
+    }
+    tc_fence_before();
+    asm volatile("barrier.cta.sync 1, %0;" ::"n"(C::THREADS) : "memory");
+    tc_fence_after();
+    tmem = *tmem_slot;
   }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
   griddep_launch_dependents();  // behind the allocation: the next kernel allocates too
   griddep_wait();  // offsets and rows may be earlier kernels' outputs
 
