@@ -73,8 +73,11 @@ struct PK {
   static constexpr bool OVERLAY = D == 128;      // P in its S's columns
   static constexpr int HALVES = D / 64;          // 128-byte wide parts of a tile
   static constexpr bool ONE = D == 64;           // a CTA takes one item, else items in turn
-  static constexpr bool CHECKER = D == 128;      // warps 10 and 11 look through V
-  static constexpr int THREADS = 64 + 128 * T + (CHECKER ? 64 : 0);
+  // Warps: four of softmax per tile, then a warpgroup of others. The registers of
+  // the launch (2 x 256 x 128 or 384 x 168 per SM) are split among them.
+  static constexpr int PRODUCER = 4 * T, ISSUER = 4 * T + 1, CHECKER = 4 * T + 2;
+  static constexpr int THREADS = 128 * (T + 1);
+  static constexpr int REGS = D == 128 ? 208 : 192, REGS_OTHERS = D == 128 ? 88 : 64;
   static constexpr int KST = D == 128 ? 2 : 3;   // K tiles in shared memory
   static constexpr int TILE = BKV * D * 2;       // bytes of a Q, K or V tile
   static constexpr int HALF = BKV * 128;
@@ -297,7 +300,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
   const uint32_t bar_o_full = bar_p_full + 8 * T;    // P V done (P apart)
   const uint32_t bar_o_done = bar_o_full + 8;        // [T] after an item's last P V
   const uint32_t bar_drain = bar_o_done + 8 * T;
-  const uint32_t bar_raw_free = bar_drain + 8;       // warps 10 and 11 may take the next
+  const uint32_t bar_raw_free = bar_drain + 8;       // the checkers may take the next
   const uint32_t bar_next = bar_raw_free + 8;        // which CTA's item comes next
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
@@ -310,7 +313,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
   volatile int* raw = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 128);
   const uint32_t next_slot = sbase + C::OFF_MISC + 160;  // the answer of cta_try_cancel
 
-  if (threadIdx.x == 0) {
+  if (warp == C::PRODUCER && lane == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar_item + 8 * i, 1);
       mbar_init(bar_item_free + 8 * i, 1 + 4 * T);  // the issuer and the softmax warps
@@ -346,11 +349,11 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
   // The producer does not wait for the allocation: it finds its first item and
   // starts its loads meanwhile.
   uint32_t tmem = 0;
-  if (warp == 0) {
+  if (warp == C::PRODUCER) {
     __syncwarp();
     asm volatile("barrier.cta.arrive 1, %0;" ::"n"(C::THREADS) : "memory");
   } else {
-    if (warp == 1) {
+    if (warp == C::ISSUER) {
       tmem_alloc(smem_u32(tmem_slot), C::COLS);
       tmem_relinquish();
     }
@@ -362,22 +365,26 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
   griddep_launch_dependents();  // behind the allocation: the next kernel allocates too
   griddep_wait();  // offsets and rows may be earlier kernels' outputs
 
-  // Looks through a V tile before the MMA reads it (by `threads` threads of one or
-  // two warps, `id` among them): rows behind the sequence's end become 0, and so
-  // do infinities and NaN on the diagonal, whose rows are noted.
-  auto look_through = [&](int st, int held, bool diag, int nth, int id, int threads) {
+  // Looks through a V tile before the MMA reads it (by 64 threads, `id` among
+  // them): rows behind the sequence's end become 0, and so do infinities and NaN
+  // on the diagonal, whose rows are noted.
+  auto carry = [](uint32_t w) {
+    return BF ? (w & 0x7F807F80u) + 0x00800080u : (w & 0x7C007C00u) + 0x04000400u;
+  };
+  auto look_through = [&](int st, int held, bool diag, int nth, int id) {
+    constexpr int threads = 64;
     uint4* vt = reinterpret_cast<uint4*>(smem + C::OFF_V + st * C::TILE);
-    for (int e = id; e < C::TILE / 16; e += threads)
-      if (((e >> 3) & (BKV - 1)) >= held) vt[e] = make_uint4(0, 0, 0, 0);
+    for (int h = 0; h < C::HALVES; ++h)
+      for (int e = held * 8 + id; e < BKV * 8; e += threads)
+        vt[h * BKV * 8 + e] = make_uint4(0, 0, 0, 0);
     if (diag) {
-      bool found = false;
+      uint32_t found = 0;  // an exponent of ones and 1 carry into the sign bit
 #pragma unroll 8
       for (int e = id; e < C::TILE / 16; e += threads) {
         const uint4 x = vt[e];
-        found |= (not_finite<BF>(x.x) | not_finite<BF>(x.y) | not_finite<BF>(x.z) |
-                  not_finite<BF>(x.w)) != 0;
+        found |= carry(x.x) | carry(x.y) | carry(x.z) | carry(x.w);
       }
-      if (found)
+      if (found & 0x80008000u)
         for (int e = id; e < C::TILE / 16; e += threads) {
           const int r = (e >> 3) & (BKV - 1);
           const uint4 x = vt[e];
@@ -392,288 +399,280 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
     fence_proxy_async_smem();
   };
 
-  if (warp == 0) {
-    // ----------------------------------------------------------- producer
-    Finder finder;
-    finder.init(a, T == 2 && !a.pair_heads ? 256 : 128);
-    uint32_t k_bits = 0, k_par = 0, v_bits = 0, v_par = 0;  // loads to drain on abort
-    uint32_t raw_uses = 0, q_par = 0, asked = 0;
-    int number = blockIdx.x;
-    Ring<KST> rk;
-    Ring<VST> rv;
-    bool ok = true;
-    auto ask = [&]() {
-      if (lane == 0) {
-        mbar_arrive_expect_tx(bar_next, 16);
-        cta_try_cancel(next_slot, bar_next);
-      }
-      ++asked;
-    };
-    for (uint32_t i = 0; ok && !(C::ONE && i); ++i) {
-      // the first item is the CTA's own, the others' owners are never launched
-      if (i) {
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_next, (asked - 1) & 1u, abort_flag, a.err,
-                                               kDevErrTimeoutPacked));
-        if (!ok) break;
-        number = cta_cancelled(next_slot);
-        __syncwarp();
-      }
-      Item it{0, 0, -1, 0};
-      while (number >= 0) {
-        it = finder.find(a, number / a.units);
-        if (C::ONE || it.tile >= 0) break;
-        // a number behind the last tile: the grid is an upper bound
-        ask();
-        ok = __all_sync(0xffffffffu, mbar_wait(bar_next, (asked - 1) & 1u, abort_flag, a.err,
-                                               kDevErrTimeoutPacked));
-        if (!ok) break;
-        number = cta_cancelled(next_slot);
-        __syncwarp();
-      }
-      if (!ok) break;
-      it.unit = number % a.units;
-      const int slot = i & 1;
-      ok = __all_sync(0xffffffffu, mbar_wait(bar_item_free + 8 * slot, (i >> 1 & 1) ^ 1, abort_flag,
-                                             a.err, kDevErrTimeoutPacked));
-      if (!ok) break;
-      if (lane == 0) items[slot] = it;
-      if (lane < 2) fix_tile[slot * 2 + lane] = 0;
-      if (lane < 8) fix_rows[slot * 8 + lane] = 0;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_item + 8 * slot);
-      if (it.tile < 0) break;
-      const Work w = work_of<T>(a, it);
-      if (lane == 0) {
-        ok = mbar_wait(bar_q_free, (i & 1) ^ 1, abort_flag, a.err, kDevErrTimeoutPacked);
-        for (int t = 0; t < T && ok; ++t) {
-          if (!w.n[t]) {  // nothing to load, but a phase like every item's
-            mbar_arrive(bar_q + 8 * t);
-            continue;
-          }
-          mbar_arrive_expect_tx(bar_q + 8 * t, C::TILE);
-          tma_load_3d(sbase + t * C::TILE, &map_q, bar_q + 8 * t, 0, w.row0 + w.qt[t],
-                      (w.ph ? w.head0 + t : w.head0) * C::HALVES);
-        }
-        if (ok) q_par = i + 1;
-      }
-      int fixes = 0;
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-      for (int j = 0; j < w.nmax && ok; ++j) {
-        // no earlier than the answer is needed, two tiles before the item's last MMA:
-        // until then it may fall to a CTA that is done before
-        if (!C::ONE && j == w.nmax - 1) ask();
-        // does some query of the CTA see a part of this tile only?
-        const bool diag = a.causal && (j == w.n[0] - 1 || j == w.n[1] - 1);
-        const bool fix = diag || (j + 1) * BKV > w.len;
+  if (warp >= 4 * T) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_OTHERS));
+    if (warp == C::PRODUCER) {
+      // ----------------------------------------------------------- producer
+      Finder finder;
+      finder.init(a, T == 2 && !a.pair_heads ? 256 : 128);
+      uint32_t k_bits = 0, k_par = 0, v_bits = 0, v_par = 0;  // loads to drain on abort
+      uint32_t raw_uses = 0, q_par = 0, asked = 0;
+      int number = blockIdx.x;
+      Ring<KST> rk;
+      Ring<VST> rv;
+      bool ok = true;
+      auto ask = [&]() {
         if (lane == 0) {
-          ok = mbar_wait(bar_k_empty + 8 * rk.st, rk.ph ^ 1, abort_flag, a.err,
-                         kDevErrTimeoutPacked);
-          if (ok) {
-            mbar_arrive_expect_tx(bar_k_full + 8 * rk.st, C::TILE);
-            tma_load_3d(sbase + C::OFF_K + rk.st * C::TILE, &map_k, bar_k_full + 8 * rk.st, 0,
-                        w.row0 + j * BKV, w.kv_head * C::HALVES);
-            k_bits |= 1u << rk.st;
-            k_par = (k_par & ~(1u << rk.st)) | (rk.ph << rk.st);
-            ok = mbar_wait(bar_v_empty + 8 * rv.st, rv.ph ^ 1, abort_flag, a.err,
-                           kDevErrTimeoutPacked);
+          mbar_arrive_expect_tx(bar_next, 16);
+          cta_try_cancel(next_slot, bar_next);
+        }
+        ++asked;
+      };
+      for (uint32_t i = 0; ok && !(C::ONE && i); ++i) {
+        // the first item is the CTA's own, the others' owners are never launched
+        if (i) {
+          ok = __all_sync(0xffffffffu, mbar_wait(bar_next, (asked - 1) & 1u, abort_flag, a.err,
+                                                 kDevErrTimeoutPacked));
+          if (!ok) break;
+          number = cta_cancelled(next_slot);
+          __syncwarp();
+        }
+        Item it{0, 0, -1, 0};
+        while (number >= 0) {
+          it = finder.find(a, number / a.units);
+          if (C::ONE || it.tile >= 0) break;
+          // a number behind the last tile: the grid is an upper bound
+          ask();
+          ok = __all_sync(0xffffffffu, mbar_wait(bar_next, (asked - 1) & 1u, abort_flag, a.err,
+                                                 kDevErrTimeoutPacked));
+          if (!ok) break;
+          number = cta_cancelled(next_slot);
+          __syncwarp();
+        }
+        if (!ok) break;
+        it.unit = number % a.units;
+        const int slot = i & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_item_free + 8 * slot, (i >> 1 & 1) ^ 1,
+                                               abort_flag, a.err, kDevErrTimeoutPacked));
+        if (!ok) break;
+        if (lane == 0) items[slot] = it;
+        if (lane < 2) fix_tile[slot * 2 + lane] = 0;
+        if (lane < 8) fix_rows[slot * 8 + lane] = 0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_item + 8 * slot);
+        if (it.tile < 0) break;
+        const Work w = work_of<T>(a, it);
+        if (lane == 0) {
+          ok = mbar_wait(bar_q_free, (i & 1) ^ 1, abort_flag, a.err, kDevErrTimeoutPacked);
+          for (int t = 0; t < T && ok; ++t) {
+            if (!w.n[t]) {  // nothing to load, but a phase like every item's
+              mbar_arrive(bar_q + 8 * t);
+              continue;
+            }
+            mbar_arrive_expect_tx(bar_q + 8 * t, C::TILE);
+            tma_load_3d(sbase + t * C::TILE, &map_q, bar_q + 8 * t, 0, w.row0 + w.qt[t],
+                        (w.ph ? w.head0 + t : w.head0) * C::HALVES);
           }
-          if (ok && fix) {
-            if (C::CHECKER)
+          if (ok) q_par = i + 1;
+        }
+        int fixes = 0;
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        for (int j = 0; j < w.nmax && ok; ++j) {
+          // no earlier than the answer is needed, two tiles before the item's last MMA:
+          // until then it may fall to a CTA that is done before
+          if (!C::ONE && j == w.nmax - 1) ask();
+          // does some query of the CTA see a part of this tile only?
+          const bool diag = a.causal && (j == w.n[0] - 1 || j == w.n[1] - 1);
+          const bool fix = diag || (j + 1) * BKV > w.len;
+          if (lane == 0) {
+            ok = mbar_wait(bar_k_empty + 8 * rk.st, rk.ph ^ 1, abort_flag, a.err,
+                           kDevErrTimeoutPacked);
+            if (ok) {
+              mbar_arrive_expect_tx(bar_k_full + 8 * rk.st, C::TILE);
+              tma_load_3d(sbase + C::OFF_K + rk.st * C::TILE, &map_k, bar_k_full + 8 * rk.st, 0,
+                          w.row0 + j * BKV, w.kv_head * C::HALVES);
+              k_bits |= 1u << rk.st;
+              k_par = (k_par & ~(1u << rk.st)) | (rk.ph << rk.st);
+              ok = mbar_wait(bar_v_empty + 8 * rv.st, rv.ph ^ 1, abort_flag, a.err,
+                             kDevErrTimeoutPacked);
+            }
+            if (ok && fix) {
               ok = mbar_wait(bar_raw_free, (raw_uses & 1u) ^ 1, abort_flag, a.err,
                              kDevErrTimeoutPacked);
-            raw[0] = rv.st;
-            raw[1] = w.len - j * BKV;
-            raw[2] = diag | (slot * 2 + fixes) << 1;  // at most two such tiles per item
-            raw[3] = j;
-          }
-          if (ok) {
-            const uint32_t bar = fix ? bar_v_raw : bar_v_full + 8 * rv.st;
-            mbar_arrive_expect_tx(bar, C::TILE);
-            tma_load_3d(sbase + C::OFF_V + rv.st * C::TILE, &map_v, bar, 0, w.row0 + j * BKV,
-                        w.kv_head * C::HALVES);
-            if (!fix) {
-              v_bits |= 1u << rv.st;
-              v_par = (v_par & ~(1u << rv.st)) | (rv.ph << rv.st);
-            } else {
-              v_bits &= ~(1u << rv.st);
+              raw[0] = rv.st;
+              raw[1] = w.len - j * BKV;
+              raw[2] = diag | (slot * 2 + fixes) << 1;  // at most two such tiles per item
+              raw[3] = j;
+            }
+            if (ok) {
+              const uint32_t bar = fix ? bar_v_raw : bar_v_full + 8 * rv.st;
+              mbar_arrive_expect_tx(bar, C::TILE);
+              tma_load_3d(sbase + C::OFF_V + rv.st * C::TILE, &map_v, bar, 0, w.row0 + j * BKV,
+                          w.kv_head * C::HALVES);
+              if (!fix) {
+                v_bits |= 1u << rv.st;
+                v_par = (v_par & ~(1u << rv.st)) | (rv.ph << rv.st);
+              } else {
+                v_bits &= ~(1u << rv.st);
+              }
             }
           }
-        }
-        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-        if (ok && fix) {
-          ++raw_uses;
-          if (!C::CHECKER) {
-            // drained here also on abort: the wait ignores the flag
-            ok = __all_sync(0xffffffffu, mbar_wait_drain(bar_v_raw, (raw_uses - 1) & 1u));
-            if (!ok && lane == 0) {
-              *abort_flag = 1;
-              atomicExch(a.err, kDevErrTimeoutPacked);
-            }
-            if (lane == 0) fix_tile[slot * 2 + fixes] = j;
-            __syncwarp();
-            look_through(rv.st, w.len - j * BKV, diag, slot * 2 + fixes, lane, 32);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar_v_full + 8 * rv.st);
+          ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+          if (ok && fix) {
+            ++raw_uses;
+            ++fixes;
           }
-          ++fixes;
+          rk.step();
+          rv.step();
         }
-        rk.step();
-        rv.step();
       }
-    }
-    if (C::CHECKER && ok && lane == 0 &&
-        mbar_wait(bar_raw_free, (raw_uses & 1u) ^ 1, abort_flag, a.err, kDevErrTimeoutPacked)) {
-      raw[0] = -1;  // warps 10 and 11 may go
-      mbar_arrive(bar_v_raw);
-    }
-    if (lane == 0 && *abort_flag) {
-      if (asked) mbar_wait_drain(bar_next, (asked - 1) & 1u);
-      if (C::CHECKER && raw_uses) mbar_wait_drain(bar_v_raw, (raw_uses - 1) & 1u);
-      for (int t = 0; t < T; ++t)
-        if (q_par) mbar_wait_drain(bar_q + 8 * t, (q_par - 1) & 1u);
-      for (int s = 0; s < KST; ++s)
-        if (k_bits & (1u << s)) mbar_wait_drain(bar_k_full + 8 * s, (k_par >> s) & 1u);
-      for (int s = 0; s < VST; ++s)
-        if (v_bits & (1u << s)) mbar_wait_drain(bar_v_full + 8 * s, (v_par >> s) & 1u);
-    }
-  } else if (warp == 1) {
-    // ----------------------------------------------------------- MMA issuer
-    // The whole warp runs this and one elected thread issues, so that what the MMAs
-    // take (descriptors, columns) is uniform to the compiler.
-    bool ok = true, issued = false;
-    auto wait = [&](uint32_t bar, uint32_t par) {
-      return __all_sync(0xffffffffu,
-                        mbar_wait(bar, par, abort_flag, a.err, kDevErrTimeoutPacked)) != 0;
-    };
-    Ring<KST> rk;   // of the next Q K^T
-    Ring<VST> rv;   // of the next P V
-    uint32_t n_p[2] = {0, 0};  // P tiles waited for
-    uint32_t n_s = 0;          // S tiles issued (P apart)
-    const uint64_t desc_q = umma_desc_sw128(sbase), desc_k = umma_desc_sw128(sbase + C::OFF_K);
-    // V tile: keys along K, head_dim along N in 64-wide groups HALF apart
-    const uint64_t desc_v = (umma_desc_sw128_mn(sbase + C::OFF_V) & ~(0x3FFFull << 16)) |
-                            ((uint64_t)(C::HALF >> 4) << 16);
-    for (uint32_t i = 0; ok && !(C::ONE && i); ++i) {
-      ok = wait(bar_item + 8 * (i & 1), i >> 1 & 1);
-      if (!ok) break;
-      const Item it = items[i & 1];
-      const Work w = work_of<T>(a, it);
-      const bool none = __shfl_sync(0xffffffffu, it.tile, 0) < 0;
-      const int n0 = __shfl_sync(0xffffffffu, w.n[0], 0), n1 = __shfl_sync(0xffffffffu, w.n[1], 0);
-      const int nmax = max(n0, n1);
-      if (lane == 0) mbar_arrive(bar_item_free + 8 * (i & 1));
-      if (none) break;
-      auto last_of = [&](int j) { return T == 2 && j < n1 ? 1 : 0; };
-      auto issue_qk = [&](int t, int j) {
-        const uint64_t dq = desc_advance(desc_q, t * C::TILE);
-        const uint64_t dk = desc_advance(desc_k, rk.st * C::TILE);
-        const bool last = t == last_of(j);
-        if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk / 4) * C::HALF + (kk % 4) * 32;
-            umma_f16_ss(tmem + C::S(t), desc_advance(dq, off), desc_advance(dk, off), IDESC_S,
-                        kk != 0);
-          }
-          umma_commit(bar_s_full + 8 * t);
-          if (last) umma_commit(bar_k_empty + 8 * rk.st);
-          if (last && j == nmax - 1) umma_commit(bar_q_free);
-        }
-        issued = true;
-        if (last) rk.step();
+      if (ok && lane == 0 &&
+          mbar_wait(bar_raw_free, (raw_uses & 1u) ^ 1, abort_flag, a.err, kDevErrTimeoutPacked)) {
+        raw[0] = -1;  // the checkers may go
+        mbar_arrive(bar_v_raw);
+      }
+      if (lane == 0 && *abort_flag) {
+        if (asked) mbar_wait_drain(bar_next, (asked - 1) & 1u);
+        if (raw_uses) mbar_wait_drain(bar_v_raw, (raw_uses - 1) & 1u);
+        for (int t = 0; t < T; ++t)
+          if (q_par) mbar_wait_drain(bar_q + 8 * t, (q_par - 1) & 1u);
+        for (int s = 0; s < KST; ++s)
+          if (k_bits & (1u << s)) mbar_wait_drain(bar_k_full + 8 * s, (k_par >> s) & 1u);
+        for (int s = 0; s < VST; ++s)
+          if (v_bits & (1u << s)) mbar_wait_drain(bar_v_full + 8 * s, (v_par >> s) & 1u);
+      }
+    } else if (warp == C::ISSUER) {
+      // ----------------------------------------------------------- MMA issuer
+      // The whole warp runs this and one elected thread issues, so that what the MMAs
+      // take (descriptors, columns) is uniform to the compiler.
+      bool ok = true, issued = false;
+      auto wait = [&](uint32_t bar, uint32_t par) {
+        return __all_sync(0xffffffffu,
+                          mbar_wait(bar, par, abort_flag, a.err, kDevErrTimeoutPacked)) != 0;
       };
-      auto issue_pv = [&](int t, int j) {
-        const uint64_t dv = desc_advance(desc_v, rv.st * C::TILE);
-        const bool last = t == last_of(j);
-        if (elect_one()) {
+      Ring<KST> rk;   // of the next Q K^T
+      Ring<VST> rv;   // of the next P V
+      uint32_t n_p[2] = {0, 0};  // P tiles waited for
+      uint32_t n_s = 0;          // S tiles issued (P apart)
+      const uint64_t desc_q = umma_desc_sw128(sbase), desc_k = umma_desc_sw128(sbase + C::OFF_K);
+      // V tile: keys along K, head_dim along N in 64-wide groups HALF apart
+      const uint64_t desc_v = (umma_desc_sw128_mn(sbase + C::OFF_V) & ~(0x3FFFull << 16)) |
+                              ((uint64_t)(C::HALF >> 4) << 16);
+      for (uint32_t i = 0; ok && !(C::ONE && i); ++i) {
+        ok = wait(bar_item + 8 * (i & 1), i >> 1 & 1);
+        if (!ok) break;
+        const Item it = items[i & 1];
+        const Work w = work_of<T>(a, it);
+        const bool none = __shfl_sync(0xffffffffu, it.tile, 0) < 0;
+        const int n0 = __shfl_sync(0xffffffffu, w.n[0], 0);
+        const int n1 = __shfl_sync(0xffffffffu, w.n[1], 0);
+        const int nmax = max(n0, n1);
+        if (lane == 0) mbar_arrive(bar_item_free + 8 * (i & 1));
+        if (none) break;
+        auto last_of = [&](int j) { return T == 2 && j < n1 ? 1 : 0; };
+        auto issue_qk = [&](int t, int j) {
+          const uint64_t dq = desc_advance(desc_q, t * C::TILE);
+          const uint64_t dk = desc_advance(desc_k, rk.st * C::TILE);
+          const bool last = t == last_of(j);
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < BKV / 16; ++kk)
-            umma_f16_ts(tmem + C::O(t), tmem + C::P(t) + kk * 8, desc_advance(dv, kk * 2048),
-                        IDESC_O, (j | kk) != 0);
-          if (!C::OVERLAY) umma_commit(bar_o_full);
-          if (last) umma_commit(bar_v_empty + 8 * rv.st);
-          if (j == (t ? n1 : n0) - 1) umma_commit(bar_o_done + 8 * t);
-        }
-        if (last) rv.step();
-      };
-      ok = wait(bar_q, i & 1) && wait(bar_k_full + 8 * rk.st, rk.ph);
-      if (C::OVERLAY) {
-        if (ok) {
-          tc_fence_after();
-          issue_qk(0, 0);
-          if (n1) {
-            ok = wait(bar_q + 8 * (T - 1), i & 1);
-            if (ok) issue_qk(1, 0);
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = (kk / 4) * C::HALF + (kk % 4) * 32;
+              umma_f16_ss(tmem + C::S(t), desc_advance(dq, off), desc_advance(dk, off), IDESC_S,
+                          kk != 0);
+            }
+            umma_commit(bar_s_full + 8 * t);
+            if (last) umma_commit(bar_k_empty + 8 * rk.st);
+            if (last && j == nmax - 1) umma_commit(bar_q_free);
           }
-        }
-        for (int j = 0; j < nmax && ok; ++j) {
-          bool v_here = false, k_here = false;
-#pragma unroll
-          for (int t = 0; t < T; ++t) {
-            const int n = t ? n1 : n0;
-            if (j >= n || !ok) continue;
-            // V and the next K are early as a rule: their waits come first, so that
-            // nothing stands between P and its MMAs
-            const bool more = j + 1 < n;
-            ok = (v_here || wait(bar_v_full + 8 * rv.st, rv.ph)) &&
-                 (!more || k_here || wait(bar_k_full + 8 * rk.st, rk.ph));
-            v_here = true;
-            k_here |= more;
-            ok = ok && wait(bar_p_full + 8 * t, n_p[t]++ & 1u);
-            if (!ok) continue;
-            tc_fence_after();
-            issue_pv(t, j);
-            if (more) issue_qk(t, j + 1);
-          }
-        }
-      } else {
-        // S is free once the softmax has read the tile before
-        auto next_s = [&](int j) {
-          ok = wait(bar_k_full + 8 * rk.st, rk.ph) && (n_s == 0 || wait(bar_s_free, (n_s - 1) & 1u));
-          if (!ok) return;
-          tc_fence_after();
-          issue_qk(0, j);
-          ++n_s;
+          issued = true;
+          if (last) rk.step();
         };
-        if (ok) next_s(0);
-        if (ok && nmax > 1) next_s(1);
-        for (int j = 0; j < nmax && ok; ++j) {
-          ok = wait(bar_p_full, n_p[0]++ & 1u) && wait(bar_v_full + 8 * rv.st, rv.ph);
-          if (!ok) break;
-          tc_fence_after();
-          issue_pv(0, j);
-          if (j + 2 < nmax) next_s(j + 2);
+        auto issue_pv = [&](int t, int j) {
+          const uint64_t dv = desc_advance(desc_v, rv.st * C::TILE);
+          const bool last = t == last_of(j);
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < BKV / 16; ++kk)
+              umma_f16_ts(tmem + C::O(t), tmem + C::P(t) + kk * 8, desc_advance(dv, kk * 2048),
+                          IDESC_O, (j | kk) != 0);
+            if (!C::OVERLAY) umma_commit(bar_o_full);
+            if (last) umma_commit(bar_v_empty + 8 * rv.st);
+            if (j == (t ? n1 : n0) - 1) umma_commit(bar_o_done + 8 * t);
+          }
+          if (last) rv.step();
+        };
+        ok = wait(bar_q, i & 1) && wait(bar_k_full + 8 * rk.st, rk.ph);
+        if (C::OVERLAY) {
+          if (ok) {
+            tc_fence_after();
+            issue_qk(0, 0);
+            if (n1) {
+              ok = wait(bar_q + 8 * (T - 1), i & 1);
+              if (ok) issue_qk(1, 0);
+            }
+          }
+          for (int j = 0; j < nmax && ok; ++j) {
+            bool v_here = false, k_here = false;
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+              const int n = t ? n1 : n0;
+              if (j >= n || !ok) continue;
+              // V and the next K are early as a rule: their waits come first, so that
+              // nothing stands between P and its MMAs
+              const bool more = j + 1 < n;
+              ok = (v_here || wait(bar_v_full + 8 * rv.st, rv.ph)) &&
+                   (!more || k_here || wait(bar_k_full + 8 * rk.st, rk.ph));
+              v_here = true;
+              k_here |= more;
+              ok = ok && wait(bar_p_full + 8 * t, n_p[t]++ & 1u);
+              if (!ok) continue;
+              tc_fence_after();
+              issue_pv(t, j);
+              if (more) issue_qk(t, j + 1);
+            }
+          }
+        } else {
+          // S is free once the softmax has read the tile before
+          auto next_s = [&](int j) {
+            ok = wait(bar_k_full + 8 * rk.st, rk.ph) &&
+                 (n_s == 0 || wait(bar_s_free, (n_s - 1) & 1u));
+            if (!ok) return;
+            tc_fence_after();
+            issue_qk(0, j);
+            ++n_s;
+          };
+          if (ok) next_s(0);
+          if (ok && nmax > 1) next_s(1);
+          for (int j = 0; j < nmax && ok; ++j) {
+            ok = wait(bar_p_full, n_p[0]++ & 1u) && wait(bar_v_full + 8 * rv.st, rv.ph);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(0, j);
+            if (j + 2 < nmax) next_s(j + 2);
+          }
         }
       }
-    }
-    if (__any_sync(0xffffffffu, *abort_flag) && issued) {
-      if (elect_one()) umma_commit(bar_drain);
-      mbar_wait_drain(bar_drain, 0);
-    }
-  } else if (C::CHECKER && warp >= 2 + 4 * T) {
-    // ----------------------------------------------------------- V tiles
-    const int id = threadIdx.x - 32 * (2 + 4 * T);
-    for (uint32_t u = 0;; ++u) {
-      const bool there = __all_sync(
-          0xffffffffu, mbar_wait(bar_v_raw, u & 1u, abort_flag, a.err, kDevErrTimeoutPacked));
-      if (id == 0) raw[4] = there;  // one decision for both warps
-      asm volatile("barrier.cta.sync 3, 64;" ::: "memory");
-      const int st = raw[0], held = raw[1], flags = raw[2], j = raw[3];
-      const bool go = raw[4] && st >= 0;
-      asm volatile("barrier.cta.sync 3, 64;" ::: "memory");
-      if (!go) break;
-      if (id == 0) fix_tile[flags >> 1] = j;
-      look_through(st, held, flags & 1, flags >> 1, id, 64);
-      asm volatile("barrier.cta.sync 3, 64;" ::: "memory");
-      if (id == 0) {
-        mbar_arrive(bar_v_full + 8 * st);
-        mbar_arrive(bar_raw_free);
+      if (__any_sync(0xffffffffu, *abort_flag) && issued) {
+        if (elect_one()) umma_commit(bar_drain);
+        mbar_wait_drain(bar_drain, 0);
+      }
+    } else {
+      // ----------------------------------------------------------- V tiles
+      const int id = threadIdx.x - 32 * C::CHECKER;
+      for (uint32_t u = 0;; ++u) {
+        const bool there = __all_sync(
+            0xffffffffu, mbar_wait(bar_v_raw, u & 1u, abort_flag, a.err, kDevErrTimeoutPacked));
+        if (id == 0) raw[4] = there;  // one decision for both warps
+        asm volatile("barrier.cta.sync 3, 64;" ::: "memory");
+        const int st = raw[0], held = raw[1], flags = raw[2], j = raw[3];
+        const bool go = raw[4] && st >= 0;
+        asm volatile("barrier.cta.sync 3, 64;" ::: "memory");
+        if (!go) break;
+        if (id == 0) fix_tile[flags >> 1] = j;
+        look_through(st, held, flags & 1, flags >> 1, id);
+        asm volatile("barrier.cta.sync 3, 64;" ::: "memory");
+        if (id == 0) {
+          mbar_arrive(bar_v_full + 8 * st);
+          mbar_arrive(bar_raw_free);
+        }
       }
     }
   } else {
     // ----------------------------------------------------------- softmax rows
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS));
     constexpr float kRescaleLog2 = 8.0f;
-    const int t = T == 2 ? (warp - 2) >> 2 : 0;
+    const int t = T == 2 ? warp >> 2 : 0;
     const int quad = warp & 3;  // this warp's TMEM lane quadrant
     const int r = quad * 32 + lane;
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
@@ -713,16 +712,29 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
         ok = wait(bar_s_full + 8 * t, tiles & 1u);
         if (!ok) break;
         tc_fence_after();
+        // Masked scores become -inf in tensor memory, so that the code below is the
+        // same for all tiles (selects in it cost every tile: 95 against 88 us for the
+        // ragged batch above).
+        if ((j + 1) * BKV > lim_min) {
+          const int valid = lim - j * BKV;
+#pragma unroll 1
+          for (int g = __reduce_min_sync(0xffffffffu, valid) >> 5; g < BKV / 32; ++g) {
+            uint32_t s[32];
+            tmem_ld_32x32b_x32(s_col + 32 * g, s);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (32 * g + e >= valid) s[e] = __float_as_uint(-INFINITY);
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+              tmem_st_32x32b_x16(s_col + 32 * g + 16 * q,
+                                 *reinterpret_cast<uint32_t(*)[16]>(s + 16 * q));
+          }
+          tmem_wait_st();
+        }
         uint32_t v[BKV];
-        const bool edge = (j + 1) * BKV > lim_min;
-        const int valid = lim - j * BKV;
         float mx[4];
         auto half_max = [&](int h0) {
-          if (edge) {
-#pragma unroll
-            for (int e = 0; e < BKV / 2; ++e)
-              if (h0 * 32 + e >= valid) v[h0 * 32 + e] = __float_as_uint(-INFINITY);
-          }
 #pragma unroll
           for (int q = h0; q < h0 + 2; ++q) {
             float m = fmaxf(__uint_as_float(v[32 * q]), __uint_as_float(v[32 * q + 31]));
@@ -800,7 +812,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
         tc_fence_after();
         const float inv = 1.f / l_run;
         const Work w = work_of<T>(a, item());
-        const int q0 = T == 2 && t ? w.qt[1] : w.qt[0], pos = q0 + r, len = w.len;
+        const int q0 = T == 2 && t ? w.qt[1] : w.qt[0], len = w.len;
         const int head = w.ph ? w.head0 + t : w.head0;
         uint32_t fixes = 0;
 #pragma unroll
@@ -877,7 +889,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
+  if (warp == C::ISSUER) {
     tc_fence_after();
     tmem_dealloc(tmem, C::COLS);
   }
@@ -946,7 +958,8 @@ sam3_status_t attention_packed(sam3_ctx_t* ctx, int dtype, const uint16_t* q, in
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o))
     return set_error(ctx, SAM3_ERR_INVALID_ARG, "attention_packed: rows must be 16-byte aligned");
   if (!scale_ok(scale))
-    return set_error(ctx, SAM3_ERR_INVALID_ARG, "attention_packed: scale must be positive and finite");
+    return set_error(ctx, SAM3_ERR_INVALID_ARG,
+                     "attention_packed: scale must be positive and finite");
   if (head_dim != 64 && head_dim != 128)
     return set_error(ctx, SAM3_ERR_SHAPE, "attention_packed: head_dim must be 64 or 128 (got %d)",
                      head_dim);
