@@ -17,43 +17,46 @@
 //     two O of 128); the next Q K^T of a tile is issued right behind the P V
 //     that reads P: the tensor pipe runs one thread's MMAs in order. While one
 //     tile's MMAs run, the other's softmax does.
-// Warps: 0 TMA producer, 1 TMEM allocator and MMA issuer (one thread), then
-// four softmax warps per query tile, one thread per row: the row's 128 scores
-// to registers, maximum, exponentials, P back to TMEM. O is rescaled in place,
-// and only when a row's maximum grew by more than 2^8. For head_dim 128 two
-// more warps look through V tiles (below).
+// Warps: four of softmax per query tile, one thread per row (the row's 128
+// scores to registers, maximum, exponentials, P back to TMEM), then the TMA
+// producer, the MMA issuer, and two that look through V tiles (below). O is
+// rescaled in place, and only when a row's maximum grew by more than 2^8. The
+// issuing warp stays converged and one elected thread issues: with a lone lane
+// an MMA took 87 clocks to issue, more than the 64 that one of 128 x 128 x 16
+// runs (8192 causal rows, 32 heads on 8: 487 -> 440 us). Registers go to the
+// softmax warps (setmaxnreg), so that nothing spills: 448 -> 435 us.
 //
 // Work: a tile of every sequence and head, longest first, so that the last to
-// finish are short (Finder). head_dim 64: a CTA each; the SM's other CTA covers
-// its begin and end. head_dim 128: the grid is as large, but a running CTA takes
+// finish are short (Finder). The grid has a CTA for each, but a running CTA takes
 // over the items of CTAs that are not launched yet (clusterlaunchcontrol), so
-// that the next item's loads and first MMAs run under this one's last tiles:
-// 16 causal sequences of 17 to 2048 rows (7,445 in all, 32 heads on 8) take 108 us,
-// dealt out in the same order to one CTA per SM beforehand 114. Results leave
-// through shared memory and TMA stores, for which nobody waits (125 us to 114).
+// that the next item's loads and first MMAs run under this one's last tiles: 16
+// causal sequences of 17 to 2048 rows (7,445 in all, 32 heads on 8 of 128) took
+// 108 us with it when the same order dealt out beforehand took 114, and four
+// images' tokens with head_dim 64 took 210 when a CTA per item took 218. Results
+// leave through shared memory and TMA stores, for which nobody waits.
 //
-// Masked places: scores are replaced before the maximum, whatever they are. V
-// needs more, because 0 * inf is NaN: in a sequence's last key tile and in the
-// causal diagonal ones the V rows behind the sequence's end become 0 and, on
-// the diagonal, so do the infinities and NaN of rows that only some queries
-// see, before the MMA reads the tile; those are added to the rows that see them
-// at the end (rare; read again from global memory). head_dim 64: the producer
-// warp does this, head_dim 128: warps 10 and 11, since there the producer's
-// loads are late by it (8192 causal rows, 32 heads on 8: 525 against 500 us).
+// Masked places: scores become -inf in tensor memory before the tile is read,
+// whatever they are. V needs more, because 0 * inf is NaN: in a sequence's last
+// key tile and in the causal diagonal ones the V rows behind the sequence's end
+// become 0 and, on the diagonal, so do the infinities and NaN of rows that only
+// some queries see, before the MMA reads the tile; those are added to the rows
+// that see them at the end (rare; read again from global memory).
 //
 // P is rounded to the inputs' type, as tcgen05 takes both operands in one: half
 // a step (fp16 2^-11, bf16 2^-8) of each weight.
 //
-// Bounds, measured: head_dim 64 by the softmax warps' issue slots, of them the
-// exponentials alone (16 per clock and SM) 133 us where the MMAs need 94: four
-// images' tokens (2592, 1733, 5184 and 901 rows, 16 heads) 237 us, 645 TFLOP/s;
-// 16 times 5184 rows 2.63 ms, 717 TFLOP/s. head_dim 128 by the chain from the
-// scores through the softmax to the next MMAs of a tile, with only one other
-// tile to fill the pipe meanwhile: 8192 causal rows, 32 heads on 8, 488 us,
-// 1127 TFLOP/s, 69 % of cuBLAS's burst rate. Tried and slower at head_dim 128: P in two halves with its
-// own commits (526 -> 571 us), an issuer that polls for whatever is ready (487 ->
-// 705), a part of the exponentials as polynomials (1/8: 492, 1/4: 527), skipping
-// masked 32-key groups of diagonal tiles (505 -> 545, a branch in the loop).
+// Bounds, measured. head_dim 64: the exponentials (16 per clock and SM; packed
+// FMAs and additions beside them leave them 90 % of it). Four images' tokens
+// (2592, 1733, 5184 and 901 rows, 16 heads): 210 us, 731 TFLOP/s, where the
+// exponentials alone need 133 us and the MMAs 94. head_dim 128: exponentials
+// and MMAs need about the same time (1024 clocks each for a 128 x 128 tile), and
+// the chain from a tile's scores through its softmax to its next scores has only
+// one other tile beside it: 8192 causal rows, 32 heads on 8, 435 us, 1265
+// TFLOP/s, 77 % of cuBLAS's burst rate; under load for seconds the power limit
+// holds it to 1070. Tried and no faster at head_dim 128: P told in two parts
+// (96 + 32 keys 446, 64 + 64 449 against 444 us), K and V looked at between P V
+// and Q K^T (453), an issuer that polls for whatever is ready, a part of the
+// exponentials as polynomials.
 #include <algorithm>
 
 #include "common.cuh"
@@ -65,26 +68,24 @@ namespace sam3 {
 namespace {
 
 constexpr int BQ = 128, BKV = 128;
-constexpr int VST = 2;
+constexpr int KST = 2, VST = 2;  // K and V tiles in shared memory
 
 template <int D>
 struct PK {
   static constexpr int T = D == 128 ? 2 : 1;     // query tiles per CTA
   static constexpr bool OVERLAY = D == 128;      // P in its S's columns
   static constexpr int HALVES = D / 64;          // 128-byte wide parts of a tile
-  static constexpr bool ONE = D == 64;           // a CTA takes one item, else items in turn
   // Warps: four of softmax per tile, then a warpgroup of others. The registers of
   // the launch (2 x 256 x 128 or 384 x 168 per SM) are split among them.
   static constexpr int PRODUCER = 4 * T, ISSUER = 4 * T + 1, CHECKER = 4 * T + 2;
   static constexpr int THREADS = 128 * (T + 1);
   static constexpr int REGS = D == 128 ? 208 : 192, REGS_OTHERS = D == 128 ? 88 : 64;
-  static constexpr int KST = D == 128 ? 2 : 3;   // K tiles in shared memory
   static constexpr int TILE = BKV * D * 2;       // bytes of a Q, K or V tile
   static constexpr int HALF = BKV * 128;
   static constexpr int OFF_K = T * TILE;
   static constexpr int OFF_V = OFF_K + KST * TILE;
   static constexpr int OFF_OUT = OFF_V + VST * TILE;  // [T] 128 rows of 64 outputs
-  static constexpr int OFF_BAR = OFF_OUT + (T == 2 ? T * HALF : 0);
+  static constexpr int OFF_BAR = OFF_OUT + T * HALF;
   static constexpr int BARS = 4 * T + 2 * KST + 2 * VST + 11;
   static constexpr int OFF_MISC = (OFF_BAR + BARS * 8 + 15) / 16 * 16;
   static constexpr int MISC = 192;
@@ -107,6 +108,7 @@ struct PackedArgs {
   int n_seqs, rows, group;
   int pair_heads;  // the CTA's two tiles are two heads (else 256 rows of one)
   int units;       // heads, or pairs of heads
+  unsigned resident;  // CTAs that run at once
   int causal;
   float c;         // scale * log2(e)
 };
@@ -276,7 +278,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
                        const __grid_constant__ CUtensorMap map_v,
                        const __grid_constant__ CUtensorMap map_o, const PackedArgs a) {
   using C = PK<D>;
-  constexpr int T = C::T, KST = C::KST;
+  constexpr int T = C::T;
   constexpr uint32_t FMT = BF ? (1u << 7) | (1u << 10) : 0u;  // bf16 operands
   constexpr uint32_t IDESC_S = umma_idesc_f16(128, BKV, 0) | FMT;
   constexpr uint32_t IDESC_O = umma_idesc_f16(128, D, 1) | FMT;
@@ -411,33 +413,33 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
       Ring<KST> rk;
       Ring<VST> rv;
       bool ok = true;
+      // The first item is the CTA's own, the next ones those of CTAs that are then
+      // never launched: where all run at once there is nothing to take over.
+      const bool others = gridDim.x > a.resident;
       auto ask = [&]() {
+        if (!others) return;
         if (lane == 0) {
           mbar_arrive_expect_tx(bar_next, 16);
           cta_try_cancel(next_slot, bar_next);
         }
         ++asked;
       };
-      for (uint32_t i = 0; ok && !(C::ONE && i); ++i) {
-        // the first item is the CTA's own, the others' owners are never launched
-        if (i) {
-          ok = __all_sync(0xffffffffu, mbar_wait(bar_next, (asked - 1) & 1u, abort_flag, a.err,
-                                                 kDevErrTimeoutPacked));
-          if (!ok) break;
-          number = cta_cancelled(next_slot);
-          __syncwarp();
-        }
+      auto answer = [&]() {
+        number = -1;
+        if (!others) return;
+        ok = __all_sync(0xffffffffu, mbar_wait(bar_next, (asked - 1) & 1u, abort_flag, a.err,
+                                               kDevErrTimeoutPacked));
+        if (ok) number = cta_cancelled(next_slot);
+        __syncwarp();
+      };
+      for (uint32_t i = 0; ok; ++i) {
+        if (i) answer();
         Item it{0, 0, -1, 0};
         while (number >= 0) {
           it = finder.find(a, number / a.units);
-          if (C::ONE || it.tile >= 0) break;
-          // a number behind the last tile: the grid is an upper bound
-          ask();
-          ok = __all_sync(0xffffffffu, mbar_wait(bar_next, (asked - 1) & 1u, abort_flag, a.err,
-                                                 kDevErrTimeoutPacked));
-          if (!ok) break;
-          number = cta_cancelled(next_slot);
-          __syncwarp();
+          if (it.tile >= 0) break;
+          ask();  // a number behind the last tile: the grid is an upper bound
+          answer();
         }
         if (!ok) break;
         it.unit = number % a.units;
@@ -470,7 +472,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
         for (int j = 0; j < w.nmax && ok; ++j) {
           // no earlier than the answer is needed, two tiles before the item's last MMA:
           // until then it may fall to a CTA that is done before
-          if (!C::ONE && j == w.nmax - 1) ask();
+          if (j == w.nmax - 1) ask();
           // does some query of the CTA see a part of this tile only?
           const bool diag = a.causal && (j == w.n[0] - 1 || j == w.n[1] - 1);
           const bool fix = diag || (j + 1) * BKV > w.len;
@@ -548,7 +550,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
       // V tile: keys along K, head_dim along N in 64-wide groups HALF apart
       const uint64_t desc_v = (umma_desc_sw128_mn(sbase + C::OFF_V) & ~(0x3FFFull << 16)) |
                               ((uint64_t)(C::HALF >> 4) << 16);
-      for (uint32_t i = 0; ok && !(C::ONE && i); ++i) {
+      for (uint32_t i = 0; ok; ++i) {
         ok = wait(bar_item + 8 * (i & 1), i >> 1 & 1);
         if (!ok) break;
         const Item it = items[i & 1];
@@ -682,10 +684,9 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
     auto wait = [&](uint32_t bar, uint32_t par) {
       return __all_sync(0xffffffffu, mbar_wait(bar, par, abort_flag, a.err, kDevErrTimeoutPacked));
     };
-    // this warp's rows of 64 outputs (head_dim 64: in the queries' place)
-    uint8_t* out = smem + (T == 2 ? C::OFF_OUT + t * C::HALF : 0) + quad * 4096;
+    uint8_t* out = smem + C::OFF_OUT + t * C::HALF + quad * 4096;  // this warp's rows of 64 outputs
     uint32_t tiles = 0, outs = 0;  // key tiles and items of this query tile so far
-    for (uint32_t i = 0; !(C::ONE && i); ++i) {
+    for (uint32_t i = 0;; ++i) {
       if (!wait(bar_item + 8 * (i & 1), i >> 1 & 1)) break;
       // What the key loop needs of the item and no more: its registers are scarce.
       // The item is read again for its end.
@@ -708,13 +709,11 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
       float m_run = -3.402823466e38f, l_run = 0.f;
       bool ok = true;
       for (int j = 0; j < n; ++j, ++tiles) {
-        if (C::ONE) tiles = j;
         ok = wait(bar_s_full + 8 * t, tiles & 1u);
         if (!ok) break;
         tc_fence_after();
         // Masked scores become -inf in tensor memory, so that the code below is the
-        // same for all tiles (selects in it cost every tile: 95 against 88 us for the
-        // ragged batch above).
+        // same for all tiles.
         if ((j + 1) * BKV > lim_min) {
           const int valid = lim - j * BKV;
 #pragma unroll 1
@@ -853,10 +852,8 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
           // Through shared memory (the warp's own 32 rows, 128-byte swizzle): one
           // TMA store takes them, and nobody waits for it. Where the sequence ends
           // among the rows, lanes store what is there, four whole lines at a time.
-          if (C::T == 2) {
-            if (lane == 0) bulk_wait_read();  // the store before has read the buffer
-            __syncwarp();
-          }
+          if (lane == 0) bulk_wait_read();  // the store before has read the buffer
+          __syncwarp();
 #pragma unroll
           for (int c8 = 0; c8 < 8; ++c8)
             *reinterpret_cast<uint4*>(out + lane * 128 + ((c8 ^ (lane & 7)) << 4)) =
@@ -934,11 +931,8 @@ sam3_status_t launch_packed(sam3_ctx_t* ctx, const uint16_t* q, int64_t q_stride
   const long long tiles = a.rows / span + std::min(a.n_seqs, a.rows);
   if (tiles * a.units > 0x7FFFFFFFll)
     return set_error(ctx, SAM3_ERR_SHAPE, "attention_packed: too many rows for one call");
-  // 64: a CTA per item; the other CTA of the SM covers its begin and end. 128: one
-  // CTA per SM, which takes over the items of CTAs not yet launched, the next
-  // item's loads and first MMAs under this one's last tiles.
-  const long long items = tiles * a.units;
-  const unsigned grid = (unsigned)items;
+  const unsigned grid = (unsigned)(tiles * a.units);
+  a.resident = ctx->num_sms * (D == 128 ? 1 : 2);
   const cudaError_t e = launch_pdl(packed_attn_kernel<D, BF>, dim3(grid), dim3(C::THREADS), C::SMEM,
                                    ctx->stream, mq, mk, mv, mo, a);
   return check_launch_ret(ctx, e, "packed_attn_kernel");
