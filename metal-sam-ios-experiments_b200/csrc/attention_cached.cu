@@ -197,15 +197,20 @@ __device__ __forceinline__ uint32_t nan_codes(uint32_t w) {
 struct Seq {
   int len, row0, fresh;
 };
-__device__ __forceinline__ Seq load_seq(const CachedArgs& a, int i, bool report) {
-  Seq s;
-  s.len = a.lens[i];
-  s.row0 = a.cu ? a.cu[i] : i;
-  const int r1 = a.cu ? a.cu[i + 1] : i + 1;
-  const bool ok = tokens_fit(s.row0, r1, a.rows, a.max_new, s.len, a.table_stride, a.page_shift);
+struct RawSeq {
+  int len, row0, row1;
+};
+__device__ __forceinline__ RawSeq fetch_seq(const CachedArgs& a, int i) {
+  return {a.lens[i], a.cu ? a.cu[i] : i, a.cu ? a.cu[i + 1] : i + 1};
+}
+__device__ __forceinline__ Seq checked_seq(const CachedArgs& a, const RawSeq& r, bool report) {
+  const bool ok =
+      tokens_fit(r.row0, r.row1, a.rows, a.max_new, r.len, a.table_stride, a.page_shift);
   if (!ok && report) atomicExch(a.err, kDevErrBadLengths);
-  s.fresh = ok ? r1 - s.row0 : 0;
-  return s;
+  return {r.len, r.row0, ok ? r.row1 - r.row0 : 0};
+}
+__device__ __forceinline__ Seq load_seq(const CachedArgs& a, int i) {
+  return checked_seq(a, fetch_seq(a, i), false);
 }
 
 // A run of cost over the items (sequence; K/V head and row block): an item costs
@@ -253,7 +258,7 @@ struct Run {
         left = 0;
         return;
       }
-      enter(load_seq(a, seq, false), a.group);
+      enter(load_seq(a, seq), a.group);
     } while (units == 0);
   }
 };
@@ -340,8 +345,10 @@ __global__ void __launch_bounds__(THREADS, 2)
   griddep_wait();  // lengths, pages, codes and queries may be earlier kernels' outputs
 
   // ------------------------------------------------- this CTA's run
-  // Each warp plans for itself (no barrier): lane l sums the costs of the
-  // sequences [l * m, l * m + m), as single tiles and as units of UNIT_TILES.
+  // Each warp plans for itself (no barrier): lane l gets the costs of the 32
+  // sequences from 32 l on, as single tiles and as units of UNIT_TILES.
+  // (Whole lines of lengths at a time: with 32 sequences in a row to each lane the
+  // plan of 1000 took 25 us.)
   const int m = (a.n_seqs + 31) / 32;
   auto cost_of = [&](const Seq& s, bool units) {
     if (s.fresh == 0) return 0;
@@ -350,12 +357,24 @@ __global__ void __launch_bounds__(THREADS, 2)
     return (units ? (tiles + UNIT_TILES - 1) / UNIT_TILES : tiles + ITEM_COST) * items;
   };
   int sum_tiles = 0, sum_units = 0;
-#pragma unroll 4
-  for (int j = 0; j < m; ++j) {
-    Seq s{0, 0, 0};
-    if (lane * m + j < a.n_seqs) s = load_seq(a, lane * m + j, blockIdx.x == 0 && warp == 0);
-    sum_tiles += cost_of(s, false);
-    sum_units += cost_of(s, true);
+  for (int j0 = 0; j0 < m; j0 += 8) {  // loads of 256 sequences in flight
+    RawSeq r[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int i = 32 * (j0 + j) + lane;
+      r[j] = i < a.n_seqs ? fetch_seq(a, i) : RawSeq{0, 0, 0};
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j0 + j >= m) break;
+      const Seq s = checked_seq(a, r[j], blockIdx.x == 0 && warp == 0);
+      const int n_tiles = __reduce_add_sync(0xffffffffu, cost_of(s, false));
+      const int n_units = __reduce_add_sync(0xffffffffu, cost_of(s, true));
+      if (lane == j0 + j) {
+        sum_tiles = n_tiles;
+        sum_units = n_units;
+      }
+    }
   }
   // Few tiles: runs of whole units of UNIT_TILES, so that short items are not cut
   // (a piece costs a join, about as much as four tiles), as long as no CTA gets
@@ -363,12 +382,15 @@ __global__ void __launch_bounds__(THREADS, 2)
   const bool few = a.whole || __reduce_add_sync(0xffffffffu, sum_units) <= (int)gridDim.x;
   const int ut = few ? UNIT_TILES : 1, extra = few ? 0 : ITEM_COST;
   const int own = few ? sum_units : sum_tiles;
-  int upto = own;
+  auto sums_to_here = [&](int v) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += v;
-  }
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    return v;
+  };
+  const int upto = sums_to_here(own);
   const int total = __shfl_sync(0xffffffffu, upto, 31);
   // equal runs, without a gap between the CTAs that have one (the join's order)
   const int ctas = min((int)gridDim.x, total), cta = min((int)blockIdx.x, ctas);
@@ -378,22 +400,17 @@ __global__ void __launch_bounds__(THREADS, 2)
   Run<D, RB> run;
   bool busy = cost > 0;
   if (busy) {
-    const int l = __ffs(__ballot_sync(0xffffffffu, upto > x0)) - 1;  // whose sequences x0 is in
-    int at = x0 - (upto - own), seq = lane * m;
+    // the 32 sequences, and the one of them, that x0 is in
+    const int l = __ffs(__ballot_sync(0xffffffffu, upto > x0)) - 1;
+    const int at = x0 - __shfl_sync(0xffffffffu, upto - own, l);
     Seq s{0, 0, 0};
-    if (lane == l) {
-      for (;; ++seq) {
-        s = load_seq(a, seq, false);
-        const int c = cost_of(s, few);
-        if (at < c) break;
-        at -= c;
-      }
-    }
-    s.len = __shfl_sync(0xffffffffu, s.len, l);
-    s.row0 = __shfl_sync(0xffffffffu, s.row0, l);
-    s.fresh = __shfl_sync(0xffffffffu, s.fresh, l);
-    run.start(__shfl_sync(0xffffffffu, seq, l), s, __shfl_sync(0xffffffffu, at, l), cost, ut, extra,
-              a.group);
+    if (32 * l + lane < a.n_seqs) s = load_seq(a, 32 * l + lane);
+    const int its = cost_of(s, few), end = sums_to_here(its);
+    const int w = __ffs(__ballot_sync(0xffffffffu, end > at)) - 1;
+    s.len = __shfl_sync(0xffffffffu, s.len, w);
+    s.row0 = __shfl_sync(0xffffffffu, s.row0, w);
+    s.fresh = __shfl_sync(0xffffffffu, s.fresh, w);
+    run.start(32 * l + w, s, at - __shfl_sync(0xffffffffu, end - its, w), cost, ut, extra, a.group);
     busy = run.left > 0;  // a run may lie inside one item's extra part
   }
   if (threadIdx.x == 64) a.meta[blockIdx.x * 4] = 0;  // warp 2 knows better later
