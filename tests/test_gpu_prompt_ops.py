@@ -690,6 +690,62 @@ def test_two_contexts_at_once(sam3):
             check_cached(got, q, host, None, table, lens, "f16", True, 0.1)
 
 
+def test_two_contexts_packed_and_cached_at_once(sam3):
+    rng = np.random.default_rng(31)
+    cfg = dict(embed_dim=256, num_heads=4, mlp_hidden=512, num_blocks=0, image_size=112, prune_after_block=0)
+    with sam3.Context(0, **cfg) as a, sam3.Context(0, **cfg) as b:
+        jobs = []
+        for ctx, dim in ((a, 64), (b, 128)):
+            lens = [700, 0, 129, 1500]
+            cu, rows = _cu(lens), sum(lens)
+            q, k, v = (_rows(rng, rows, n, dim, "f16") for n in (4, 2, 2))
+            bufs = [ctx.upload(_bits(x, "f16")) for x in (q, k, v)] + [ctx.upload(cu), ctx.alloc(rows * 4 * dim * 2)]
+            clens = [3000, 17, 900]
+            host, table = filled(rng, ctx, sam3, clens, 2, 32, dim)
+            dc = DeviceCache(ctx, sam3, host, dim)
+            cq = _rows(rng, 3, 4, dim, "f16")
+            cbufs = [ctx.upload(_bits(cq, "f16")), ctx.upload(table), ctx.upload(np.asarray(clens, np.int32)),
+                     ctx.alloc(3 * 4 * dim * 2)]
+            jobs.append((ctx, dim, lens, cu, q, k, v, bufs, clens, host, table, dc, cq, cbufs))
+        for _ in range(20):  # both kinds in flight on two streams
+            for ctx, dim, lens, cu, *_, bufs, clens, host, table, dc, cq, cbufs in jobs:
+                ctx.attention_packed(sam3.F16, bufs[0], 4 * dim, bufs[1], 2 * dim, bufs[2], 2 * dim, bufs[3],
+                                     len(lens), sum(lens), 4, 2, dim, 0.1, True, bufs[4], 4 * dim)
+                ctx.attention_cached(dc.c, sam3.F16, cbufs[0], 4 * dim, None, 3, 3, 1, cbufs[1], table.shape[1],
+                                     cbufs[2], 4, 0.1, True, cbufs[3], 4 * dim)
+        for ctx, dim, lens, cu, q, k, v, bufs, clens, host, table, dc, cq, cbufs in jobs:
+            ctx.sync()
+            check_packed(ctx.download(bufs[4], (sum(lens), 4, dim), np.uint16), q, k, v, cu, "f16", True, 0.1)
+            check_cached(ctx.download(cbufs[3], (3, 4, dim), np.uint16), cq, host, None, table, clens, "f16", True, 0.1)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_rows_before_and_behind_the_sequences_are_left(ctx, sam3, dim):
+    rng = np.random.default_rng(32)
+    lens, new = [300, 40], [5, 2]
+    cu = np.array([3, 8, 10], np.int32)  # of 14 rows
+    table, pages = tables(rng, lens, 16)
+    host = P.Cache(pages, 1, 16, dim)
+    dc = DeviceCache(ctx, sam3, host, dim)
+    first = [n - m for n, m in zip(lens, new)]
+    k, v = (_rows(rng, sum(first), 1, dim, "f16") for _ in range(2))
+    append(ctx, sam3, dc, k, v, _cu(first), table, first, "f16")
+    host.append(k, v, _cu(first), table, first)
+    q, k, v = (_rows(rng, 14, n, dim, "f16") for n in (2, 1, 1))
+    for x in (q, k, v):
+        x[:3], x[10:] = np.nan, np.inf
+    append(ctx, sam3, dc, k, v, cu, table, lens, "f16", max_new=5)
+    host.append(k, v, cu, table, lens)
+    same_cache(dc.read(), host)
+    got = attend(ctx, sam3, dc, q, cu, table, lens, "f16", True, 0.1, max_new=5)
+    check_cached(got, q, host, cu, table, lens, "f16", True, 0.1)
+    assert (got[:3] == GUARD).all() and (got[10:] == GUARD).all()
+    got, _ = run_packed(ctx, sam3, q, k, v, cu, "f16", True, 0.1)
+    check_packed(got, q, k, v, cu, "f16", True, 0.1)
+    assert (got[:3] == GUARD).all() and (got[10:] == GUARD).all()
+    dc.free()
+
+
 def test_profile_and_launch_counters(ctx, sam3):
     rng = np.random.default_rng(22)
     ctx.profile_enable(True)
