@@ -46,12 +46,12 @@
 // maximum of x + log2(vs), at most 2^8.8 < 448; the row sum adds P / vs in fp32.
 //
 // Measured (32 heads on 8 of 128): two contexts of 131,072 and 100,003 tokens,
-// pages of 128, 474 MB: 79 us, 6.0 TB/s, 92 % of a copy's rate, and 2 for the
-// join; 64 contexts of 33 to 4096 tokens, one new token each, pages of 64: 30
+// pages of 128, 474 MB: 79 us, 6.0 TB/s, 92 % of a copy's rate, and 2 to 3 for
+// the join; 64 contexts of 33 to 4096 tokens, one new token each, pages of 64: 30
 // us for 114 MB, where plan, first loads, and the end and join of items that
 // are cut cost about 10. 8 contexts of 5200 to 5500 tokens, 1 to 8 new tokens, 16
-// heads on 4 of 64, pages of 32: 23.5 us, bound by the 32 rows' terms, which read
-// the cache twice. One context of 77 tokens: 7.0 us, latency from the lengths to
+// heads on 4 of 64, pages of 32: 23.8 us, bound by the 32 rows' terms, which read
+// the cache twice. One context of 77 tokens: 7.4 us, latency from the lengths to
 // the result. (With the codes unpacked by the threads and fed to mma.sync the
 // four took 115, 57, 25 and 7.8 us.) Pages of 16 tokens with head_dim 64 cost
 // a long context 28 % more than larger ones: a TMA box of 1 KB each.
