@@ -150,6 +150,7 @@ struct Finder {
   static constexpr int KEEP = 4;
   int row0[KEEP], len[KEEP], tiles[KEEP];
   int span, most;
+  int total;     // tiles, known once find has found none
   int at, seen;  // the 32 sequences that are looked at (the first; -1: none), tiles before
 
   __device__ __forceinline__ int load(const PackedArgs& a, int i, int& r0, int& n) const {
@@ -196,7 +197,10 @@ struct Finder {
         else
           hi = mid - 1;
       }
-      if (lo == 0) return {0, 0, -1, 0};
+      if (lo == 0) {
+        total = at_least(a.causal, 1);
+        return {0, 0, -1, 0};
+      }
       int rank = number - at_least(a.causal, lo + 1), tile = lo - 1;
       if (!a.causal) {
         tile = rank % lo;
@@ -242,6 +246,7 @@ struct Finder {
       if (at < 0) break;
       look();
     }
+    total = seen;
     return {0, 0, -1, 0};
   }
 };
@@ -422,42 +427,60 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
       finder.init(a, T == 2 && !a.pair_heads ? 256 : 128);
       uint32_t k_bits = 0, k_par = 0, v_bits = 0, v_par = 0;  // loads to drain on abort
       uint32_t raw_uses = 0, q_par = 0, asked = 0;
-      int number = blockIdx.x;
       Ring<KST> rk;
       Ring<VST> rv;
       bool ok = true;
       // The first item is the CTA's own, the next ones those of CTAs that are then
       // never launched: where all run at once there is nothing to take over.
-      const bool others = gridDim.x > a.resident;
+      bool others = gridDim.x > a.resident, outstanding = false;
+      int held = -1;  // numbers taken over and not yet worked on, one per lane
       auto ask = [&](int n, uint32_t slots) {
         if (lane == 0) mbar_arrive_expect_tx(bar_next, 16 * n);
         __syncwarp();
         if (lane < n) cta_try_cancel(slots + 16 * lane, bar_next);
         ++asked;
       };
-      auto answered = [&]() {
+      auto answered = [&](int n, uint32_t slots) {  // numbers in `held`
         ok = __all_sync(0xffffffffu, mbar_wait(bar_next, (asked - 1) & 1u, abort_flag, a.err,
                                                kDevErrTimeoutPacked));
-        return ok;
+        if (!ok) return;
+        held = lane < n ? cta_cancelled(slots + 16 * lane) : -1;
+        __syncwarp();
+        // nothing may be asked for once a refusal has been seen
+        others = !__any_sync(0xffffffffu, lane < n && held < 0);
       };
+      auto held_set = [&]() { return __ballot_sync(0xffffffffu, held >= 0); };
       for (uint32_t i = 0; ok; ++i) {
-        if (i) {
-          number = others && answered() ? cta_cancelled(next_slot) : -1;
-          __syncwarp();
-        }
         Item it{0, 0, -1, 0};
-        if (number >= 0) it = finder.find(a, number / a.units);
-        // A number behind the last tile (the grid is an upper bound): so are all that
-        // are not launched yet. They are done away with, several at a time (one by
-        // one: 334 against 184 us for 1000 sequences of 1 to 80 rows).
-        while (ok && others && number >= 0 && it.tile < 0) {
-          ask(C::EMPTY, empty_slots);
-          if (answered())
-            number = __reduce_min_sync(
-                0xffffffffu, lane < C::EMPTY ? cta_cancelled(empty_slots + 16 * lane) : 0);
+        int number = -1;
+        for (bool own = i == 0;; own = false) {
+          if (outstanding) {
+            outstanding = false;
+            answered(1, next_slot);
+            if (!ok) break;
+          }
+          number = blockIdx.x;
+          if (!own) {
+            const uint32_t set = held_set();
+            if (!set) break;
+            const int l = __ffs(set) - 1;
+            number = __shfl_sync(0xffffffffu, held, l);
+            if (lane == l) held = -1;
+          }
+          it = finder.find(a, number / a.units);
+          if (it.tile >= 0) break;
+          // A number behind the last tile (the grid is an upper bound), as a rule like
+          // all that are not launched yet. They are done away with several at a time
+          // (one by one: 334 against 184 us for 1000 sequences of 1 to 80 rows).
+          while (ok && others && !held_set()) {
+            ask(C::EMPTY, empty_slots);
+            answered(C::EMPTY, empty_slots);
+            if (held >= 0 && held / a.units >= finder.total) held = -1;
+          }
+          if (!ok) break;
         }
         if (!ok) break;
-        it.unit = max(number, 0) % a.units;
+        it.unit = number % a.units;
         const int slot = i & 1;
         ok = __all_sync(0xffffffffu, mbar_wait(bar_item_free + 8 * slot, (i >> 1 & 1) ^ 1,
                                                abort_flag, a.err, kDevErrTimeoutPacked));
@@ -487,7 +510,10 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
         for (int j = 0; j < w.nmax && ok; ++j) {
           // no earlier than the answer is needed, two tiles before the item's last MMA:
           // until then it may fall to a CTA that is done before
-          if (j == w.nmax - 1 && others) ask(1, next_slot);
+          if (j == w.nmax - 1 && others && !held_set()) {
+            ask(1, next_slot);
+            outstanding = true;
+          }
           // does some query of the CTA see a part of this tile only?
           const bool diag = a.causal && (j == w.n[0] - 1 || j == w.n[1] - 1);
           const bool fix = diag || (j + 1) * BKV > w.len;
