@@ -314,8 +314,10 @@ sam3_status_t sam3_kv_append(sam3_ctx_t* ctx, const sam3_kv_cache_t* cache, int3
  * new token sees the tokens up to itself, else all of its sequence. Made for
  * one or a few new tokens per sequence: up to 16 query rows (new tokens times
  * heads per K/V head) read the cache once, more read it again for each 16.
- * Sequences may share pages. The weights are rounded to fp16's 11 bits before
- * they multiply v's codes; an infinity in a row of q makes its result NaN.
+ * Sequences may share pages. Before they multiply v's codes, the weights are
+ * rounded to 11 bits; those whose product with v's scale is more than 2^26 below
+ * the row's largest such product, to within 2^-37 of that. An infinity in a row
+ * of q makes its result NaN.
  * n_seqs <= SAM3_CACHED_MAX_SEQS. o must not overlap q. */
 sam3_status_t sam3_attention_cached(sam3_ctx_t* ctx, const sam3_kv_cache_t* cache, int32_t dtype,
                                     const uint16_t* q, int64_t q_stride, const int32_t* cu_new,

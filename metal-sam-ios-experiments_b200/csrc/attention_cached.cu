@@ -13,13 +13,21 @@
 //   S^T[line, column] = K[line, 128 bytes] . Q[column, 128 bytes]
 //   O^T[byte, column] += V[line, byte] . P[line, column]
 // A line is 128 bytes of codes: one token of head_dim 128 or two of 64. The
-// large operand is the M = 128 side, the few rows are columns of the N side, and
-// each row takes three columns, the terms of an exact split of an 11-bit
+// large operand is the M = 128 side, the few rows are columns of the N side.
+// A row of Q takes three columns, the terms of an exact split of an 11-bit
 // number into e4m3 numbers: y = t0 + t1/16 + t2/256, each term the rounding
 // (4 bits, to nearest) of what is left. fp16 and bf16 queries (scaled by a
-// power of two to at most 448) are represented exactly down to 2^-6, smaller
-// elements to within 2^-18; the weights p are rounded to fp16 (half a step of
-// 2^-11) and split the same way. Products are exact and sums fp32. For
+// power of two to at most 256) are represented exactly down to 2^-6, smaller
+// elements to within 2^-18, 2^-26 of the row's largest.
+// A row's weights p are rounded to fp16 (half a step of 2^-11) and take four
+// columns, e5m2 numbers: p = t0 + t1/8 + t2/64 + t3/512, each term the three
+// leading bits of what is left. e5m2 is fp16's upper byte, so the split is exact
+// for every fp16 number, the subnormal ones too, and a weight that is far below
+// its row's largest keeps its bits: all 11 down to 2^-26 of it, and what lies
+// below to within 2^-37. (Three e4m3 terms end 2^-23 below the largest: of a
+// row with one heavy key and 130,000 light ones that hold a fifth of the sum,
+// 5 % of the light ones' share went. The fourth term costs 4 % at 16 rows of
+// head_dim 64, 2 % at 16 of 128 and nothing with fewer.) Products are exact and sums fp32. For
 // head_dim 64 a column serves one of the line's two tokens: Q's other half is
 // zero, and of O^T only the half of the column's token is used (the tensor
 // cores have room: an MMA is bound by its 128-row operand up to 64 columns).
@@ -42,8 +50,9 @@
 // and row sum in the workspace, and cached_join_kernel adds the pieces in the
 // order of the CTAs (no atomics: the result does not depend on timing).
 //
-// V's scale joins the exponent: P = 2^(x + log2(vs) - M + 6) with M the running
-// maximum of x + log2(vs), at most 2^8.8 < 448; the row sum adds P / vs in fp32.
+// V's scale joins the exponent: P = 2^(x + log2(vs) - M + 12) with M the running
+// maximum of x + log2(vs), at most 2^14.8 < 57344, e5m2's largest; "largest"
+// above is that of p times vs. The row sum adds P / vs in fp32.
 //
 // Measured (32 heads on 8 of 128): two contexts of 131,072 and 100,003 tokens,
 // pages of 128, 474 MB: 79 us, 6.0 TB/s, 92 % of a copy's rate, and 2 to 3 for
@@ -71,10 +80,9 @@ constexpr int LINES = 128;             // lines per tile
 constexpr int TILE = LINES * 128;      // bytes of K or V per tile
 constexpr int UNIT_TILES = 4;          // tiles per unit of small jobs
 constexpr int ITEM_COST = 2;           // what an item costs besides its tiles, in tiles
-constexpr float P_EXP = 6.f;           // the weight at the running maximum is 2^6
+constexpr float P_EXP = 12.f;          // the weight at the running maximum is 2^12
 constexpr float NO_MAX = 1e30f;        // P_EXP - M of a row that has seen nothing
-constexpr float P_TOP = 8.8f;          // and may grow to 2^8.8 < 448 before M moves
-constexpr float T1 = 1.f / 16, T2 = 1.f / 256;  // weights of the second and third term
+constexpr float P_TOP = 14.8f;         // and may grow to 2^14.8 before M moves
 enum : int { kFirst = 1, kLast = 2, kFinal = 4, kCheck = 8 };
 constexpr int kNever = 0x7FFFFFFF;
 
@@ -82,14 +90,14 @@ template <int D, int RB>
 struct Cfg {
   static constexpr int TPL = 128 / D;             // tokens per line
   static constexpr int TT = LINES * TPL;          // tokens per tile
-  static constexpr int NC = 3 * RB * TPL;         // columns used
-  static constexpr int N = (NC + 15) / 16 * 16;   // columns of the MMAs
-  static constexpr int PW = N <= 32 ? 32 : N <= 64 ? 64 : 128;  // bytes of a line of P
+  static constexpr int NS = (3 * RB * TPL + 15) / 16 * 16;  // columns of S^T
+  static constexpr int N = 4 * RB * TPL;          // columns of O^T
+  static constexpr int PW = N <= 32 ? 32 : N;     // bytes of a line of P
   static constexpr int ST = N <= 32 ? 3 : 2;      // ring stages (K and V tile each)
   static constexpr uint32_t COLS = N <= 16 ? 32 : N <= 32 ? 64 : N <= 64 ? 128 : 256;
   static constexpr int GRAN = TT / 16;            // scale entries per tile (16 tokens)
-  static constexpr int OFF_Q = ST * 2 * TILE;               // [2][N][128]
-  static constexpr int OFF_P = OFF_Q + 2 * N * 128;         // [LINES][PW]
+  static constexpr int OFF_Q = ST * 2 * TILE;               // [2][NS][128]
+  static constexpr int OFF_P = OFF_Q + 2 * NS * 128;        // [LINES][PW]
   static constexpr int OFF_SCALE = OFF_P + LINES * PW;      // [ST][GRAN] float4
   static constexpr int OFF_INFO = OFF_SCALE + ST * GRAN * 16;     // [ST] int4
   static constexpr int OFF_ITEM = OFF_INFO + ST * 16;       // [2] ItemInfo
@@ -101,12 +109,15 @@ struct Cfg {
   static constexpr int OFF_MISC = OFF_BAR + BARS * 8;
   static constexpr int SMEM = OFF_MISC + 128 + 1024;
   // column of term t of row r for token p of a line: a pair of rows takes six
-  // neighbours, as split3 gives them
-  static constexpr __host__ __device__ int col(int p, int r, int t) {
+  // neighbours of S^T, as split3 gives them, or eight of O^T
+  static constexpr __host__ __device__ int col_s(int p, int r, int t) {
     return (p * RB + r) / 2 * 6 + 2 * t + (r & 1);
   }
-  // row of a column (any row for those not used)
-  static constexpr __host__ __device__ int row_of(int n) { return (n / 6 * 2 + (n & 1)) % RB; }
+  static constexpr __host__ __device__ int col_o(int p, int r, int t) {
+    return (p * RB + r) / 2 * 8 + 2 * t + (r & 1);
+  }
+  // row of a column of O^T
+  static constexpr __host__ __device__ int row_of(int n) { return (n / 8 * 2 + (n & 1)) % RB; }
 };
 static_assert(2 * (Cfg<128, 8>::SMEM + 1024) <= 228 * 1024, "two CTAs per SM");
 static_assert(2 * (Cfg<128, 16>::SMEM + 1024) <= 228 * 1024, "two CTAs per SM");
@@ -185,6 +196,26 @@ __device__ __forceinline__ void split3(__half2 h, uint16_t (&t)[3]) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(b) : "h"(t[i]));
     h = __hmul2(__hsub2(h, *reinterpret_cast<const __half2*>(&b)), __float2half2_rn(16.f));
   }
+}
+
+// The four terms of two pairs of fp16 numbers below 57344, as e5m2 code pairs in
+// the order of the columns: every subtraction and product below is exact.
+__device__ __forceinline__ uint4 split4(__half2 a, __half2 b) {
+  auto pair = [](__half2 h, uint32_t& t01, uint32_t& t23) {
+    uint32_t t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      t[i] = *reinterpret_cast<const uint32_t*>(&h) & 0xFF00FF00u;
+      if (i < 3)
+        h = __hmul2(__hsub2(h, *reinterpret_cast<const __half2*>(&t[i])), __float2half2_rn(8.f));
+    }
+    t01 = __byte_perm(t[0], t[1], 0x7531);
+    t23 = __byte_perm(t[2], t[3], 0x7531);
+  };
+  uint4 w;
+  pair(a, w.x, w.y);
+  pair(b, w.z, w.w);
+  return w;
 }
 
 // Bytes of w whose code is NaN (0x7F or 0xFF), as 0xFF.
@@ -274,7 +305,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     cached_attn_kernel(const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const CachedArgs a) {
   using C = Cfg<D, RB>;
-  constexpr int TPL = C::TPL, N = C::N, ST = C::ST;
+  constexpr int TPL = C::TPL, NS = C::NS, N = C::N, ST = C::ST;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t sbase = smem_u32(smem);
@@ -566,8 +597,8 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
   } else if (busy && warp == 1) {
     // ------------------------------------------------------------- MMA issuer
-    constexpr uint32_t IDESC_S = umma_idesc_e4m3(128, N, 0);
-    constexpr uint32_t IDESC_O = umma_idesc_e4m3(128, N, 1);
+    constexpr uint32_t IDESC_S = umma_idesc_f8(128, NS, 0, kE4M3);
+    constexpr uint32_t IDESC_O = umma_idesc_f8(128, N, 1, kE5M2);
     const uint32_t s_col = tmem, o_col = tmem + C::COLS / 2;
     struct Slot {
       int st = 0;
@@ -626,7 +657,7 @@ __global__ void __launch_bounds__(THREADS, 2)
           if (!(flags & kFirst) || here(bar_q + 8 * (items & 1), (items >> 1) & 1u)) {
             if (flags & kFirst) ++items;
             const uint64_t dk = desc_advance(desc_k, qk.st * 2 * TILE);
-            const uint64_t dq = desc_advance(desc_q, ((items - 1) & 1) * N * 128);
+            const uint64_t dq = desc_advance(desc_q, ((items - 1) & 1) * NS * 128);
             tc_fence_after();
             if (elect_one()) {
 #pragma unroll
@@ -687,7 +718,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       if (!__all_sync(0xffffffffu, mbar_wait(bar_q_empty + 8 * b, (item >> 1 & 1) ^ 1, abort_flag,
                                              a.err, kDevErrTimeoutCached)))
         break;
-      uint8_t* qb = smem + C::OFF_Q + b * N * 128;
+      uint8_t* qb = smem + C::OFF_Q + b * NS * 128;
       float rs = 0.f;
 #pragma unroll
       for (int i = 0; i < RB; ++i) {
@@ -716,7 +747,7 @@ __global__ void __launch_bounds__(THREADS, 2)
         for (int p = 0; p < TPL; ++p)
 #pragma unroll
           for (int k = 0; k < 3; ++k) {
-            const int n = C::col(p, i, k);
+            const int n = C::col_s(p, i, k);
             if (D == 128) {
               const uint32_t at = (uint32_t)(lane * 4) ^ ((n & 7) << 4);
               *reinterpret_cast<uint32_t*>(qb + n * 128 + at) =
@@ -796,18 +827,28 @@ __global__ void __launch_bounds__(THREADS, 2)
     const int line = (warp - 4) * 32 + lane;
     const uint32_t lane_base = tmem + ((uint32_t)((warp - 4) * 32) << 16);
     const uint32_t s_col = lane_base, o_col = lane_base + C::COLS / 2;
-    constexpr int CH = RB < 16 ? RB : 16;  // rows that tensor memory is read for at a time
-    // columns col(p, r0, 0) ... of CH rows, their three terms added
-    auto read_rows = [&](uint32_t col, float (&v)[CH]) {
-      constexpr int W = CH == 4 ? 4 : CH == 8 ? 8 : 16;
-      uint32_t s[3 * CH / W][W];
+    // columns of S^T from col on: the scores of all rows, their three terms added
+    auto read_scores = [&](uint32_t col, float (&v)[RB]) {
+      constexpr int W = RB;  // a load
+      uint32_t s[3][W];
 #pragma unroll
-      for (int i = 0; i < 3 * CH / W; ++i) tmem_ld_32x32b(col + W * i, s[i]);
+      for (int i = 0; i < 3; ++i) tmem_ld_32x32b(col + W * i, s[i]);
       tmem_wait_ld();
       auto at = [&](int n) { return __uint_as_float(s[n / W][n % W]); };
 #pragma unroll
-      for (int r = 0; r < CH; ++r)
-        v[r] = fmaf(at(C::col(0, r, 2)), T2, fmaf(at(C::col(0, r, 1)), T1, at(C::col(0, r, 0))));
+      for (int r = 0; r < RB; ++r)
+        v[r] = fmaf(at(C::col_s(0, r, 2)), 1.f / 256,
+                    fmaf(at(C::col_s(0, r, 1)), 1.f / 16, at(C::col_s(0, r, 0))));
+    };
+    // 16 columns of O^T from col on: the outputs of 4 rows, their four terms added
+    auto read_outputs = [&](uint32_t col, float* v) {
+      uint32_t s[16];
+      tmem_ld_32x32b(col, s);
+      tmem_wait_ld();
+      auto at = [&](int r, int t) { return __uint_as_float(s[C::col_o(0, r, t)]); };
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        v[r] = fmaf(fmaf(fmaf(at(r, 3), 1.f / 8, at(r, 2)), 1.f / 8, at(r, 1)), 1.f / 8, at(r, 0));
     };
     float4* wmax = reinterpret_cast<float4*>(smem + C::OFF_MAX);
     uint8_t* pb = smem + C::OFF_P;
@@ -828,14 +869,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       tc_fence_after();
       float x[TPL][RB];
 #pragma unroll
-      for (int p = 0; p < TPL; ++p)
-#pragma unroll
-        for (int c = 0; c < RB / CH; ++c) {
-          float v[CH];
-          read_rows(s_col + C::col(p, c * CH, 0), v);
-#pragma unroll
-          for (int r = 0; r < CH; ++r) x[p][c * CH + r] = v[r];
-        }
+      for (int p = 0; p < TPL; ++p) read_scores(s_col + C::col_s(p, 0, 0), x[p]);
       tc_fence_before();
       mbar_arrive(bar_s_free);
       const float4 sc = scales[stage * C::GRAN + line * TPL / 16];
@@ -871,7 +905,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       }
       bool o_waited = false;
       if (vote_any(grow)) {
-        // the rows' maxima over the tile; M moves where they exceed it by 0.8
+        // the rows' maxima over the tile; M moves where they exceed it by 2.8
         if (!ok) *softmax_failed = 1;
 #pragma unroll
         for (int r = 0; r < RB; ++r) {
@@ -929,35 +963,24 @@ __global__ void __launch_bounds__(THREADS, 2)
         const bool w = mbar_wait(bar_o, (i - 1) & 1u, abort_flag, a.err, kDevErrTimeoutCached);
         ok = __all_sync(0xffffffffu, w) && ok;
       }
-      // the weights' terms: a line of P in the order of the columns
-      uint16_t terms[N / 2];
-#pragma unroll
-      for (int p = 0; p < TPL; ++p)
-#pragma unroll
-        for (int r = 0; r < RB; r += 2) {
-          const float p0 = ex2_approx(x[p][r] + off[r]), p1 = ex2_approx(x[p][r + 1] + off[r + 1]);
-          l[r] = fmaf(p0, sc.z, l[r]);
-          l[r + 1] = fmaf(p1, sc.z, l[r + 1]);
-          uint16_t t[3];
-          split3(__floats2half2_rn(p0, p1), t);
-#pragma unroll
-          for (int k = 0; k < 3; ++k) terms[C::col(p, r, k) / 2] = t[k];
-        }
-#pragma unroll
-      for (int n = C::NC / 2; n < N / 2; ++n) terms[n] = 0;
+      // the weights' terms: a line of P in the order of the columns, its 16-byte
+      // groups (4 rows each) swizzled like the tensor cores' PW-byte pattern
       {
-        // 16-byte groups swizzled like the tensor cores' PW-byte pattern
         constexpr int G = C::PW / 16;
         const int sw = (line * C::PW >> 7) & (G - 1);
 #pragma unroll
-        for (int c = 0; c < N / 16; ++c) {
-          uint32_t w[4];
+        for (int p = 0; p < TPL; ++p)
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            w[q] = terms[8 * c + 2 * q] | (uint32_t)terms[8 * c + 2 * q + 1] << 16;
-          *reinterpret_cast<uint4*>(pb + line * C::PW + ((c ^ sw) << 4)) =
-              make_uint4(w[0], w[1], w[2], w[3]);
-        }
+          for (int r = 0; r < RB; r += 4) {
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              w[e] = ex2_approx(x[p][r + e] + off[r + e]);
+              l[r + e] = fmaf(w[e], sc.z, l[r + e]);
+            }
+            *reinterpret_cast<uint4*>(pb + line * C::PW + (((p * RB + r) / 4 ^ sw) << 4)) =
+                split4(__floats2half2_rn(w[0], w[1]), __floats2half2_rn(w[2], w[3]));
+          }
       }
       if (check) {
         // Codes of tokens that no row sees become 0 (their weight is 0, but 0 *
@@ -1008,12 +1031,7 @@ __global__ void __launch_bounds__(THREADS, 2)
         const int half = TPL == 2 ? line >> 6 : 0, d = TPL == 2 ? line & 63 : line;
         float v[RB];
 #pragma unroll
-        for (int c = 0; c < RB / CH; ++c) {
-          float o[CH];
-          read_rows(o_col + C::col(half, c * CH, 0), o);
-#pragma unroll
-          for (int r = 0; r < CH; ++r) v[c * CH + r] = o[r];
-        }
+        for (int r = 0; r < RB; r += 4) read_outputs(o_col + C::col_o(half, r, 0), v + r);
         const uint32_t bits = poison[line];
         if (bits) {
 #pragma unroll

@@ -232,7 +232,7 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// D(tmem) (+)= A(smem desc) * B(smem desc)^T, kind::f8f6f4 (e4m3 bytes), fp32
+// D(tmem) (+)= A(smem desc) * B(smem desc)^T, kind::f8f6f4 (bytes), fp32
 // accumulate.
 __device__ __forceinline__ void umma_f8_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
                                            uint32_t idesc, uint32_t accumulate) {
@@ -319,10 +319,11 @@ __host__ __device__ constexpr uint32_t umma_idesc_f16(int m, int n, int b_mn_maj
          (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-// Instruction descriptor, kind::f8f6f4: D f32, A/B e4m3, both K-major or both
-// M/N-major.
-__host__ __device__ constexpr uint32_t umma_idesc_e4m3(int m, int n, int mn_major) {
-  return (1u << 4) | (static_cast<uint32_t>(mn_major & 1) << 15) |
+// Instruction descriptor, kind::f8f6f4: D f32, A e4m3, B of the given type (that
+// kind takes them apart), both K-major or both M/N-major.
+enum : uint32_t { kE4M3 = 0, kE5M2 = 1 };
+__host__ __device__ constexpr uint32_t umma_idesc_f8(int m, int n, int mn_major, uint32_t b_type) {
+  return (1u << 4) | (b_type << 10) | (static_cast<uint32_t>(mn_major & 1) << 15) |
          (static_cast<uint32_t>(mn_major & 1) << 16) |
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }

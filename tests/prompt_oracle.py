@@ -159,3 +159,38 @@ def attend(q, k, v, scale, first, dtype, p_dtype, vmax=None):
         ds = 2 * (d + 4) * 2.0 ** -24 * size + 2.0 ** -21 + 2 * n * 2.0 ** -24
         tol[:, h] = u * np.abs(o[:, h]) + TINY[dtype] + (1 + u) * (up + ds[:, None]) * a + small
     return o, tol
+
+
+def attend_codes(q, kc, ks, vc, vs, scale, first, dtype):
+    """Cached attention with a bound for each result by itself: q [m, heads, d]
+    at positions first.. (None: all see all), kc and vc [n, kv, d] the codes'
+    numbers, ks and vs [n, kv] their scales. Against attend(), whose share for
+    small weights is n times the worst step:
+      - a weight p_j is held as P_j = C p_j vs_j, rounded to fp16, with the row's
+        largest P_j at least 2^12 (the running maximum lags by 2.8 at most, and
+        a maximum that moved scales earlier errors down): 2^-11 of each weight,
+        and half a subnormal step, 2^-25, of each P_j below fp16's normal
+        numbers: 2^-37 max_j(p_j vs_j) sum_j |vc_j| in the result;
+      - a query element is held to within 2^-26 of its row's largest;
+      - the tensor cores may cut each sum's last bit: n 2^-23 sum_j p_j |v_j|;
+        a thread's share of the row sum has n / 64 terms, then 64 at most.
+    """
+    m, heads, d = q.shape
+    n, kv, _ = kc.shape
+    g = heads // kv
+    o, tol = np.zeros((m, heads, d)), np.zeros((m, heads, d))
+    seen = np.ones((m, n), bool) if first is None else np.arange(n)[None] <= first + np.arange(m)[:, None]
+    for h in range(heads):
+        k, v = kc[:, h // g] * ks[:, h // g, None], vc[:, h // g] * vs[:, h // g, None]
+        s = np.where(seen, (q[:, h] @ k.T) * scale, -np.inf)
+        size = np.where(seen, (np.abs(q[:, h]) @ np.abs(k).T) * scale, 0.0).max(1)
+        part = np.where(seen, np.abs(k).sum(1)[None], 0.0).max(1) * np.abs(q[:, h]).max(1) * scale
+        p = np.exp(s - s.max(1, keepdims=True))
+        p /= p.sum(1, keepdims=True)
+        o[:, h] = p @ v
+        a = p @ np.abs(v)
+        ds = 2 * ((d + 4) * 2.0 ** -24 * size + 2.0 ** -26 * part) + 2.0 ** -21
+        rel = U["f16"] + ds + n * 2.0 ** -23 + (n / 64 + 64) * 2.0 ** -24
+        small = 2.0 ** -37 * (p * vs[:, h // g]).max(1)[:, None] * (seen @ np.abs(vc[:, h // g]))
+        tol[:, h] = U[dtype] * np.abs(o[:, h]) + TINY[dtype] + (1 + U[dtype]) * (rel[:, None] * a + small)
+    return o, tol
