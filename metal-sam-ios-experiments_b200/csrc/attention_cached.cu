@@ -327,6 +327,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 4);
   volatile int* softmax_failed = reinterpret_cast<volatile int*>(misc + 8);
+  volatile int* progress = reinterpret_cast<volatile int*>(misc + 12);  // tiles passed on
   volatile int* raw_stage = reinterpret_cast<volatile int*>(misc + 64);
   volatile int* k_nan = reinterpret_cast<volatile int*>(misc + 68);       // [ST]
   float4* scales = reinterpret_cast<float4*>(smem + C::OFF_SCALE);
@@ -359,6 +360,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     for (int s = 0; s < ST; ++s) k_nan[s] = kNever;
     *abort_flag = 0;
     *softmax_failed = 0;
+    *progress = 0;
     fence_mbar_init();
     prefetch_tmap(&map_k);
     prefetch_tmap(&map_v);
@@ -559,6 +561,7 @@ __global__ void __launch_bounds__(THREADS, 2)
           if (tile == tile1 - 1) flags |= final_item ? kLast | kFinal : kLast;
           if ((tile + 1) * C::TT > lim_min || hole) flags |= kCheck;
           infos[stage] = make_int4(tile * C::TT, len, flags, lim_min);
+          *progress = *progress + 1;
           if (raw)
             *raw_stage = stage;
           else if (TPL == 2)
@@ -715,8 +718,9 @@ __global__ void __launch_bounds__(THREADS, 2)
     load_rows();
     for (uint32_t item = 0;; ++item) {
       const int b = item & 1;
-      if (!__all_sync(0xffffffffu, mbar_wait(bar_q_empty + 8 * b, (item >> 1 & 1) ^ 1, abort_flag,
-                                             a.err, kDevErrTimeoutCached)))
+      if (!__all_sync(0xffffffffu, mbar_wait_idle(bar_q_empty + 8 * b, (item >> 1 & 1) ^ 1,
+                                                  abort_flag, progress, a.err,
+                                                  kDevErrTimeoutCached)))
         break;
       uint8_t* qb = smem + C::OFF_Q + b * NS * 128;
       float rs = 0.f;
@@ -785,9 +789,10 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
   } else if (TPL == 2 && busy && warp == 3) {
     // ------------------------------------------- K lines shared by two tokens
+    // (there may be none in the whole run)
     for (uint32_t i = 0;; ++i) {
-      if (!__all_sync(0xffffffffu,
-                      mbar_wait(bar_raw, i & 1u, abort_flag, a.err, kDevErrTimeoutCached)))
+      if (!__all_sync(0xffffffffu, mbar_wait_idle(bar_raw, i & 1u, abort_flag, progress, a.err,
+                                                  kDevErrTimeoutCached)))
         break;
       const int st = *raw_stage;
       if (st < 0) break;

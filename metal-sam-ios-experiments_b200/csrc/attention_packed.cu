@@ -330,6 +330,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
   // the V tile to look through: stage (-1: no more), rows of the sequence in it,
   // whether some query sees a part of it only, its place in fix_tile, its number
   volatile int* raw = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 128);
+  volatile int* progress = raw + 5;  // key tiles that the producer has passed on
   const uint32_t next_slot = sbase + C::OFF_MISC + 160;  // the answer of cta_try_cancel
   const uint32_t empty_slots = next_slot + 16;           // [EMPTY] such
 
@@ -360,6 +361,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
     mbar_init(bar_raw_free, 1);
     mbar_init(bar_next, 1);
     *abort_flag = 0;
+    *progress = 0;
     fence_mbar_init();
     prefetch_tmap(&map_q);
     prefetch_tmap(&map_k);
@@ -537,6 +539,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
               raw[2] = diag | (slot * 2 + fixes) << 1;  // at most two such tiles per item
               raw[3] = j;
             }
+            *progress = *progress + 1;
             if (ok) {
               const uint32_t bar = fix ? bar_v_raw : bar_v_full + 8 * rv.st;
               mbar_arrive_expect_tx(bar, C::TILE);
@@ -693,9 +696,12 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
     } else {
       // ----------------------------------------------------------- V tiles
       const int id = threadIdx.x - 32 * C::CHECKER;
+      // Such a tile may never come: without a mask, and with whole tiles, the two
+      // warps wait until the CTA's last item.
       for (uint32_t u = 0;; ++u) {
-        const bool there = __all_sync(
-            0xffffffffu, mbar_wait(bar_v_raw, u & 1u, abort_flag, a.err, kDevErrTimeoutPacked));
+        const bool there =
+            __all_sync(0xffffffffu, mbar_wait_idle(bar_v_raw, u & 1u, abort_flag, progress, a.err,
+                                                   kDevErrTimeoutPacked));
         if (id == 0) raw[4] = there;  // one decision for both warps
         asm volatile("barrier.cta.sync 3, 64;" ::: "memory");
         const int st = raw[0], held = raw[1], flags = raw[2], j = raw[3];

@@ -3,9 +3,9 @@
 // Inline-PTX wrappers for mbarriers, TMA (cp.async.bulk.tensor, no cluster
 // multicast anywhere in this library), and the tcgen05 tensor-core / tensor-
 // memory instructions, plus a bounded mbarrier wait: every spin in this
-// library gives up after kWaitTimeoutNs, records an error code in device
-// memory and lets the kernel unwind, so a logic error surfaces as
-// SAM3_ERR_TIMEOUT instead of a hung GPU.
+// library gives up after kWaitTimeoutNs (mbar_wait_idle: that long without
+// progress), records an error code in device memory and lets the kernel unwind,
+// so a logic error surfaces as SAM3_ERR_TIMEOUT instead of a hung GPU.
 #pragma once
 
 #include <cuda.h>
@@ -106,7 +106,32 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   }
 }
 
-// Same, ignoring the abort flag (used to drain in-flight copies on the way out).
+// Same, where what is waited for may be as far away as the rest of the kernel's
+// work: the limit counts from the last change of *progress, which a warp that
+// does that work keeps counting up.
+__device__ __forceinline__ bool mbar_wait_idle(uint32_t bar, uint32_t parity,
+                                               volatile int* abort_flag, volatile int* progress,
+                                               int* err, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  uint64_t t0 = global_timer_ns();
+  int seen = *progress;
+  while (true) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*abort_flag) return false;
+    const uint64_t now = global_timer_ns();
+    const int at = *progress;
+    if (at != seen) {
+      seen = at;
+      t0 = now;
+    } else if (now - t0 > kWaitTimeoutNs) {
+      *abort_flag = 1;
+      atomicExch(err, code);
+      return false;
+    }
+  }
+}
+
+// Same as mbar_wait, ignoring the abort flag (used to drain in-flight copies on the way out).
 __device__ __forceinline__ bool mbar_wait_drain(uint32_t bar, uint32_t parity) {
   const uint64_t t0 = global_timer_ns();
   while (!mbar_try_wait(bar, parity)) {

@@ -54,3 +54,58 @@ def test_cached_light_keys_beside_a_heavy_one(ctx, sam3, dim, group, dtype):
     assert (tol[:, :, :dim // 2] < 0.015 * np.abs(light)).all() and (light > 5).all()
     err = np.abs(P.from_bits(got, dtype) - o)
     assert (err <= tol).all(), float((err / tol).max())
+
+
+# ------------------------------------------------------------------ calls of seconds
+# Warps that have nothing to do meanwhile wait longer than any single wait may
+# take: without a mask, and with whole tiles, no V or K tile is looked through.
+CFG = dict(embed_dim=256, num_heads=4, mlp_hidden=512, num_blocks=0, image_size=112, prune_after_block=0, max_batch=1)
+
+
+def test_packed_call_of_seconds(sam3):
+    torch = pytest.importorskip("torch")
+    n, heads, dim = 1 << 20, 8, 64  # 2.3e15 operations
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(41)
+    q, k, v = (torch.randn(n, h, dim, generator=gen, device="cuda").half() for h in (heads, 1, 1))
+    v += 2.0
+    o = torch.zeros_like(q)
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    with sam3.Context(0, **CFG) as ctx:
+        ctx.attention_packed(sam3.F16, q, heads * dim, k, dim, v, dim, cu, 1, n, heads, 1, dim, 0.125, False, o, heads * dim)
+        ctx.sync()  # SAM3_ERR_TIMEOUT if a wait had run out
+    at = [0, 1, n // 3, n - 1]
+    x, kk, vv = (t.cpu().numpy().astype(np.float64) for t in (q[at], k, v))
+    want, tol = P.attend(x, kk, vv, 0.125, None, "f16", "f16")
+    assert (np.abs(o[at].cpu().numpy().astype(np.float64) - want) <= tol).all()
+    assert (o[:, :, 0] > 1).all()  # every row was reached
+
+
+def test_cached_call_of_seconds(sam3):
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(42)
+    seqs, kv, group, page, dim, pool = 1024, 16, 16, 128, 64, 32
+    times = 1600  # each sequence reads the pool that often: 6.6 million tokens
+    host = P.Cache(pool, kv, page, dim)
+    host.codes = [P.to_codes(rng.standard_normal(c.shape) * 16 + add) for c, add in zip(host.codes, (0.0, 64.0))]
+    host.scales = [np.full_like(s, 2.0 ** -5) for s in host.scales]
+    q = P.rounded(rng.standard_normal((1, kv * group, dim)), "f16")
+    bits = torch.from_numpy(P.to_bits(q, "f16").view(np.int16)).cuda()
+    rows = bits.expand(seqs, -1, -1).contiguous()
+    o = torch.zeros_like(rows)
+    table = (torch.arange(pool * times, device="cuda", dtype=torch.int32) % pool).expand(seqs, -1).contiguous()
+    lens = torch.zeros(seqs, dtype=torch.int32, device="cuda")
+    want, tol = P.attend_codes(q, *per_token(host, np.arange(pool), pool * page), 0.125, None, "f16")
+    with sam3.Context(0, **CFG) as ctx:
+        dc = DeviceCache(ctx, sam3, host, dim)
+        for n, slack in ((1, 0.0), (times, times * pool * page * 2.0 ** -23)):
+            lens.fill_(n * pool * page)
+            torch.cuda.synchronize()
+            ctx.attention_cached(dc.c, sam3.F16, rows, kv * group * dim, None, seqs, seqs, 1, table, table.shape[1],
+                                 lens, kv * group, 0.125, True, o, kv * group * dim)
+            ctx.sync()
+            got = P.from_bits(o.cpu().numpy().view(np.uint16), "f16")
+            # v > 0 but for a few in 10^5: sum p |v| is the result; each sum's last bit may be cut
+            assert (np.abs(got - want) <= tol + slack * np.abs(want)).all()
+        dc.free()
