@@ -455,6 +455,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     const uint32_t copy_bytes = (uint32_t)page * D;
     int stage = 0;
     uint32_t phase = 0, used = 0, raws = 0;
+    int passed = 0;  // tiles
     bool ok = true;
     Run<D, RB>& r = run;
     // Pages come in windows of 32, one per lane, with their scales. Loads run
@@ -561,7 +562,7 @@ __global__ void __launch_bounds__(THREADS, 2)
           if (tile == tile1 - 1) flags |= final_item ? kLast | kFinal : kLast;
           if ((tile + 1) * C::TT > lim_min || hole) flags |= kCheck;
           infos[stage] = make_int4(tile * C::TT, len, flags, lim_min);
-          *progress = *progress + 1;
+          *progress = ++passed;
           if (raw)
             *raw_stage = stage;
           else if (TPL == 2)

@@ -429,6 +429,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
       finder.init(a, T == 2 && !a.pair_heads ? 256 : 128);
       uint32_t k_bits = 0, k_par = 0, v_bits = 0, v_par = 0;  // loads to drain on abort
       uint32_t raw_uses = 0, q_par = 0, asked = 0;
+      int passed = 0;  // key tiles
       Ring<KST> rk;
       Ring<VST> rv;
       bool ok = true;
@@ -539,7 +540,6 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
               raw[2] = diag | (slot * 2 + fixes) << 1;  // at most two such tiles per item
               raw[3] = j;
             }
-            *progress = *progress + 1;
             if (ok) {
               const uint32_t bar = fix ? bar_v_raw : bar_v_full + 8 * rv.st;
               mbar_arrive_expect_tx(bar, C::TILE);
@@ -558,6 +558,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
             ++raw_uses;
             ++fixes;
           }
+          if (lane == 0) *progress = ++passed;
           rk.step();
           rv.step();
         }
