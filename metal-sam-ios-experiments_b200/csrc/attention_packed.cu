@@ -383,8 +383,10 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
     asm volatile("barrier.cta.sync 1, %0;" ::"n"(C::THREADS) : "memory");
     tc_fence_after();
     tmem = *tmem_slot;
+    // Behind the allocation, as the next kernel allocates too; so not by the
+    // producer, which does not wait for it (one thread speaks for its CTA).
+    griddep_launch_dependents();
   }
-  griddep_launch_dependents();  // behind the allocation: the next kernel allocates too
   griddep_wait();  // offsets and rows may be earlier kernels' outputs
 
   // Looks through a V tile before the MMA reads it (by 64 threads, `id` among

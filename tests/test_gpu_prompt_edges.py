@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import prompt_oracle as P
-from test_gpu_prompt_ops import DeviceCache, attend
+from test_gpu_prompt_ops import _cu, DeviceCache, attend, filled
 
 pytestmark = pytest.mark.gpu
 
@@ -109,3 +109,49 @@ def test_cached_call_of_seconds(sam3):
             # v > 0 but for a few in 10^5: sum p |v| is the result; each sum's last bit may be cut
             assert (np.abs(got - want) <= tol + slack * np.abs(want)).all()
         dc.free()
+
+
+# ------------------------------------------------------------------ one after another
+def test_kernels_that_begin_under_each_others_end(ctx, sam3):
+    # Each kernel's begin overlaps the end of the one before, and their shares of
+    # tensor memory differ: the results are those of calls waited for.
+    rng = np.random.default_rng(43)
+    jobs = []
+    for dim, heads, kv in ((64, 4, 2), (128, 4, 2), (128, 3, 1), (64, 16, 1), (128, 16, 1)):
+        lens = [1, 300, 77, 1400]
+        rows = sum(lens)
+        q, k, v = (P.rounded(rng.standard_normal((rows, h, dim)), "f16") for h in (heads, kv, kv))
+        bufs = [ctx.upload(P.to_bits(x, "f16")) for x in (q, k, v)]
+        host, table = filled(rng, ctx, sam3, [3000, 17, 900], kv, 32, dim)
+        dc = DeviceCache(ctx, sam3, host, dim)
+        more = [ctx.upload(_cu(lens)), ctx.upload(table), ctx.upload(np.asarray([3000, 17, 900], np.int32))]
+        outs = [ctx.alloc(rows * heads * dim * 2), ctx.alloc(3 * heads * dim * 2)]
+        jobs.append((dim, heads, kv, rows, bufs, table, dc, more, outs))
+
+    def call(job, which):
+        dim, heads, kv, rows, bufs, table, dc, more, outs = job
+        if which == 0:
+            ctx.attention_packed(sam3.F16, bufs[0], heads * dim, bufs[1], kv * dim, bufs[2], kv * dim, more[0], 4,
+                                 rows, heads, kv, dim, 0.1, True, outs[0], heads * dim)
+        else:
+            ctx.attention_cached(dc.c, sam3.F16, bufs[0], heads * dim, None, 3, 3, 1, more[1], table.shape[1],
+                                 more[2], heads, 0.1, True, outs[1], heads * dim)
+
+    def results():
+        ctx.sync()
+        return [ctx.download(o, (o.nbytes // 2,), np.uint16) for job in jobs for o in job[-1]]
+
+    for job in jobs:
+        for which in (0, 1):
+            call(job, which)
+            ctx.sync()
+    want = results()
+    for turn in range(6):
+        order = [(job, which) for job in jobs for which in (0, 1)] * 3
+        for i in np.random.default_rng(turn).permutation(len(order)):
+            call(*order[i])
+        assert all(np.array_equal(a, b) for a, b in zip(results(), want))
+    for job in jobs:
+        for b in job[4] + job[7] + job[8]:
+            b.free()
+        job[6].free()
