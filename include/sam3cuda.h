@@ -278,7 +278,8 @@ sam3_status_t sam3_attention(sam3_ctx_t* ctx, const uint16_t* qkv, int32_t batch
 /* o [rows, heads, head_dim] = softmax attention of each row over its own
  * sequence's rows: all of them, or with causal != 0 those up to itself.
  * head_dim 64 or 128. Accumulation and softmax in fp32; the weights are rounded
- * to dtype before they multiply v. o must not overlap q, k or v. */
+ * to dtype before they multiply v (fp16: those below 2^-21 of the row's largest
+ * to within 2^-32 of that). o must not overlap q, k or v. */
 sam3_status_t sam3_attention_packed(sam3_ctx_t* ctx, int32_t dtype, const uint16_t* q,
                                     int64_t q_stride, const uint16_t* k, int64_t k_stride,
                                     const uint16_t* v, int64_t v_stride, const int32_t* cu,

@@ -42,8 +42,12 @@
 // some queries see, before the MMA reads the tile; those are added to the rows
 // that see them at the end (rare; read again from global memory).
 //
-// P is rounded to the inputs' type, as tcgen05 takes both operands in one: half
-// a step (fp16 2^-11, bf16 2^-8) of each weight.
+// P is rounded to the inputs' type (kind::f16 takes both operands in one): half
+// a step (fp16 2^-11, bf16 2^-8) of each weight. fp16 ends at 2^-24, so its
+// weights are 2^7 at the running maximum, and at most 2^15 before O is rescaled:
+// a weight keeps its 11 bits down to 2^-21 of its row's largest and is held to
+// within 2^-32 of that below (at 1 it would be 2^-14 and 2^-25, and thousands of
+// light keys beside a heavy one come out 17 % off).
 //
 // Bounds, measured. head_dim 64: the exponentials (16 per clock and SM; packed
 // FMAs and additions beside them leave them 90 % of it). Four images' tokens
@@ -724,6 +728,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
     // ----------------------------------------------------------- softmax rows
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS));
     constexpr float kRescaleLog2 = 8.0f;
+    constexpr float kTopLog2 = BF ? 0.f : 7.f;  // the weight at the running maximum
     const int t = T == 2 ? warp >> 2 : 0;
     const int quad = warp & 3;  // this warp's TMEM lane quadrant
     const int r = quad * 32 + lane;
@@ -809,6 +814,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
         const bool grow = m_tile > m_run + kRescaleLog2;
         const float m_use = grow ? m_tile : m_run;
         const float alpha = grow ? ex2_approx(m_run - m_use) : 1.0f;  // 0 on the first tile
+        const float to = kTopLog2 - m_use;
         float2 ls[2] = {{0.f, 0.f}, {0.f, 0.f}};
         uint32_t pk[BKV / 2];
 #pragma unroll
@@ -817,7 +823,7 @@ __global__ void __launch_bounds__(PK<D>::THREADS, D == 128 ? 1 : 2)
           // single FMAs and additions in some 1300 (the exponentials' own time: 1024)
           const float2 x = __ffma2_rn(
               make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])),
-              make_float2(c, c), make_float2(-m_use, -m_use));
+              make_float2(c, c), make_float2(to, to));
           const float2 p = make_float2(ex2_approx(x.x), ex2_approx(x.y));
           ls[e & 1] = __fadd2_rn(ls[e & 1], p);
           pk[e] = pack2<BF>(p.x, p.y);

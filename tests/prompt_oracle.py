@@ -115,7 +115,7 @@ class Cache:
 
 
 # ------------------------------------------------------------------ attention
-def attend(q, k, v, scale, first, dtype, p_dtype, vmax=None):
+def attend(q, k, v, scale, first, dtype, p_dtype, vmax=None, least=2.0 ** -25):
     """q [m, heads, d] at positions first.. (None: all see all), k, v [n, kv, d]:
     the result [m, heads, d] and how far a kernel may be from it.
 
@@ -124,7 +124,7 @@ def attend(q, k, v, scale, first, dtype, p_dtype, vmax=None):
       - each weight is rounded once before the product: u_p A, and weights that
         fall below fp16's normal numbers by half a subnormal step each. With the
         running maximum at most 2^8 below the true one this is n 2^-25 max|v|
-        (packed). Cached: a weight is 2^6 at the maximum M of x + log2(vs) and is
+        (packed; least: what a weight's half step is instead). Cached: a weight is 2^6 at the maximum M of x + log2(vs) and is
         kept to within 2^-18 below 2^-6 (three e4m3 terms), so n weights are off
         by n 2^-18 448 in sum; the token that set M adds 2^6 / vs to the row sum:
         n 2^-24 448 max(vs) (vmax = max(vs)). Queries: each is kept to within
@@ -151,7 +151,7 @@ def attend(q, k, v, scale, first, dtype, p_dtype, vmax=None):
         o[:, h] = p @ vv
         a = p @ np.abs(vv)
         top = np.where(seen[:, :, None], np.abs(vv)[None], 0.0).max(1) if m * n * d <= 1 << 24 else np.abs(vv).max(0)[None]
-        small = n * 2.0 ** -25 * top if vmax is None else n * 2.0 ** -24 * 448 * vmax
+        small = n * least * top if vmax is None else n * 2.0 ** -24 * 448 * vmax
         if p_dtype == "bf16":
             small = 0.0
         if vmax is not None:  # the queries' share, added to what fp32 sums cost

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import prompt_oracle as P
-from test_gpu_prompt_ops import _cu, DeviceCache, attend, filled
+from test_gpu_prompt_ops import _cu, DeviceCache, attend, filled, run_packed
 
 pytestmark = pytest.mark.gpu
 
@@ -54,6 +54,27 @@ def test_cached_light_keys_beside_a_heavy_one(ctx, sam3, dim, group, dtype):
     assert (tol[:, :, :dim // 2] < 0.015 * np.abs(light)).all() and (light > 5).all()
     err = np.abs(P.from_bits(got, dtype) - o)
     assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim,heads,kv", [(64, 2, 1), (128, 2, 1), (128, 1, 1)])
+def test_packed_light_keys_beside_a_heavy_one(ctx, sam3, dim, heads, kv, causal):
+    # 8191 keys whose weight is 2^-22.7 of the first one's: 2.4 of fp16's smallest
+    # steps if that is 1, and hundreds if it is 2^7.
+    rng = np.random.default_rng(44)
+    n = 8192
+    q, k = np.zeros((n, heads, dim)), np.zeros((n, kv, dim))
+    q[:, :, 0], k[0, :, 0] = 1.0, 15.75
+    v = P.rounded(rng.uniform(1000, 2000, (n, kv, dim)), "f16")
+    v[0, :, :dim // 2] = 0.0  # here the result is the light keys' alone
+    got, _ = run_packed(ctx, sam3, q, k, v, [0, n], "f16", causal, 1.0)
+    for r in (n - 1, n - 100, n // 2, 0):
+        o, tol = P.attend(q[r:r + 1], k, v, 1.0, r if causal else None, "f16", "f16", least=2.0 ** -32)
+        if r > n - 200:
+            light = o[:, :, :dim // 2]
+            assert (light > 1.5).all() and (tol[:, :, :dim // 2] < 0.005 * light).all()
+        err = np.abs(P.from_bits(got[r:r + 1], "f16") - o)
+        assert (err <= tol).all(), float((err / tol).max())
 
 
 # ------------------------------------------------------------------ calls of seconds
