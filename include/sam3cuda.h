@@ -269,7 +269,9 @@ sam3_status_t sam3_attention(sam3_ctx_t* ctx, const uint16_t* qkv, int32_t batch
  * not fit the buffers is skipped, a page number outside the pool hides that
  * page's tokens (sam3_attention_cached) or drops them (sam3_kv_append), and
  * the next sam3_sync returns SAM3_ERR_INVALID_ARG. Keys that a row does not see
- * take no part in it, whatever their rows hold, infinities and NaN included.
+ * take no part in it, whatever their rows hold, infinities and NaN included. An
+ * infinity in v of a key that is seen becomes an infinity in the result or, where
+ * the key's weight rounds to 0, a NaN (sam3_attention_packed; the cache holds none).
  *
  * All three can be captured into CUDA graphs and replayed with other lengths
  * and page tables in the same buffers; the replays of one context are

@@ -40,7 +40,8 @@
 // key tile and in the causal diagonal ones the V rows behind the sequence's end
 // become 0 and, on the diagonal, so do the infinities and NaN of rows that only
 // some queries see, before the MMA reads the tile; those are added to the rows
-// that see them at the end (rare; read again from global memory).
+// that see them at the end (rare; read again from global memory), whatever their
+// weight; in other tiles the MMA multiplies, and 0 times an infinity is NaN.
 //
 // P is rounded to the inputs' type (kind::f16 takes both operands in one): half
 // a step (fp16 2^-11, bf16 2^-8) of each weight. fp16 ends at 2^-24, so its

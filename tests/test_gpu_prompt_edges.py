@@ -77,6 +77,26 @@ def test_packed_light_keys_beside_a_heavy_one(ctx, sam3, dim, heads, kv, causal)
         assert (err <= tol).all(), float((err / tol).max())
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim,heads,kv", [(64, 2, 1), (128, 2, 1), (128, 1, 1)])
+def test_packed_infinities_in_keys_of_no_weight(ctx, sam3, dim, heads, kv, dtype):
+    # In a whole tile 0 times an infinity is NaN, in a diagonal one the infinity is
+    # added; never is it lost, nor does it reach another column or row.
+    rng = np.random.default_rng(45)
+    n = 600
+    q, k, v = (P.rounded(rng.standard_normal((n, h, dim)), dtype) for h in (heads, kv, kv))
+    q[:, :, 0], k[:, :, 0] = 30.0, 0.0
+    k[[20, 590], :, 0] = -30.0  # e^-900 at most beside the others
+    clean, _ = run_packed(ctx, sam3, q, k, v, [0, n], dtype, True, 1.0)
+    v[20, 0, 5], v[590, 0, 7] = np.inf, -np.inf
+    got, _ = run_packed(ctx, sam3, q, k, v, [0, n], dtype, True, 1.0)
+    g = P.from_bits(got, dtype)
+    assert not np.isfinite(g[20:, :, 5]).any() and not np.isfinite(g[590:, :, 7]).any()
+    hit = np.zeros((n, heads, dim), bool)
+    hit[20:, :, 5] = hit[590:, :, 7] = True
+    assert np.array_equal(got[~hit], clean[~hit])
+
+
 # ------------------------------------------------------------------ calls of seconds
 # Warps that have nothing to do meanwhile wait longer than any single wait may
 # take: without a mask, and with whole tiles, no V or K tile is looked through.
