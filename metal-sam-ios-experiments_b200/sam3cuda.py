@@ -174,10 +174,12 @@ def ptr(x):
     """Device address of a DeviceBuffer / tensor-like / int; None stays None."""
     if x is None or type(x) is int:
         return x
+    if isinstance(x, DeviceBuffer):
+        return x.ptr
     try:
         return x.data_ptr()
     except AttributeError:
-        return x.ptr if isinstance(x, DeviceBuffer) else int(x)
+        return int(x)
 
 
 def default_config(**overrides) -> EncoderConfig:

@@ -37,3 +37,15 @@ def test_dtype_and_limit_constants_match_the_header(sam3):
     src = open(os.path.join(ROOT, "include", "sam3cuda.h")).read()
     assert f"SAM3_F16 = {sam3.F16}, SAM3_BF16 = {sam3.BF16}" in src
     assert f"#define SAM3_CACHED_MAX_SEQS {sam3.CACHED_MAX_SEQS}" in src
+
+
+def test_a_device_buffer_is_not_asked_for_data_ptr(sam3):
+    class Buffer(sam3.DeviceBuffer):
+        def __init__(self):  # no device
+            self.ptr = 4096
+
+        def data_ptr(self):
+            raise AssertionError("asked")
+
+    assert sam3.ptr(Buffer()) == 4096
+    assert [sam3.ptr(x) for x in (None, 0, 1 << 40)] == [None, 0, 1 << 40]
