@@ -237,7 +237,7 @@ __device__ __forceinline__ RawSeq fetch_seq(const CachedArgs& a, int i) {
 __device__ __forceinline__ Seq checked_seq(const CachedArgs& a, const RawSeq& r, bool report) {
   const bool ok =
       tokens_fit(r.row0, r.row1, a.rows, a.max_new, r.len, a.table_stride, a.page_shift);
-  if (!ok && report) atomicExch(a.err, kDevErrBadLengths);
+  if (!ok && report) report_bad_index(a.err, kDevErrBadLengths);
   return {r.len, r.row0, ok ? r.row1 - r.row0 : 0};
 }
 __device__ __forceinline__ Seq load_seq(const CachedArgs& a, int i) {
@@ -469,7 +469,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       const int p = window + lane;
       int s = p < pages ? row[p] : -1;
       if (p < pages && !page_fits(s, a.num_pages)) {
-        atomicExch(a.err, kDevErrBadPage);
+        report_bad_index(a.err, kDevErrBadPage);
         s = -1;
       }
       return s;

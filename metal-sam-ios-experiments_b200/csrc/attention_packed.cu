@@ -164,7 +164,7 @@ struct Finder {
     r0 = a.cu[i];
     const int r1 = a.cu[i + 1];
     if (!rows_fit(r0, r1, a.rows)) {
-      atomicExch(a.err, kDevErrBadLengths);
+      report_bad_index(a.err, kDevErrBadLengths);
       r0 = 0;
       return 0;
     }

@@ -34,6 +34,10 @@ enum DevErr : int {
   kDevErrBadPage = 0x203,     // a page number of a page table
 };
 
+// An index is out of range. A wait that ran out stays reported: its kernel's
+// results are missing, not skipped.
+__device__ __forceinline__ void report_bad_index(int* err, int code) { atomicCAS(err, 0, code); }
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }

@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(THREADS, 4) kv_append_kernel(const AppendArgs 
   const int row0 = a.cu ? a.cu[seq] : seq;
   const int row1 = a.cu ? a.cu[seq + 1] : seq + 1;
   if (!tokens_fit(row0, row1, a.rows, a.max_new, len, a.table_stride, a.page_shift)) {
-    if (threadIdx.x == 0) atomicExch(a.err, kDevErrBadLengths);
+    if (threadIdx.x == 0) report_bad_index(a.err, kDevErrBadLengths);
     return;
   }
   const int fresh = row1 - row0;
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(THREADS, 4) kv_append_kernel(const AppendArgs 
   }
   // the page's number is first needed here: it travels with the rows
   if (!page_fits(slot, a.num_pages)) {
-    if (threadIdx.x == 0) atomicExch(a.err, kDevErrBadPage);
+    if (threadIdx.x == 0) report_bad_index(a.err, kDevErrBadPage);
     return;
   }
 #pragma unroll

@@ -432,3 +432,29 @@ def test_projection_rows_go_in_as_they_lie(ctx, sam3, oracle):
     check_packed(ctx.download(do, (rows, heads, dim), np.uint16), q, k, v, cu, "f16", True, 0.125)
     check_cached(ctx.download(dc_out, (rows, heads, dim), np.uint16), q, host, cu, table, lens, "f16", True, 0.125)
     dc.free()
+
+
+# ------------------------------------------------------------------ what is reported
+def test_a_bad_entry_does_not_hide_a_wait_that_ran_out(sam3):
+    with sam3.Context(0, **CFG) as ctx:
+        table, pages = tables(np.random.default_rng(53), [20], 16)
+        host = P.Cache(pages, 1, 16, 64)
+        dc = DeviceCache(ctx, sam3, host, 64)
+        bits, bad = ctx.upload(np.zeros((1, 64), np.uint16)), ctx.upload(np.array([5, 3], np.int32))
+        table, lens, o = ctx.upload(table), ctx.upload(np.array([1 << 29], np.int32)), ctx.alloc(128)
+        calls = (lambda: ctx.attention_packed(sam3.F16, bits, 64, bits, 64, bits, 64, bad, 1, 1, 1, 1, 64, 0.1, True, o, 64),
+                 lambda: ctx.kv_append(dc.c, sam3.F16, bits, 64, bits, 64, None, 1, 1, 1, table, 3, lens),
+                 lambda: ctx.attention_cached(dc.c, sam3.F16, bits, 64, None, 1, 1, 1, table, 3, lens, 1, 0.1, True, o, 64))
+        for call in calls:  # each by itself
+            call()
+            with pytest.raises(sam3.SAM3Error) as e:
+                ctx.sync()
+            assert e.value.status == sam3.ERR_INVALID_ARG
+        ctx.selftest_wait_timeout()
+        for call in calls:
+            call()
+        with pytest.raises(sam3.SAM3Error) as e:
+            ctx.sync()
+        assert e.value.status == sam3.ERR_TIMEOUT
+        ctx.sync()
+        dc.free()
