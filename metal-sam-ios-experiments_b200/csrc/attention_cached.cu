@@ -59,8 +59,8 @@
 // the join; 64 contexts of 33 to 4096 tokens, one new token each, pages of 64: 30
 // us for 114 MB, where plan, first loads, and the end and join of items that
 // are cut cost about 10. 8 contexts of 5200 to 5500 tokens, 1 to 8 new tokens, 16
-// heads on 4 of 64, pages of 32: 23.8 us, bound by the 32 rows' terms, which read
-// the cache twice. One context of 77 tokens: 7.4 us, latency from the lengths to
+// heads on 4 of 64, pages of 32: 24.2 us, bound by the 32 rows' terms, which read
+// the cache twice. One context of 77 tokens: 6.8 us, latency from the lengths to
 // the result. (With the codes unpacked by the threads and fed to mma.sync the
 // four took 115, 57, 25 and 7.8 us.) Pages of 16 tokens with head_dim 64 cost
 // a long context 28 % more than larger ones: a TMA box of 1 KB each.
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   // Each warp plans for itself (no barrier): lane l gets the costs of the 32
   // sequences from 32 l on, as single tiles and as units of UNIT_TILES.
   // (Whole lines of lengths at a time: with 32 sequences in a row to each lane the
-  // plan of 1000 took 25 us.)
+  // plan of 1000 took 25 us, and a single sequence's call 0.3 us less.)
   const int m = (a.n_seqs + 31) / 32;
   auto cost_of = [&](const Seq& s, bool units) {
     if (s.fresh == 0) return 0;
@@ -1255,7 +1255,8 @@ sam3_status_t pick_rows(sam3_ctx_t* ctx, const CUtensorMap& mk, const CUtensorMa
   if (rows <= 8) return launch_cached<D, 8, BF>(ctx, mk, mv, a, capacity);
   // More rows read the cache again for each 16. (32 at a time for head_dim 128: a
   // thread holds 32 scores and spills, 77 against 39 us at 16 contexts of 4000 and
-  // 32 rows. 8 at a time: 46 us, and 29.6 against 27.4 at 16 rows.)
+  // 32 rows. 8 at a time: 46 us, and 29.6 against 27.4 at 16 rows. At head_dim 64 a
+  // thread holds 32 scores with 16 rows, of two tokens, and spills 68 bytes.)
   return launch_cached<D, 16, BF>(ctx, mk, mv, a, capacity);
 }
 

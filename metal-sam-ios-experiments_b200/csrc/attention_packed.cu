@@ -61,7 +61,7 @@
 // holds it to 1070. Tried and no faster at head_dim 128: P told in two parts
 // (96 + 32 keys 446, 64 + 64 449 against 444 us), K and V looked at between P V
 // and Q K^T (453), an issuer that polls for whatever is ready, a part of the
-// exponentials as polynomials.
+// exponentials as polynomials (the last two while a lone lane still issued).
 #include <algorithm>
 
 #include "common.cuh"

@@ -20,10 +20,11 @@
 // the rounding, so each is read once. Measured: 8 prompts of 8192 tokens (8
 // heads of 128, pages of 128) 65 us, 6.2 TB/s, 94 % of a copy's rate (89 us with
 // two CTAs per SM and pages before heads in the grid); four images' tokens
-// (10,410 rows, 16 heads of 64, pages of 16) 14.2 us, 4.5 TB/s: the
+// (10,410 rows, 16 heads of 64, pages of 16) 13.6 us, 4.7 TB/s: the
 // same chain of loads at the begin and the end is a larger part of it. One token
-// each of 64 sequences: 5.4 us, a launch, three dependent loads (length, page,
-// scale) and a store.
+// each of 64 sequences: 4.9 us, a launch, three dependent loads (length, page,
+// scale) and a store. Four CTAs per SM leave 64 registers a thread, and 12 to 84
+// bytes spill; three do without (4 bytes at most) and take 69.3, 14.4 and 4.9 us.
 #include <algorithm>
 
 #include "common.cuh"
