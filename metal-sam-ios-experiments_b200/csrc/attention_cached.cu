@@ -17,8 +17,8 @@
 // A row of Q takes three columns, the terms of an exact split of an 11-bit
 // number into e4m3 numbers: y = t0 + t1/16 + t2/256, each term the rounding
 // (4 bits, to nearest) of what is left. fp16 and bf16 queries (scaled by a
-// power of two to at most 256) are represented exactly down to 2^-6, smaller
-// elements to within 2^-18, 2^-26 of the row's largest.
+// power of two, the largest to [128, 256)) are represented exactly down to 2^-6,
+// smaller elements to within 2^-18, 2^-25 of the row's largest.
 // A row's weights p are rounded to fp16 (half a step of 2^-11) and take four
 // columns, e5m2 numbers: p = t0 + t1/8 + t2/64 + t3/512, each term the three
 // leading bits of what is left. e5m2 is fp16's upper byte, so the split is exact
@@ -27,10 +27,11 @@
 // below to within 2^-37. (Three e4m3 terms end 2^-23 below the largest: of a
 // row with one heavy key and 130,000 light ones that hold a fifth of the sum,
 // 5 % of the light ones' share went. The fourth term costs 4 % at 16 rows of
-// head_dim 64, 2 % at 16 of 128 and nothing with fewer.) Products are exact and sums fp32. For
-// head_dim 64 a column serves one of the line's two tokens: Q's other half is
-// zero, and of O^T only the half of the column's token is used (the tensor
-// cores have room: an MMA is bound by its 128-row operand up to 64 columns).
+// head_dim 64, 2 % at 16 of 128 and nothing with fewer.) Products are exact and
+// sums fp32. For head_dim 64 a column serves one of the line's two tokens: Q's
+// other half is zero, and of O^T only the half of the column's token is used (the
+// tensor cores have room: an MMA is bound by its 128-row operand up to 64
+// columns).
 // 0 * NaN is NaN, so a line's other token must not be a NaN code that the row
 // does not see: warp 3 looks through the K lines where that can be, the odd
 // token behind a sequence's end and the newest tokens, before the MMA.

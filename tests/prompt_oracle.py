@@ -124,12 +124,11 @@ def attend(q, k, v, scale, first, dtype, p_dtype, vmax=None, least=2.0 ** -25):
       - each weight is rounded once before the product: u_p A, and weights that
         fall below fp16's normal numbers by half a subnormal step each. With the
         running maximum at most 2^8 below the true one this is n 2^-25 max|v|
-        (packed; least: what a weight's half step is instead). Cached: a weight is 2^6 at the maximum M of x + log2(vs) and is
-        kept to within 2^-18 below 2^-6 (three e4m3 terms), so n weights are off
-        by n 2^-18 448 in sum; the token that set M adds 2^6 / vs to the row sum:
-        n 2^-24 448 max(vs) (vmax = max(vs)). Queries: each is kept to within
-        2^-18 of a row scaled to [128, 256), 2^-25 of its largest element, a
-        score to within d 2^-25 max|q| max|k| scale;
+        (packed; least: what a weight's half step is instead). Cached: n 2^-24 448
+        max(vs) (vmax = max(vs)) for weights that are held to within 2^-24 of the
+        largest, wider than the kernel needs: attend_codes has its own bound.
+        Queries: each is kept to within 2^-18 of a row scaled to [128, 256), 2^-25
+        of its largest element, a score to within d 2^-25 max|q| max|k| scale;
       - a score is a sum of d products in fp32, and its exponential is good to
         2^-22, in numerator and denominator: 2 (d + 4) 2^-24 |q| |k| scale + 2^-21;
       - sums over n weights in fp32: n 2^-24 each, above and below.
@@ -171,7 +170,8 @@ def attend_codes(q, kc, ks, vc, vs, scale, first, dtype):
         a maximum that moved scales earlier errors down): 2^-11 of each weight,
         and half a subnormal step, 2^-25, of each P_j below fp16's normal
         numbers: 2^-37 max_j(p_j vs_j) sum_j |vc_j| in the result;
-      - a query element is held to within 2^-26 of its row's largest;
+      - a query element is held to within 2^-25 of its row's largest (2^-18 of a
+        row scaled to [128, 256));
       - the tensor cores may cut each sum's last bit: n 2^-23 sum_j p_j |v_j|;
         a thread's share of the row sum has n / 64 terms, then 64 at most.
     """
@@ -189,7 +189,7 @@ def attend_codes(q, kc, ks, vc, vs, scale, first, dtype):
         p /= p.sum(1, keepdims=True)
         o[:, h] = p @ v
         a = p @ np.abs(v)
-        ds = 2 * ((d + 4) * 2.0 ** -24 * size + 2.0 ** -26 * part) + 2.0 ** -21
+        ds = 2 * ((d + 4) * 2.0 ** -24 * size + 2.0 ** -25 * part) + 2.0 ** -21
         rel = U["f16"] + ds + n * 2.0 ** -23 + (n / 64 + 64) * 2.0 ** -24
         small = 2.0 ** -37 * (p * vs[:, h // g]).max(1)[:, None] * (seen @ np.abs(vc[:, h // g]))
         tol[:, h] = U[dtype] * np.abs(o[:, h]) + TINY[dtype] + (1 + U[dtype]) * (rel[:, None] * a + small)
